@@ -146,6 +146,16 @@ _SIGNATURES = {
                                      _p, _p, _p, _p, _p], _int),
     "miq_adaround_linear_bwd_adam_i16": ([_p, _p, _p, _p, _i64, _i64, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _p, _p, _flt, _flt,
                                           _dbl, _dbl, _dbl, _dbl, _dbl, _dbl, _int, _p, _p], _int),
+    "miq_layer_norm_bwd_workspace_bytes": ([_i64, _i64], _i64),
+    "miq_layer_norm_fwd_f32": ([_p, _p, _p, _i64, _i64, _flt, _p, _p, _p, _p], _int),
+    "miq_layer_norm_fwd_bf16": ([_p, _p, _p, _i64, _i64, _flt, _p, _p, _p, _p], _int),
+    "miq_layer_norm_bwd_f32": ([_p, _p, _p, _p, _p, _i64, _i64, _p, _p, _p, _p, _p], _int),
+    "miq_layer_norm_bwd_bf16": ([_p, _p, _p, _p, _p, _i64, _i64, _p, _p, _p, _p, _p], _int),
+    "miq_linear_workspace_bytes": ([_i64, _i64, _i64, _int, _int, _int], _i64),
+    "miq_linear_fwd_f32": ([_p, _p, _p, _p, _i64, _i64, _i64, _int, _p, _p, _p, _i64, _p], _int),
+    "miq_linear_fwd_bf16": ([_p, _p, _p, _p, _i64, _i64, _i64, _int, _p, _p, _p, _i64, _p], _int),
+    "miq_linear_bwd_f32": ([_p, _p, _p, _p, _i64, _i64, _i64, _int, _p, _p, _p, _p, _i64, _p], _int),
+    "miq_linear_bwd_bf16": ([_p, _p, _p, _p, _i64, _i64, _i64, _int, _p, _p, _p, _p, _i64, _p], _int),
 }
 
 # Entry points declared in include/miq.h; the loader insists on every one of them.

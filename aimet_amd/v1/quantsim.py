@@ -69,7 +69,8 @@ def _op_type(module: nn.Module) -> str:
     for classes, name in _OP_TYPES:
         if isinstance(module, classes):
             return name
-    return type(module).__name__
+    # modules of this package that are an op together with what follows it say which
+    return getattr(module, "_quantsim_op_type", None) or type(module).__name__
 
 
 def _declared_inputs(module: nn.Module) -> int:
@@ -429,6 +430,8 @@ class QuantizationSimModel:
                 module = rec["module"]
                 if isinstance(module, nn.ConvTranspose2d) and module.groups != 1:
                     continue
+                if getattr(module, "_quantsim_op_type", None):
+                    continue                      # an activation or a residual lies between
                 reader = only_consumer(rec)
                 if reader is not None and reader["type"] == "BatchNormalization":
                     foldable[reader["name"]] = rec

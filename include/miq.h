@@ -10,7 +10,8 @@
  *
  * Each declaration names the reference interface it replaces (paths relative to the reference root;
  * DLQ = ModelOptimizations/DlQuantization, TSRC = TrainingExtensions/torch/src,
- * TORCH = TrainingExtensions/torch/src/python/aimet_torch).
+ * TORCH = TrainingExtensions/torch/src/python/aimet_torch,
+ * COMMON = TrainingExtensions/common/src/python/aimet_common).
  */
 #ifndef MIQ_H
 #define MIQ_H
@@ -701,6 +702,59 @@ int miq_v2_sqnr_search_f32(const float* hist, const float* minmax, int64_t num_h
 int64_t miq_column_error_splits(int64_t blocks, int64_t rows, int64_t cols);
 int miq_column_error_f32(const float* a, const float* b, int64_t blocks, int64_t rows, int64_t cols, int kind,
                          int64_t splits, float* partial, void* stream);
+
+/* ---------------------------------------------------------------------------------------------------------------
+ * Layer norm over rows of `width` values (contiguous), and its backward pass.  The reference quantizes nn.LayerNorm as
+ * a leaf module (TORCH/v2/nn/true_quant.py and the "LayerNormalization" op type) and leaves its arithmetic to torch.
+ *   m = mean(x), v = mean((x - m)^2), r = 1 / sqrt(v + eps), xhat = (x - m) r, y = xhat weight + bias
+ *   gw = grad weight, dx = r (gw - mean(gw) - xhat mean(gw xhat)), dweight = sum grad xhat, dbias = sum grad
+ * float32 arithmetic, one rounding to bfloat16 at the end.  weight and bias (each may be NULL: 1 and 0) have x's type.
+ * mean, rstd: float[rows] each, written by the forward pass for the backward pass; both NULL where none follows.
+ * dx, dweight, dbias may each be NULL where that gradient is not wanted.  With rows = 0, dweight and dbias are zeros.
+ * The sums of dweight and dbias are formed in an order that the shape alone decides.
+ * workspace: miq_layer_norm_bwd_workspace_bytes() bytes, needed for dweight and dbias.  out == in is not allowed. */
+int64_t miq_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t width);
+int miq_layer_norm_fwd_f32(const float* x, const float* weight, const float* bias, int64_t rows, int64_t width,
+                           float eps, float* y, float* mean, float* rstd, void* stream);
+int miq_layer_norm_fwd_bf16(const uint16_t* x, const uint16_t* weight, const uint16_t* bias, int64_t rows,
+                            int64_t width, float eps, uint16_t* y, float* mean, float* rstd, void* stream);
+int miq_layer_norm_bwd_f32(const float* x, const float* grad, const float* weight, const float* mean,
+                           const float* rstd, int64_t rows, int64_t width, float* dx, float* dweight, float* dbias,
+                           void* workspace, void* stream);
+int miq_layer_norm_bwd_bf16(const uint16_t* x, const uint16_t* grad, const uint16_t* weight, const float* mean,
+                            const float* rstd, int64_t rows, int64_t width, uint16_t* dx, uint16_t* dweight,
+                            uint16_t* dbias, void* workspace, void* stream);
+
+/* ---------------------------------------------------------------------------------------------------------------
+ * Matrix product with bias, activation and residual in its epilogue, and its backward pass: one supergroup
+ * ([Gemm, Relu] and the like; COMMON/quantsim_config/default_config.json) as one call.
+ *   z = x weight^T + bias, y = act(z) + residual        x [rows, in], weight [out, in], bias [out], y, residual [rows, out]
+ *   dz = grad act'(z), dx = dz weight, dweight = dz^T x, dbias = sum over rows of dz  (the residual's gradient is grad)
+ * All tensors contiguous and of one type.  Sums are float32; z is rounded nowhere on its way to y, and y once.
+ * bias and residual may be NULL.  saved (NULL where no backward pass follows, or for MIQ_ACT_NONE): what the backward
+ * pass needs of z, [rows, out], float for the f32 entry points and half for the bf16 ones.  dx, dweight, dbias may each
+ * be NULL where that gradient is not wanted.
+ * workspace: miq_linear_workspace_bytes() bytes, 256-byte aligned (may be NULL where that is 0); nothing in it outlives
+ * the call on its stream.  out == in is not allowed. */
+#define MIQ_ACT_NONE 0
+#define MIQ_ACT_RELU 1
+#define MIQ_ACT_SILU 2
+#define MIQ_ACT_GELU 3      /* z Phi(z) */
+#define MIQ_ACT_GELU_TANH 4 /* z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2 */
+int64_t miq_linear_workspace_bytes(int64_t rows, int64_t in_features, int64_t out_features, int activation, int bf16,
+                                   int backward);
+int miq_linear_fwd_f32(const float* x, const float* weight, const float* bias, const float* residual, int64_t rows,
+                       int64_t in_features, int64_t out_features, int activation, float* y, float* saved,
+                       void* workspace, int64_t workspace_bytes, void* stream);
+int miq_linear_fwd_bf16(const uint16_t* x, const uint16_t* weight, const uint16_t* bias, const uint16_t* residual,
+                        int64_t rows, int64_t in_features, int64_t out_features, int activation, uint16_t* y,
+                        uint16_t* saved, void* workspace, int64_t workspace_bytes, void* stream);
+int miq_linear_bwd_f32(const float* grad, const float* saved, const float* x, const float* weight, int64_t rows,
+                       int64_t in_features, int64_t out_features, int activation, float* dx, float* dweight,
+                       float* dbias, void* workspace, int64_t workspace_bytes, void* stream);
+int miq_linear_bwd_bf16(const uint16_t* grad, const uint16_t* saved, const uint16_t* x, const uint16_t* weight,
+                        int64_t rows, int64_t in_features, int64_t out_features, int activation, uint16_t* dx,
+                        uint16_t* dweight, uint16_t* dbias, void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,72 @@
+"""Arguments that the layer norm and linear entry points refuse, and their workspace sizes, on the host: every check
+comes before the first use of the GPU."""
+import ctypes
+
+import pytest
+
+P = ctypes.c_void_p(256)         # stands for a device pointer; never read
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from aimet_amd._lib import lib as l
+    return l
+
+
+def _refused(lib, rc, word):
+    assert rc == -1, rc
+    assert word.encode() in lib.miq_last_error(), lib.miq_last_error()
+
+
+@pytest.mark.parametrize("suffix", ["f32", "bf16"])
+def test_layer_norm_refusals(lib, suffix):
+    fwd, bwd = getattr(lib, "miq_layer_norm_fwd_" + suffix), getattr(lib, "miq_layer_norm_bwd_" + suffix)
+    _refused(lib, fwd(P, None, None, -1, 8, 1e-5, P, None, None, None), "rows")
+    _refused(lib, fwd(P, None, None, 4, 0, 1e-5, P, None, None, None), "width")
+    _refused(lib, fwd(P, None, None, 1 << 31, 8, 1e-5, P, None, None, None), "2^31")
+    _refused(lib, fwd(None, None, None, 4, 8, 1e-5, P, None, None, None), "null")
+    _refused(lib, fwd(P, None, None, 4, 8, 1e-5, None, None, None, None), "null")
+    _refused(lib, fwd(P, None, None, 4, 8, 1e-5, P, P, None, None), "together")
+    _refused(lib, bwd(P, P, None, None, P, 4, 8, P, None, None, None, None), "null")
+    _refused(lib, bwd(P, P, None, P, P, 4, 8, P, P, None, None, None), "workspace")
+    assert fwd(None, None, None, 0, 8, 1e-5, None, None, None, None) == 0
+    assert bwd(None, None, None, None, None, 0, 8, None, None, None, None, None) == 0
+    assert lib.miq_layer_norm_bwd_workspace_bytes(-1, 8) == 0
+    assert lib.miq_layer_norm_bwd_workspace_bytes(1000, 64) > 0
+
+
+@pytest.mark.parametrize("suffix", ["f32", "bf16"])
+def test_linear_refusals(lib, suffix):
+    fwd, bwd = getattr(lib, "miq_linear_fwd_" + suffix), getattr(lib, "miq_linear_bwd_" + suffix)
+    big = 1 << 40
+    _refused(lib, fwd(P, P, None, None, -1, 8, 8, 0, P, None, P, big, None), "negative")
+    _refused(lib, fwd(P, P, None, None, 1 << 31, 8, 8, 0, P, None, P, big, None), "2^31")
+    _refused(lib, fwd(P, P, None, None, 4, 8, 8, 5, P, None, P, big, None), "activation")
+    _refused(lib, fwd(None, P, None, None, 4, 8, 8, 0, P, None, P, big, None), "null")
+    _refused(lib, fwd(P, P, None, None, 4, 8, 8, 0, None, None, P, big, None), "null")
+    _refused(lib, bwd(P, None, P, P, 4, 8, 8, 3, P, P, P, P, big, None), "null")            # saved is missing
+    _refused(lib, bwd(P, None, None, P, 4, 8, 8, 0, P, P, P, P, big, None), "x")
+    _refused(lib, bwd(P, None, P, None, 4, 8, 8, 0, P, P, P, P, big, None), "weight")
+    _refused(lib, bwd(P, P, P, P, 4, 8, 8, 3, P, P, P, P, 0, None), "workspace")
+    for rows, n_in, n_out in ((1, 64, 64), (300, 1000, 77), (5000, 512, 4096)):
+        need = lib.miq_linear_workspace_bytes(rows, n_in, n_out, 3, int(suffix == "bf16"), 0)
+        if need:
+            _refused(lib, fwd(P, P, None, None, rows, n_in, n_out, 3, P, None, P, need - 1, None), "workspace")
+    assert fwd(None, None, None, None, 0, 8, 8, 0, None, None, None, 0, None) == 0
+    assert lib.miq_linear_workspace_bytes(-1, 8, 8, 0, 0, 1) == 0
+
+
+def test_functions_refuse_before_any_launch():
+    import torch
+    from aimet_amd.v2.nn import fused
+    x, w = torch.zeros(4, 8), torch.zeros(6, 8)
+    for call in (lambda: fused.linear(x, w), lambda: fused.layer_norm(x, 8), lambda: fused.layer_norm(x, 7),
+                 lambda: fused.layer_norm(x, ()), lambda: fused.layer_norm(x, 8, torch.ones(7))):
+        with pytest.raises(RuntimeError):
+            call()
+    with pytest.raises(ValueError):
+        fused.linear(x, w, None, "swish")
+    with pytest.raises(ValueError):
+        fused.FusedLinear(8, 6, activation="swish")
+    with pytest.raises(ValueError):
+        fused.FusedLinear.from_linear(torch.nn.Linear(8, 6), "swish")

@@ -1,0 +1,682 @@
+"""Layer norm and the matrix product with bias, activation and residual (aimet_amd.v2.nn.fused), forward and backward,
+against float64.
+
+Tolerances are bounds on what rounding can do, formed element by element from the float64 values.  u = 2^-24 is half a
+step of float32, relative.  A float32 sum of n terms in any order is off by at most n u times the sum of the terms'
+magnitudes; where the kernels sum a row by 64 lanes and more, n / 64 + 16 stands for n.  Storing in bfloat16 adds 2^-8
+of the value.
+"""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+DTYPES = [torch.float32, torch.bfloat16]
+ACTIVATIONS = ["none", "relu", "silu", "gelu", "gelu_tanh"]
+
+
+@pytest.fixture(scope="module")
+def fused():
+    from aimet_amd.v2.nn import fused as f
+    return f
+
+
+def step_of(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def randn(*shape, dtype=torch.float32, seed=0, scale=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(*shape, generator=g, device="cuda") * scale).to(dtype)
+
+
+def assert_within(got, want, tol, what):
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    off = (got.double() - want).abs() - tol
+    off = torch.where(torch.isnan(want) & torch.isnan(got), torch.full_like(off, -1.0), off)
+    if off.numel():
+        worst = off.max().item()
+        assert worst <= 0, f"{what}: {worst:.3g} past the bound, {int((off > 0).sum())} of {off.numel()} elements"
+
+
+# ----------------------------------------------------------------------------------------------------- layer norm
+def norm_oracle(x, w, b, eps, g):
+    """y, dx, dw, db in float64 and their bounds (without the storage rounding)."""
+    d = x.shape[1]
+    x, g = x.double(), g.double()
+    w = torch.ones(d, dtype=torch.float64, device=x.device) if w is None else w.double()
+    b = torch.zeros(d, dtype=torch.float64, device=x.device) if b is None else b.double()
+    n = d / 64 + 16
+    m = x.mean(1, keepdim=True)
+    c = x - m
+    r = 1 / torch.sqrt((c * c).mean(1, keepdim=True) + eps)
+    h = c * r
+    y = h * w + b
+    # xhat: the mean is off by n u mean|x|, the rest by a few roundings and half the relative error of the variance
+    eh = U * ((n + 4) * r * x.abs().mean(1, keepdim=True) + (n + 8) * h.abs())
+    # a shifted mean moves the variance by its square: (n u mean|x|)^2 r^2 relative, on every value
+    eh = eh + h.abs() * ((n + 4) * U * r * x.abs().mean(1, keepdim=True)) ** 2
+    ty = eh * w.abs() + 4 * U * ((h * w).abs() + b.abs())
+    gw = g * w
+    m1, m2 = gw.mean(1, keepdim=True), (gw * h).mean(1, keepdim=True)
+    dx = r * (gw - m1 - h * m2)
+    parts = gw.abs() + gw.abs().mean(1, keepdim=True) + h.abs() * (gw * h).abs().mean(1, keepdim=True)
+    tdx = r * (U * (n + 8) * parts + eh * m2.abs() + h.abs() * (gw.abs() * eh).mean(1, keepdim=True))
+    # r itself: relative error of half the variance's, and the shift of the mean
+    tdx = tdx + r * parts * ((n + 8) * U + ((n + 4) * U * r * x.abs().mean(1, keepdim=True)) ** 2)
+    rows = x.shape[0]
+    dw, db = (g * h).sum(0), g.sum(0)
+    tdw = (rows + 2) * U * (g * h).abs().sum(0) + (g.abs() * eh).sum(0)
+    tdb = (rows + 1) * U * g.abs().sum(0)
+    return (y, dx, dw, db), (ty, tdx, tdw, tdb)
+
+
+def check_norm(fused, x, w, b, g, eps=1e-5):
+    dtype = x.dtype
+    leaves = [None if t is None else t.clone().requires_grad_() for t in (x, w, b)]
+    y = fused.layer_norm(leaves[0], (x.shape[1],), leaves[1], leaves[2], eps)
+    assert y.dtype == dtype
+    with torch.no_grad():
+        assert torch.equal(y, fused.layer_norm(x, x.shape[1], w, b, eps))      # the same values without autograd
+    wanted = [t for t in leaves if t is not None]
+    grads = dict(zip([id(t) for t in wanted], torch.autograd.grad(y, wanted, g)))
+    want, tol = norm_oracle(x, w, b, eps, g)
+    got = [y] + [None if t is None else grads[id(t)] for t in leaves]
+    for name, a, e, t in zip(("y", "dx", "dweight", "dbias"), got, want, tol):
+        if a is not None:
+            assert a.dtype == dtype
+            store = step_of(dtype) * (e.abs() + t) if dtype != torch.float32 else 0
+            assert_within(a.detach(), e, t + store, name)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,width", [(1, 1), (1, 2), (1, 64), (3, 7), (5, 1001), (17, 1024), (2, 4096), (1, 16384),
+                                        (300, 100), (4, 20000), (3, 40001), (1030, 65), (2100, 512), (33, 8200)])
+def test_layer_norm(fused, dtype, rows, width):
+    x = randn(rows, width, dtype=dtype, seed=1)
+    w, b = (1 + 0.2 * randn(width, seed=2)).to(dtype), randn(width, dtype=dtype, seed=3, scale=0.1)
+    check_norm(fused, x, w, b, randn(rows, width, dtype=dtype, seed=4))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("with_weight,with_bias", [(False, False), (True, False), (False, True)])
+def test_layer_norm_without_parameters(fused, dtype, with_weight, with_bias):
+    x, g = randn(37, 260, dtype=dtype, seed=1), randn(37, 260, dtype=dtype, seed=2)
+    w = randn(260, dtype=dtype, seed=3) if with_weight else None
+    b = randn(260, dtype=dtype, seed=4) if with_bias else None
+    check_norm(fused, x, w, b, g)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_layer_norm_of_rows_far_from_zero_and_of_outliers(fused, dtype):
+    """Variance from differences to the mean, not from E[x^2] - m^2: a mean of 1000 standard deviations survives."""
+    x = randn(6, 768, seed=1)
+    x[0] += 1000
+    x[1] *= 1e-4
+    x[2, 5] = 3e4
+    x[3] = 7.25                                             # no variance at all: xhat is 0
+    x[4] *= 1e6
+    check_norm(fused, x.to(dtype), randn(768, dtype=dtype, seed=2), randn(768, dtype=dtype, seed=3),
+               randn(6, 768, dtype=dtype, seed=4))
+
+
+def test_layer_norm_keeps_bad_rows_to_themselves(fused):
+    for dtype in DTYPES:
+        x = randn(9, 300, dtype=dtype, seed=1)
+        good = fused.layer_norm(x, 300)
+        x[2, 7], x[4, 0], x[6, 299] = float("nan"), float("inf"), -float("inf")
+        y = fused.layer_norm(x, 300)
+        bad = [2, 4, 6]
+        assert torch.isnan(y[bad]).all()
+        rest = [i for i in range(9) if i not in bad]
+        assert torch.equal(y[rest], good[rest])
+
+
+def test_layer_norm_shapes_strides_and_alignment(fused):
+    for dtype in DTYPES:
+        for width in (24, 25, 1024):
+            # trailing dimensions, a transposed input, storage that starts one element into an allocation, a grad of
+            # stride 0
+            base = randn(4 * 6 * width + 1, dtype=dtype, seed=width)
+            x = base[1:].view(4, 6, width)
+            want = fused.layer_norm(x.clone(), (6, width))
+            assert want.shape == x.shape
+            assert torch.equal(fused.layer_norm(x, (6, width)), want)
+            t = randn(width, 40, dtype=dtype, seed=5).t()
+            assert not t.is_contiguous() or width == 1
+            assert torch.equal(fused.layer_norm(t, width), fused.layer_norm(t.contiguous(), width))
+            w0 = randn(width + 3, dtype=dtype, seed=6)
+            leaf = x.clone().requires_grad_()
+            w = w0[3:].clone().requires_grad_()
+            y = fused.layer_norm(leaf, width, w0[3:])
+            assert torch.equal(y, fused.layer_norm(leaf, width, w))
+            y2 = fused.layer_norm(leaf, width, w)
+            one = torch.ones((), dtype=dtype, device="cuda")
+            a = torch.autograd.grad(y2, [leaf, w], one.expand_as(y2), retain_graph=True)
+            b = torch.autograd.grad(y2, [leaf, w], torch.ones_like(y2))
+            assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_layer_norm_without_rows(fused):
+    for dtype in DTYPES:
+        x = torch.empty(0, 48, dtype=dtype, device="cuda", requires_grad=True)
+        w = torch.ones(48, dtype=dtype, device="cuda", requires_grad=True)
+        b = torch.ones(48, dtype=dtype, device="cuda", requires_grad=True)
+        y = fused.layer_norm(x, 48, w, b)
+        assert y.shape == (0, 48)
+        dx, dw, db = torch.autograd.grad(y, [x, w, b], torch.empty_like(y))
+        assert dx.shape == (0, 48) and not dw.any() and not db.any()
+
+
+def test_layer_norm_gradient_against_differences(fused):
+    """Directional central differences of the float64 forward, with a step whose truncation and rounding are far below
+    the bound of the float32 gradient."""
+    x, w, b, g = randn(5, 33, seed=1), randn(33, seed=2), randn(33, seed=3), randn(5, 33, seed=4)
+    leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+    grads = torch.autograd.grad(fused.layer_norm(leaves[0], 33, leaves[1], leaves[2]), leaves, g)
+    _, tol = norm_oracle(x, w, b, 1e-5, g)
+    for k in range(3):
+        v = randn(*leaves[k].shape, seed=10 + k).double()
+        side = []
+        for s in (1e-5, -1e-5):
+            p = [t.double() for t in (x, w, b)]
+            p[k] = p[k] + s * v
+            side.append((norm_oracle(*p, 1e-5, g)[0][0] * g.double()).sum())
+        want = (side[0] - side[1]) / 2e-5
+        bound = (tol[1 + k] * v.abs()).sum() + 1e-7 * (grads[k].double() * v).abs().sum()
+        assert abs((grads[k].double() * v).sum() - want) <= bound
+
+
+def test_layer_norm_offsets_past_32_bits(fused):
+    rows, width = 270000, 8200                                # 2.2e9 elements
+    x = torch.zeros(rows, width, dtype=torch.bfloat16, device="cuda")
+    tail = randn(3, width, dtype=torch.bfloat16, seed=1)
+    x[-3:] = tail
+    y = fused.layer_norm(x, width)
+    assert torch.equal(y[-3:], fused.layer_norm(tail, width)) and not y[-5].any()
+    del y
+    from aimet_amd import ops
+    _, stats = ops.layer_norm_fwd(x, width, want_stats=True)
+    dx, dw, _ = ops.layer_norm_bwd(x, x, width, None, stats, True, True, False)
+    _, s3 = ops.layer_norm_fwd(tail, width, want_stats=True)
+    dx3, dw3, _ = ops.layer_norm_bwd(tail, tail, width, None, s3, True, True, False)
+    assert torch.equal(dx[-3:], dx3)
+    want, tol = norm_oracle(tail, None, None, 1e-5, tail)
+    bound = tol[2] + 2 ** -8 * want[2].abs()                  # the other rows add zeros
+    assert_within(dw, want[2], bound, "dweight")
+    assert_within(dw3, want[2], bound, "dweight of the tail alone")
+
+
+# --------------------------------------------------------------------------------------------------------- linear
+def act64(z, kind):
+    f = torch.nn.functional
+    return {"none": lambda t: t, "relu": torch.relu, "silu": f.silu, "gelu": f.gelu,
+            "gelu_tanh": lambda t: f.gelu(t, approximate="tanh")}[kind](z)
+
+
+# |act'| <= 1.13 and |act''| <= 1.2 hold for every activation here (GELU: 1.129 at sqrt 2 and 0.798 at 0; its tanh form
+# and SiLU: below); ReLU has no second derivative away from 0, where its slope jumps by 1
+SLOPE, CURVE = 1.13, 1.2
+
+
+def linear_oracle(x, w, b, act, res, g):
+    """y, dx, dw, db in float64 and their bounds (without the storage rounding of the result)."""
+    dtype = x.dtype
+    x, w, g = x.double(), w.double(), g.double()
+    b = torch.zeros(w.shape[0], dtype=torch.float64, device=x.device) if b is None else b.double()
+    rows, k = x.shape
+    n = w.shape[0]
+    z = (x @ w.t() + b).requires_grad_()
+    y = act64(z, act)
+    slope, = torch.autograd.grad(y.sum(), z)
+    z, y = z.detach(), y.detach()
+    r = torch.zeros_like(y) if res is None else res.double()
+    # the product: any order; float32 operands go in as two halves of 11 bits, off by 2^-22 relative together
+    tz = (k + 6) * U * (x.abs() @ w.abs().t()) + 2 * U * (z.abs() + b.abs())
+    # the activation: 2^-21 of |z| + 1 covers the 1 ulp exponential, reciprocal and error function and their products
+    ta = 0 if act in ("none", "relu") else 2.0 ** -21 * (z.abs() + 1)
+    ty = SLOPE * tz + ta + U * (y.abs() + r.abs())
+    # derivative at the z that was kept: float32, or a half (2^-11 relative, at least half of 2^-24)
+    kept = tz if dtype == torch.float32 else tz + 2.0 ** -11 * z.abs() + 2.0 ** -25
+    if act == "none":
+        ts = torch.zeros_like(z)
+    elif act == "relu":
+        ts = (z.abs() <= tz).double()
+    else:
+        ts = CURVE * kept.clamp(max=1.0) + 2.0 ** -20 * (1 + z.abs())
+    dz = g * slope
+    tdz = g.abs() * ts + U * dz.abs()
+    if dtype != torch.float32 and act != "none":
+        tdz = tdz + step_of(dtype) * (dz.abs() + tdz)         # it goes through the matrix unit in bfloat16
+    dx, dw, db = dz @ w, dz.t() @ x, dz.sum(0)
+    tdx = tdz @ w.abs() + (n + 6) * U * (dz.abs() @ w.abs())
+    tdw = tdz.t() @ x.abs() + (rows + 6) * U * (dz.abs().t() @ x.abs())
+    tdb = tdz.sum(0) + (rows + 1) * U * dz.abs().sum(0)
+    return (y + r, dx, dw, db), (ty, tdx, tdw, tdb)
+
+
+def linear_case(rows, k, n, dtype, residual, seed=0, bias=True):
+    x = randn(rows, k, dtype=dtype, seed=seed + 1)
+    w = randn(n, k, dtype=dtype, seed=seed + 2, scale=1 / math.sqrt(max(k, 1)))
+    b = randn(n, dtype=dtype, seed=seed + 3) if bias else None
+    res = randn(rows, n, dtype=dtype, seed=seed + 4) if residual else None
+    return x, w, b, res, randn(rows, n, dtype=dtype, seed=seed + 5)
+
+
+def check_linear(fused, x, w, b, res, g, act):
+    dtype = x.dtype
+    named = {"x": x, "weight": w, "bias": b, "residual": res}
+    leaves = {k: v.clone().requires_grad_() for k, v in named.items() if v is not None}
+    y = fused.linear(leaves["x"], leaves["weight"], leaves.get("bias"), act, leaves.get("residual"))
+    assert y.dtype == dtype
+    with torch.no_grad():
+        assert torch.equal(y, fused.linear(x, w, b, act, res))
+    grads = dict(zip(leaves, torch.autograd.grad(y, list(leaves.values()), g)))
+    want, tol = linear_oracle(x, w, b, act, res, g)
+    got = (y.detach(), grads["x"], grads["weight"], grads.get("bias"))
+    for name, a, e, t in zip(("y", "dx", "dweight", "dbias"), got, want, tol):
+        if a is None:
+            continue
+        assert a.dtype == dtype
+        store = step_of(dtype) * (e.abs() + t) if dtype != torch.float32 else 0
+        assert_within(a, e, t + store, name)
+        if dtype == torch.float32 and act != "relu" and e.numel() >= 4096:
+            # rounding errors of random sign: 2 u sqrt(terms) of the values' norm, and a few u for the activation
+            terms = {"y": x.shape[1], "dx": w.shape[0], "dweight": x.shape[0], "dbias": x.shape[0]}[name]
+            first = 0 if name == "y" else x.shape[1]
+            assert (a.double() - e).norm() <= (2 * math.sqrt(terms + first) + 8) * U * e.norm(), name
+    if res is not None:
+        assert torch.equal(grads["residual"], g)
+
+
+SIZES = [(1, 1, 1), (1, 64, 64), (1, 4096, 1000), (2, 77, 33), (3, 1, 5), (5, 1001, 130), (16, 512, 256),
+         (17, 640, 96), (33, 200, 72), (64, 256, 512), (65, 264, 320), (130, 136, 100), (200, 1003, 515),
+         (257, 512, 300), (300, 64, 2049), (512, 1024, 768)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,k,n", SIZES)
+def test_linear(fused, dtype, rows, k, n):
+    check_linear(fused, *linear_case(rows, k, n, dtype, True), "gelu")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ACTIVATIONS)
+@pytest.mark.parametrize("rows,k,n", [(1, 96, 40), (50, 160, 136), (300, 328, 264)])
+def test_linear_activations(fused, dtype, act, rows, k, n):
+    check_linear(fused, *linear_case(rows, k, n, dtype, False), act)
+    check_linear(fused, *linear_case(rows, k, n, dtype, True, seed=50, bias=False), act)
+
+
+def test_linear_without_rows_or_features(fused):
+    for dtype in DTYPES:
+        for act in ("none", "silu"):
+            x = torch.empty(0, 24, dtype=dtype, device="cuda", requires_grad=True)
+            w = randn(40, 24, dtype=dtype).requires_grad_()
+            b = randn(40, dtype=dtype).requires_grad_()
+            y = fused.linear(x, w, b, act)
+            assert y.shape == (0, 40)
+            dx, dw, db = torch.autograd.grad(y, [x, w, b], torch.empty_like(y))
+            assert dx.shape == (0, 24) and not dw.any() and not db.any()
+            # no input features: the bias is all there is
+            x0, w0 = torch.empty(5, 0, dtype=dtype, device="cuda"), torch.empty(40, 0, dtype=dtype, device="cuda")
+            y = fused.linear(x0, w0, b.detach(), "none")
+            assert torch.equal(y, b.detach().expand(5, 40))
+
+
+def test_linear_keeps_bad_rows_to_themselves(fused):
+    """An infinity or a NaN in a row of x reaches that row of the output alone, as what float32 arithmetic makes of it."""
+    for dtype in DTYPES:
+        for rows in (7, 300):
+            x, w, b, _, _ = linear_case(rows, 200, 264, dtype, False)
+            good = fused.linear(x, w, b)
+            x[1, 3], x[2, 199], x[4, 0] = float("inf"), -float("inf"), float("nan")
+            y = fused.linear(x, w, b)
+            keep = [i for i in range(rows) if i not in (1, 2, 4)]
+            assert torch.equal(y[keep], good[keep])
+            assert torch.isnan(y[4]).all()
+            want = torch.where(w[:, 3] > 0, 1.0, -1.0)
+            assert torch.equal(y[1].float(), want * float("inf"))
+            assert torch.equal(y[2].float(), torch.where(w[:, 199] > 0, -1.0, 1.0) * float("inf"))
+
+
+@pytest.mark.parametrize("rows", [3, 40, 300])
+def test_linear_of_float32_far_from_one(fused, rows):
+    """Rows of very different magnitudes, values of very different magnitudes in a row, and the ends of the range."""
+    x, w, _, _, g = linear_case(rows, 256, 300, torch.float32, False)
+    x = x * torch.logspace(-30, 30, rows, device="cuda")[:, None]
+    w = w * torch.logspace(-4, 4, 300, device="cuda")[torch.randperm(300, device="cuda")][:, None]
+    x[:, ::7] *= 1e-3
+    check_linear(fused, x, w, None, None, g, "none")
+    with torch.no_grad():
+        big = torch.full((rows, 64), 3e38, device="cuda")
+        tiny = torch.full((72, 64), 1e-38, device="cuda")
+        y = fused.linear(big, tiny)
+        want = float(torch.tensor(3e38).double() * torch.tensor(1e-38).double() * 64)
+        assert (y.double() - want).abs().max() <= 70 * U * want
+        assert not fused.linear(torch.zeros(rows, 64, device="cuda"), tiny).any()
+
+
+def test_linear_shapes_strides_and_alignment(fused):
+    for dtype in DTYPES:
+        for k, n in ((64, 72), (65, 71), (256, 264)):
+            x, w, b, res, g = linear_case(130, k, n, dtype, True)
+            want = fused.linear(x, w, b, "silu", res)
+            assert torch.equal(fused.linear(x.view(2, 5, 13, k), w, b, "silu", res.view(2, 5, 13, n)).view(130, n), want)
+            assert torch.equal(fused.linear(x[3], w, b, "silu", res[3]), fused.linear(x[3:4], w, b, "silu", res[3:4])[0])
+
+            def shifted(t):
+                """The same values, one element into an allocation."""
+                flat = torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")[1:]
+                return flat.copy_(t.reshape(-1)).view(t.shape)
+            odd = [shifted(t).requires_grad_() for t in (x, w, b, res)]
+            even = [t.clone().requires_grad_() for t in (x, w, b, res)]
+            ya = fused.linear(odd[0], odd[1], odd[2], "silu", odd[3])
+            yb = fused.linear(even[0], even[1], even[2], "silu", even[3])
+            assert torch.equal(ya, want) and torch.equal(yb, want)
+            ga, gb = torch.autograd.grad(ya, odd, shifted(g)), torch.autograd.grad(yb, even, g)
+            assert all(torch.equal(p, q) for p, q in zip(ga, gb))
+            # transposed operands, a grad of stride 0
+            assert torch.equal(fused.linear(x.t().contiguous().t(), w.t().contiguous().t(), b, "silu", res), want)
+            y2 = fused.linear(even[0], even[1], even[2], "silu", even[3])
+            one = torch.ones((), dtype=dtype, device="cuda")
+            p = torch.autograd.grad(y2, even[:3], one.expand_as(y2), retain_graph=True)
+            q = torch.autograd.grad(y2, even[:3], torch.ones_like(y2))
+            assert all(torch.equal(i, j) for i, j in zip(p, q))
+
+
+def test_linear_results_do_not_change_from_run_to_run(fused):
+    for dtype in DTYPES:
+        x, w, b, res, g = linear_case(700, 520, 392, dtype, True)
+        first = None
+        for _ in range(3):
+            leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+            y = fused.linear(*leaves, "gelu", res)
+            out = [y, *torch.autograd.grad(y, leaves, g)]
+            first = first or out
+            assert all(torch.equal(p, q) for p, q in zip(first, out))
+
+
+def test_linear_some_gradients_only(fused):
+    x, w, b, res, g = linear_case(40, 96, 56, torch.float32, True)
+    leaves = [t.clone().requires_grad_() for t in (x, w, b, res)]
+    every = torch.autograd.grad(fused.linear(leaves[0], leaves[1], leaves[2], "gelu", leaves[3]), leaves, g)
+    for k in range(4):
+        some = [t.clone().requires_grad_(i == k) for i, t in enumerate((x, w, b, res))]
+        got, = torch.autograd.grad(fused.linear(some[0], some[1], some[2], "gelu", some[3]), some[k], g)
+        assert torch.equal(got, every[k])
+
+
+def test_linear_gradient_against_differences(fused):
+    x, w, b, res, g = linear_case(6, 20, 13, torch.float32, True)
+    for act in ("silu", "gelu", "gelu_tanh"):
+        leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+        grads = torch.autograd.grad(fused.linear(*leaves, act, res), leaves, g)
+        _, tol = linear_oracle(x, w, b, act, res, g)
+        for k in range(3):
+            v = randn(*leaves[k].shape, seed=20 + k).double()
+            side = []
+            for s in (1e-5, -1e-5):
+                p = [t.double() for t in (x, w, b)]
+                p[k] = p[k] + s * v
+                side.append((act64(p[0] @ p[1].t() + p[2], act) * g.double()).sum())
+            want = (side[0] - side[1]) / 2e-5
+            bound = (tol[1 + k] * v.abs()).sum() + 1e-7 * (grads[k].double() * v).abs().sum()
+            assert abs((grads[k].double() * v).sum() - want) <= bound, (act, k)
+
+
+def test_linear_offsets_past_32_bits(fused):
+    rows, n = 300000, 16000                                    # 4.8e9 outputs
+    x = torch.zeros(rows, 8, dtype=torch.bfloat16, device="cuda")
+    x[-2:] = randn(2, 8, dtype=torch.bfloat16, seed=1)
+    w = randn(n, 8, dtype=torch.bfloat16, seed=2)
+    y = fused.linear(x, w)
+    assert torch.equal(y[-2:], fused.linear(x[-2:].clone(), w)) and not y[-4].any()
+    dx, dw, db = _backward_of_itself(y, x, w)
+    assert torch.equal(db, y[-2:].float().sum(0).bfloat16())
+    assert not dx[:-2].any()
+
+
+def _backward_of_itself(y, x, w):
+    from aimet_amd import ops
+    return ops.linear_bwd(y, None, x, w, "none")
+
+
+# ------------------------------------------------------------------------------------------- streams, graphs, devices
+def test_on_a_side_stream(fused):
+    x, w, b, res, g = linear_case(200, 256, 264, torch.bfloat16, True)
+    want = fused.linear(fused.layer_norm(x, 256), w, b, "gelu", res)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = fused.linear(fused.layer_norm(x, 256), w, b, "gelu", res)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [4, 200])
+def test_captured_training_step(fused, dtype, rows):
+    """Forward and backward of norm -> linear in a graph, replayed with new inputs between eager work."""
+    x, w, b, res, g = linear_case(rows, 256, 264, dtype, True)
+    nw = randn(256, dtype=dtype, seed=9)
+    static = [t.clone().requires_grad_() for t in (x, nw, w, b, res)]
+
+    def step(t, grad):
+        y = fused.linear(fused.layer_norm(t[0], 256, t[1]), t[2], t[3], "gelu", t[4])
+        return [y.detach(), *torch.autograd.grad(y, t, grad)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(static, g)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()]
+    outs = []
+    for graph in graphs:                                       # two graphs, each with workspaces of its own
+        with torch.cuda.graph(graph):
+            outs.append(step(static, g))
+    for k in range(4):
+        with torch.no_grad():
+            for i, t in enumerate(static):
+                t.copy_(randn(*t.shape, dtype=dtype, seed=100 * k + i, scale=0.5))
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        want = step([t.detach().clone().requires_grad_() for t in static], g)
+        for out in outs:
+            assert all(torch.equal(p, q) for p, q in zip(out, want)), k
+
+
+def test_two_streams_at_once(fused):
+    """Calls that overlap share no scratch memory."""
+    cases = [linear_case(900, 512, 520, torch.float32, False, seed=s) for s in (1, 2)]
+    from aimet_amd import ops
+    want = []
+    for x, w, b, _, g in cases:
+        y, saved = ops.linear_fwd(x, w, b, "gelu", want_saved=True)
+        want.append((y, *ops.linear_bwd(g, saved, x, w, "gelu")))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for k, (x, w, b, _, g) in enumerate(cases):
+            with torch.cuda.stream(streams[k]):
+                y, saved = ops.linear_fwd(x, w, b, "gelu", want_saved=True)
+                got[k].append((y, *ops.linear_bwd(g, saved, x, w, "gelu")))
+    torch.cuda.synchronize()
+    for k in range(2):
+        for out in got[k]:
+            assert all(torch.equal(p, q) for p, q in zip(out, want[k]))
+
+
+# ------------------------------------------------------------------------------------------------------- refusals
+def test_refusals(fused):
+    x, w, b, res, _ = linear_case(4, 32, 24, torch.float32, True)
+    bad = [
+        lambda: fused.linear(x.double(), w.double()),                         # types
+        lambda: fused.linear(x.half(), w.half()),
+        lambda: fused.linear(x, w.bfloat16()),
+        lambda: fused.linear(x, w, b.bfloat16()),
+        lambda: fused.linear(x.cpu(), w.cpu()),                               # devices
+        lambda: fused.linear(x, w.cpu()),
+        lambda: fused.linear(x, w[:, :31]),                                   # shapes
+        lambda: fused.linear(x, w, b[:23]),
+        lambda: fused.linear(x, w, b, "none", res[:1]),                       # a residual is not broadcast
+        lambda: fused.linear(x, w[0]),
+        lambda: fused.layer_norm(x, 31),
+        lambda: fused.layer_norm(x, (4, 31)),
+        lambda: fused.layer_norm(x, 32, w[0, :31]),
+        lambda: fused.layer_norm(x, 32, w[0].bfloat16()),
+        lambda: fused.layer_norm(x.double(), 32),
+        lambda: fused.layer_norm(x.cpu(), 32),
+    ]
+    for k, call in enumerate(bad):
+        with pytest.raises(RuntimeError):
+            call()
+            pytest.fail(f"call {k} was not refused")
+    with pytest.raises(ValueError, match="activation"):
+        fused.linear(x, w, b, "swish")
+    # twice differentiable is not offered
+    leaf = x.clone().requires_grad_()
+    d, = torch.autograd.grad(fused.layer_norm(leaf, 32).square().sum(), leaf, create_graph=True)
+    with pytest.raises(RuntimeError):
+        d.sum().backward()
+
+
+# ------------------------------------------------------------------------------------------- modules and simulation
+class Block(torch.nn.Module):
+    """The MLP half of a transformer block, on the fused modules."""
+
+    def __init__(self, fused, width=64, hidden=160, activation="gelu"):
+        super().__init__()
+        self.norm = fused.FusedLayerNorm(width)
+        self.up = fused.FusedLinear(width, hidden, activation=activation)
+        self.down = fused.FusedLinear(hidden, width)
+
+    def forward(self, x):
+        return self.down(self.up(self.norm(x)), x)
+
+
+class TorchBlock(torch.nn.Module):
+    """The same block on torch's modules."""
+
+    def __init__(self, block):
+        super().__init__()
+        self.norm, self.up, self.down = block.norm, block.up, block.down
+        self.activation = block.up.activation
+
+    def forward(self, x):
+        f = torch.nn.functional
+        h = f.layer_norm(x, self.norm.normalized_shape, self.norm.weight, self.norm.bias, self.norm.eps)
+        return f.linear(act64(f.linear(h, self.up.weight, self.up.bias), self.activation), self.down.weight,
+                        self.down.bias) + x
+
+
+@pytest.mark.parametrize("activation", ["relu", "silu", "gelu", "gelu_tanh"])
+def test_block_trains_like_its_float64_form(fused, activation):
+    """Norm -> up + activation -> down + residual, forward and every gradient.  The bound is one for the chain: each of
+    the three operators adds errors of random sign of at most 2 u sqrt(terms) + 8 u of its result's norm, and the next
+    operators amplify them by no more than their condition, taken as 16."""
+    torch.manual_seed(0)
+    block = Block(fused, activation=activation).cuda()
+    x = randn(3, 50, 64, seed=1).requires_grad_()
+    g = randn(3, 50, 64, seed=2)
+    params = [x, *block.parameters()]
+    got = torch.autograd.grad(block(x), params, g)
+    ref = TorchBlock(block).cuda().double()
+    x64 = x.detach().double().requires_grad_()
+    want = torch.autograd.grad(ref(x64), [x64, *ref.parameters()], g.double())
+    for a, e in zip(got, want):
+        assert (a.double() - e).norm() <= 16 * 3 * (2 * math.sqrt(160 + 64) + 8) * U * e.norm()
+
+
+def test_modules_are_made_from_torch_modules_and_pickle(fused):
+    import copy
+    import pickle
+    torch.manual_seed(0)
+    lin, norm = torch.nn.Linear(24, 40).cuda(), torch.nn.LayerNorm(24).cuda()
+    f, n = fused.FusedLinear.from_linear(lin, "silu"), fused.FusedLayerNorm.from_layer_norm(norm)
+    assert f.weight is lin.weight and f.bias is lin.bias and n.weight is norm.weight
+    x = randn(7, 24, seed=3)
+    with torch.no_grad():
+        y, h = f(x), n(x)
+        assert torch.allclose(y, torch.nn.functional.silu(lin(x)), atol=1e-5)
+        assert torch.allclose(h, norm(x), atol=1e-5)
+        for m, want in ((f, y), (n, h)):
+            for other in (copy.deepcopy(m), pickle.loads(pickle.dumps(m))):
+                assert torch.equal(other(x), want)
+    assert set(f.state_dict()) == set(lin.state_dict()) and "silu" in repr(f)
+    none = fused.FusedLinear.from_linear(torch.nn.Linear(24, 40, bias=False).cuda())
+    assert none.bias is None and none(x).shape == (7, 40)
+
+
+def test_quantized_modules_quantize_around_the_kernels(fused):
+    """Quantizers placed by hand: the output is the quantizer of the fused product of quantized operands, to the bit."""
+    from aimet_amd.v2.nn import QuantizationMixin
+    from aimet_amd.v2.quantization.affine import QuantizeDequantize
+    torch.manual_seed(0)
+    q = QuantizationMixin.from_module(fused.FusedLinear(32, 48, activation="gelu").cuda())
+    assert isinstance(q, fused.QuantizedFusedLinear)
+    q.input_quantizers[0] = QuantizeDequantize((), 8, False).cuda()
+    q.output_quantizers[0] = QuantizeDequantize((), 8, False).cuda()
+    q.param_quantizers["weight"] = QuantizeDequantize((48, 1), 4, True).cuda()
+    x, r = randn(10, 32, seed=1), randn(10, 48, seed=2)
+    with torch.no_grad(), q.compute_encodings():
+        q(x, r)
+    leaf, res = x.clone().requires_grad_(), r.clone().requires_grad_()
+    y = q(leaf, res)
+    xq, wq = q.input_quantizers[0](leaf), q.param_quantizers["weight"](q.weight)
+    want = q.output_quantizers[0](fused.linear(xq, wq, q.bias, "gelu", res))
+    assert torch.equal(y, want)
+    g = randn(10, 48, seed=3)
+    wanted = [leaf, res, q.weight, q.bias]
+    for a, b in zip(torch.autograd.grad(y, wanted, g, retain_graph=True), torch.autograd.grad(want, wanted, g)):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("version", ["v1", "v2"])
+def test_simulation_of_a_fused_block(fused, version):
+    """Both simulation models take the block: one quantizer behind each fused module, per-channel weights, encodings by
+    calibration, a training step through them; as "Gemm" and "LayerNormalization" for the configuration."""
+    if version == "v1":
+        from aimet_amd.v1.quantsim import QuantizationSimModel
+    else:
+        from aimet_amd.v2.quantsim import QuantizationSimModel
+    torch.manual_seed(0)
+    block = Block(fused).cuda().eval()
+    x = randn(6, 64, seed=1)
+    config = {"defaults": {"ops": {"is_output_quantized": "True"},
+                           "params": {"is_quantized": "True", "is_symmetric": "True"},
+                           "strict_symmetric": "False", "per_channel_quantization": "True"},
+              "params": {"bias": {"is_quantized": "False"}},
+              "op_type": {"LayerNormalization": {"params": {"weight": {"is_quantized": "False"}},
+                                                 "per_channel_quantization": "False"}},
+              "supergroups": [], "model_input": {"is_input_quantized": "True"}, "model_output": {}}
+    sim = QuantizationSimModel(block, x, config_file=config)
+    sim.compute_encodings(lambda m, _: m(x), None)
+    with torch.no_grad():
+        want, got = block(x), sim.model(x)
+    assert 0 < (got - want).norm() < 0.05 * want.norm()
+    for name in ("up", "down"):
+        q = getattr(sim.model, name).param_quantizers["weight"]
+        assert (len(q.encoding) if version == "v1" else q.get_min().numel()) == getattr(block, name).out_features
+    leaf = x.clone().requires_grad_()
+    sim.model(leaf).square().mean().backward()
+    assert torch.isfinite(leaf.grad).all() and leaf.grad.any()
+
+
+def test_autocast(fused):
+    x, w, b, res, g = linear_case(20, 64, 48, torch.float32, True)
+    leaves = [t.clone().requires_grad_() for t in (x, w, b, res)]
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        y = fused.linear(leaves[0], leaves[1], leaves[2], "gelu", leaves[3])
+        h = fused.layer_norm(x.bfloat16(), 64, w[0])
+    assert y.dtype == torch.bfloat16 and h.dtype == torch.float32
+    assert torch.equal(y, fused.linear(*(t.bfloat16() for t in (x, w, b)), "gelu", res.bfloat16()))
+    assert torch.equal(h, fused.layer_norm(x.bfloat16().float(), 64, w[0]))
+    grads = torch.autograd.grad(y, leaves, g.bfloat16())
+    assert all(d.dtype == torch.float32 for d in grads)
