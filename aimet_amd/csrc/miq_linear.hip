@@ -2,79 +2,133 @@
 //
 //   z = x w^T + b, y = act(z) + residual                          x [rows, in], w [out, in], y [rows, out]
 //   dz = g act'(z), dx = dz w, dw = dz^T x, db = sum over rows of dz, dresidual = g
-#include "miq_activation.h"
-#include "miq_io.h"
+#include "miq_product.h"
 
 #include <algorithm>
-#include <type_traits>
 
 namespace miq
 {
 namespace
 {
-// What the backward pass keeps of z = x w^T + b.  float32 tensors keep it as it is.  bfloat16 ones keep a half: as
-// many bytes, three bits more, and z matters only through act'(z), which is flat far out, so saturating at the
-// largest half loses nothing.  A z > 0 too small for a half is kept as the smallest one: ReLU's derivative goes by
-// its sign.  NaN stays NaN.
+// ------------------------------------------------------------------------------------------ operands made ready
+// A product reads 16-byte chunks of 16-bit operands.  bfloat16 tensors whose rows are whole chunks are read as they
+// lie; others are copied, k contiguous, rows padded with zeros.
+//
+// float32 operands become two halves of 11 significant bits each, row by row (a row: what shares one m or n):
+//   s = 14 - floor(log2 of the row's largest finite magnitude), t = x 2^s, coarse = half(t), fine = half(t - coarse)
+// so |t - coarse - fine| <= 2^-23 |t| for |t| >= 2^-14 2^11 ulps of a half, and never more than 2^-25: 2^-39 of the
+// row's largest.  A product of two operands is the sum of coarse coarse + coarse fine + fine coarse; fine fine, which is
+// left out, is at most 2^-22 of it and has no sign of its own: about the error of float32 arithmetic itself.  Three
+// passes through the half-precision matrix unit run at about 5 times the rate of the float32 one.
+// coarse of an infinity or NaN is itself, its fine is 0.
+__device__ __forceinline__ int row_shift(uint32_t largest /* bits of a finite float32 */)
+{
+    if (largest == 0)
+        return 0;
+    const int e = (int) (largest >> 23);
+    return 14 - (e ? e - 127 : (31 - __clz(largest)) - 149);
+}
+
+__device__ __forceinline__ void split_value(float x, int shift, uint16_t* coarse, uint16_t* fine)
+{
+    const float t    = ldexpf(x, shift);
+    const _Float16 c = (_Float16) t;
+    const float f    = t - (float) c;
+    const _Float16 d = __builtin_isfinite(t) ? (_Float16) f : (_Float16) 0.f;
+    *coarse          = __builtin_bit_cast(uint16_t, c);
+    *fine            = __builtin_bit_cast(uint16_t, d);
+}
+
+__device__ __forceinline__ uint32_t finite_magnitude(float x)
+{
+    const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
+    return b < 0x7f800000u ? b : 0u;
+}
+
+// out[r][0 .. kp) = src[r][0 .. k), zeros behind; float32: out[r][0 .. kp) coarse, out[r][kp .. 2 kp) fine, scale[r] = -s
 template <typename T>
-using Saved = std::conditional_t<std::is_same<T, float>::value, float, _Float16>;
-
-__device__ __forceinline__ void save_z(float* p, float z)
+__global__ __launch_bounds__(kBlock) void pack_rows_kernel(const T* __restrict__ src, int64_t k, int64_t kp,
+                                                           uint16_t* __restrict__ out, int* __restrict__ scale)
 {
-    *p = z;
-}
-__device__ __forceinline__ void save_z(_Float16* p, float z)
-{
-    const float c = z > 65504.f ? 65504.f : z < -65504.f ? -65504.f : z;
-    *p            = (_Float16) (z > 0.f && z < 0x1p-24f ? 0x1p-24f : c);
-}
-
-constexpr int kTile = 64, kDeep = 16;
-
-// C[m, n] = sum over k of A(m, k) B(n, k): A(m, k) = a[m * ams + k * aks], B likewise.
-// One 64 x 64 tile of C in a block of 256 threads, 4 x 4 values in each, operands through LDS in float32.
-template <typename T, int ACT>
-__global__ __launch_bounds__(kBlock) void product_kernel(const T* __restrict__ a, int64_t ams, int64_t aks,
-                                                         const T* __restrict__ b, int64_t bns, int64_t bks, int64_t m,
-                                                         int64_t n, int64_t k, const T* __restrict__ bias,
-                                                         const T* __restrict__ residual, T* __restrict__ c,
-                                                         Saved<T>* __restrict__ saved)
-{
-    using IO = IOTraits<T>;
-    __shared__ float la[kDeep][kTile + 4], lb[kDeep][kTile + 4];
-    const int64_t tiles_n = (n + kTile - 1) / kTile;
-    const int64_t m0 = (blockIdx.x / tiles_n) * kTile, n0 = (blockIdx.x % tiles_n) * kTile;
-    const int tm = threadIdx.x / 16, tn = threadIdx.x % 16;
-    float acc[4][4] = {};
-    for (int64_t k0 = 0; k0 < k; k0 += kDeep)
+    const int64_t r = blockIdx.x;
+    const T* from   = src + r * k;
+    if constexpr (std::is_same<T, float>::value)
     {
-        for (int i = threadIdx.x; i < kTile * kDeep; i += kBlock)
-        {
-            const int kk = i % kDeep, r = i / kDeep;
-            la[kk][r] = m0 + r < m && k0 + kk < k ? IO::load1(a + (m0 + r) * ams + (k0 + kk) * aks) : 0.f;
-            lb[kk][r] = n0 + r < n && k0 + kk < k ? IO::load1(b + (n0 + r) * bns + (k0 + kk) * bks) : 0.f;
-        }
+        __shared__ uint32_t lds[kBlock / 64];
+        uint32_t largest = 0;
+        for (int64_t c = threadIdx.x; c < k; c += kBlock)
+            largest = max(largest, finite_magnitude(from[c]));
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1)
+            largest = max(largest, (uint32_t) __shfl_xor((int) largest, o, 64));
+        if ((threadIdx.x & 63) == 0)
+            lds[threadIdx.x >> 6] = largest;
         __syncthreads();
 #pragma unroll
-        for (int kk = 0; kk < kDeep; ++kk)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    acc[i][j] = fmaf(la[kk][tm * 4 + i], lb[kk][tn * 4 + j], acc[i][j]);
-        __syncthreads();
+        for (int i = 0; i < kBlock / 64; ++i)
+            largest = max(largest, lds[i]);
+        const int shift = row_shift(largest);
+        uint16_t* to    = out + r * 2 * kp;
+        for (int64_t c = threadIdx.x; c < kp; c += kBlock)
+            split_value(c < k ? from[c] : 0.f, shift, to + c, to + kp + c);
+        if (threadIdx.x == 0)
+            scale[r] = -shift;
     }
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j)
+    else
+        for (int64_t c = threadIdx.x; c < kp; c += kBlock)
+            out[r * kp + c] = c < k ? from[c] : (uint16_t) 0;
+}
+
+__global__ __launch_bounds__(kBlock) void clear_kernel(uint32_t* p, int64_t n)
+{
+    const int64_t i = (int64_t) blockIdx.x * kBlock + threadIdx.x;
+    if (i < n)
+        p[i] = 0;
+}
+
+// largest[c] = largest finite magnitude of column c of src [k][count] (bits; cleared before)
+__global__ __launch_bounds__(kBlock) void column_max_kernel(const float* __restrict__ src, int64_t k, int64_t count,
+                                                            int64_t rows_per_slice, uint32_t* __restrict__ largest)
+{
+    const int64_t c = (int64_t) blockIdx.x * kBlock + threadIdx.x;
+    if (c >= count)
+        return;
+    const int64_t first = blockIdx.y * rows_per_slice;
+    const int64_t last  = first + rows_per_slice < k ? first + rows_per_slice : k;
+    uint32_t m          = 0;
+    for (int64_t r = first; r < last; ++r)
+        m = max(m, finite_magnitude(src[r * count + c]));
+    atomicMax(largest + c, m);   // a maximum is the same in any order
+}
+
+// as pack_rows_kernel, of the transpose: src [k][count], row r of the result is column r of src
+template <typename T>
+__global__ __launch_bounds__(kBlock) void pack_columns_kernel(const T* __restrict__ src, int64_t k, int64_t count,
+                                                              int64_t kp, const uint32_t* __restrict__ largest,
+                                                              uint16_t* __restrict__ out, int* __restrict__ scale)
+{
+    __shared__ T tile[64][65];
+    const int64_t across = (count + 63) / 64;
+    const int64_t r0 = blockIdx.x % across * 64, k0 = blockIdx.x / across * 64;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int i = wave; i < 64; i += kBlock / 64)
+        tile[i][lane] = k0 + i < k && r0 + lane < count ? src[(k0 + i) * count + r0 + lane] : (T) 0;
+    __syncthreads();
+    for (int i = wave; i < 64; i += kBlock / 64)
+    {
+        const int64_t r = r0 + i, c = k0 + lane;
+        if (r >= count || c >= kp)
+            continue;
+        if constexpr (std::is_same<T, float>::value)
         {
-            const int64_t r = m0 + tm * 4 + i, q = n0 + tn * 4 + j;
-            if (r >= m || q >= n)
-                continue;
-            const float z = acc[i][j] + (bias ? IO::load1(bias + q) : 0.f);
-            if (saved)
-                save_z(saved + r * n + q, z);
-            IO::store1(c + r * n + q, act_value<ACT>(z) + (residual ? IO::load1(residual + r * n + q) : 0.f));
+            const int shift = row_shift(largest[r]);
+            split_value(tile[lane][i], shift, out + r * 2 * kp + c, out + r * 2 * kp + kp + c);
+            if (c == 0)
+                scale[r] = -shift;
         }
+        else
+            out[r * kp + c] = tile[lane][i];
+    }
 }
 
 // dz = g act'(z) and its column sums over a slice of the rows
@@ -148,28 +202,177 @@ int check_shape(int64_t rows, int64_t in, int64_t out, int activation)
     return MIQ_OK;
 }
 
-template <typename T, int ACT>
-int product(const T* a, int64_t ams, int64_t aks, const T* b, int64_t bns, int64_t bks, int64_t m, int64_t n,
-            int64_t k, const T* bias, const T* residual, T* c, Saved<T>* saved, hipStream_t s)
+// ------------------------------------------------------------------------------------------------ host side
+bool aligned(const void* p)
 {
-    const int64_t tiles = ((m + kTile - 1) / kTile) * ((n + kTile - 1) / kTile);
-    if (tiles == 0)
+    return ((uintptr_t) p & 15) == 0;
+}
+
+// A matrix that a product reads: k contiguous ("rows", [count][k]) or count contiguous ("columns", [k][count])
+template <typename T>
+struct Matrix
+{
+    const T* p;
+    int64_t count, k;
+    bool columns;
+};
+
+struct Plan
+{
+    bool pack_a, pack_b;
+    int64_t kp;               // length of packed rows
+    bool big;                 // 256 x 256 tiles, else 128 x 128
+    int splits;
+    int64_t a_bytes, b_bytes, scale_a, scale_b, partial, total;   // of the workspace
+};
+
+// bfloat16 operands whose rows are whole 16-byte chunks are read as they lie.  `at_any_address`: for the size of a
+// workspace, which is asked for before the addresses are known.
+template <typename T>
+Plan plan_product(const Matrix<T>& a, const Matrix<T>& b, bool at_any_address)
+{
+    constexpr bool kF32 = std::is_same<T, float>::value;
+    Plan p              = {};
+    const int64_t m = a.count, n = b.count, k = a.k;
+    const auto odd = [&](const Matrix<T>& x) {
+        return kF32 || (x.columns ? x.count : x.k) % 8 != 0 || at_any_address || !aligned(x.p);
+    };
+    p.pack_a = odd(a), p.pack_b = odd(b);
+    if (a.columns && (p.pack_a || p.pack_b))
+        p.pack_a = p.pack_b = true;   // both in columns, or both in rows
+    p.kp = kF32 ? (k + kSlice - 1) / kSlice * kSlice : (k + 7) / 8 * 8;
+    const int64_t big = ((m + 255) / 256) * ((n + 255) / 256), small = ((m + 127) / 128) * ((n + 127) / 128);
+    p.big               = big >= 200;
+    const int64_t slices = (k + kSlice - 1) / kSlice;
+    p.splits = p.big ? 1 : (int) std::max<int64_t>(1, std::min<int64_t>(512 / std::max<int64_t>(small, 1), slices / 8));
+    const int64_t each = (kF32 ? 2 : 1) * p.kp * 2;
+    p.a_bytes = p.pack_a ? up256(m * each) : 0, p.b_bytes = p.pack_b ? up256(n * each) : 0;
+    p.scale_a = kF32 ? up256(m * 8) : 0, p.scale_b = kF32 ? up256(n * 8) : 0;
+    p.partial = p.splits > 1 ? up256(p.splits * m * n * 4) : 0;
+    p.total   = p.a_bytes + p.b_bytes + p.scale_a + p.scale_b + p.partial;
+    return p;
+}
+
+template <typename T>
+int pack(const Matrix<T>& x, int64_t kp, char* to, char* scale, hipStream_t s)
+{
+    if (x.count == 0 || kp == 0)
         return MIQ_OK;
-    MIQ_CHECK_ARG(tiles <= INT32_MAX, "the product has too many tiles");
-    hipLaunchKernelGGL((product_kernel<T, ACT>), dim3((unsigned) tiles), dim3(kBlock), 0, s, a, ams, aks, b, bns, bks,
-                       m, n, k, bias, residual, c, saved);
+    int* exponents    = (int*) scale;
+    uint32_t* largest = (uint32_t*) scale + x.count;
+    if (!x.columns)
+    {
+        hipLaunchKernelGGL(pack_rows_kernel<T>, dim3((unsigned) x.count), dim3(kBlock), 0, s, x.p, x.k, kp,
+                           (uint16_t*) to, exponents);
+        MIQ_CHECK_LAUNCH();
+        return MIQ_OK;
+    }
+    if constexpr (std::is_same<T, float>::value)
+    {
+        const unsigned columns = (unsigned) ((x.count + kBlock - 1) / kBlock);
+        hipLaunchKernelGGL(clear_kernel, dim3(columns), dim3(kBlock), 0, s, largest, x.count);
+        MIQ_CHECK_LAUNCH();
+        const int64_t slices = slope_slices(x.k, x.count);
+        hipLaunchKernelGGL(column_max_kernel, dim3(columns, (unsigned) slices), dim3(kBlock), 0, s, x.p, x.k, x.count,
+                           (x.k + slices - 1) / slices, largest);
+        MIQ_CHECK_LAUNCH();
+    }
+    const int64_t tiles = ((x.count + 63) / 64) * ((kp + 63) / 64);
+    MIQ_CHECK_ARG(tiles <= INT32_MAX, "an operand has too many tiles");
+    hipLaunchKernelGGL(pack_columns_kernel<T>, dim3((unsigned) tiles), dim3(kBlock), 0, s, x.p, x.k, x.count, kp,
+                       largest, (uint16_t*) to, exponents);
     MIQ_CHECK_LAUNCH();
     return MIQ_OK;
+}
+
+template <typename T, int ACT, bool AC, bool BC>
+int launch_product(Product<T>& p, bool big, hipStream_t s)
+{
+    const int tile = big ? 256 : 128;
+    p.tiles_m = (int) ((p.e.m + tile - 1) / tile), p.tiles_n = (int) ((p.e.n + tile - 1) / tile);
+    const int64_t blocks = (int64_t) p.tiles_m * p.tiles_n * p.splits;
+    MIQ_CHECK_ARG(blocks <= INT32_MAX, "the product has too many tiles");
+    if (big)
+        hipLaunchKernelGGL((product_kernel<T, ACT, 2, 4, 8, 4, AC, BC>), dim3((unsigned) blocks), dim3(512), 0, s, p);
+    else
+        hipLaunchKernelGGL((product_kernel<T, ACT, 2, 2, 4, 4, AC, BC>), dim3((unsigned) blocks), dim3(256), 0, s, p);
+    MIQ_CHECK_LAUNCH();
+    if (p.splits > 1)
+    {
+        const int64_t groups = (p.e.n + 7) / 8 * p.e.m;
+        hipLaunchKernelGGL((join_kernel<T, ACT>), dim3((unsigned) ((groups + kBlock - 1) / kBlock)), dim3(kBlock), 0, s,
+                           p.partial, p.splits, p.e);
+        MIQ_CHECK_LAUNCH();
+    }
+    return MIQ_OK;
+}
+
+// c[m, n] = act(sum over k of a(m, k) b(n, k) + bias) + residual
+template <typename T, int ACT>
+int product(const Matrix<T>& a, const Matrix<T>& b, const T* bias, const T* residual, T* c, Saved<T>* saved,
+            char* workspace, hipStream_t s)
+{
+    if (a.count == 0 || b.count == 0)
+        return MIQ_OK;
+    const Plan plan = plan_product(a, b, false);
+    Product<T> p    = {};
+    char* const pa = workspace;
+    char* const pb = pa + plan.a_bytes;
+    char* const sa = pb + plan.b_bytes;
+    char* const sb = sa + plan.scale_a;
+    p.a = {(const uint16_t*) a.p, a.columns ? a.count : a.k, a.count};
+    p.b = {(const uint16_t*) b.p, b.columns ? b.count : b.k, b.count};
+    const int64_t ld = (std::is_same<T, float>::value ? 2 : 1) * plan.kp;
+    if (plan.pack_a)
+    {
+        if (int rc = pack(a, plan.kp, pa, sa, s))
+            return rc;
+        p.a = {(const uint16_t*) pa, ld, a.count};
+    }
+    if (plan.pack_b)
+    {
+        if (int rc = pack(b, plan.kp, pb, sb, s))
+            return rc;
+        p.b = {(const uint16_t*) pb, ld, b.count};
+    }
+    p.k       = plan.pack_a && plan.pack_b ? plan.kp : a.k;
+    p.scale_a = (const int*) sa, p.scale_b = (const int*) sb;
+    p.splits  = plan.splits;
+    p.partial = (float*) (sb + plan.scale_b);
+    p.e       = {bias, residual, c, saved, a.count, b.count,
+                 b.count % 8 == 0 && aligned(bias) && aligned(residual) && aligned(c) && aligned(saved)};
+    if constexpr (std::is_same<T, float>::value)
+        return launch_product<T, ACT, false, false>(p, plan.big, s);
+    else
+    {
+        const bool ac = a.columns && !plan.pack_a, bc = b.columns && !plan.pack_b;
+        if constexpr (ACT == MIQ_ACT_NONE)
+        {
+            if (ac && bc)
+                return launch_product<T, ACT, true, true>(p, plan.big, s);
+            if (bc)
+                return launch_product<T, ACT, false, true>(p, plan.big, s);
+        }
+        return launch_product<T, ACT, false, false>(p, plan.big, s);
+    }
+}
+
+template <typename T>
+int64_t product_bytes(int64_t m, int64_t n, int64_t k, bool ac, bool bc)
+{
+    if (m == 0 || n == 0)
+        return 0;
+    return plan_product<T>({nullptr, m, k, ac}, {nullptr, n, k, bc}, true).total;
 }
 
 template <typename T>
 int64_t workspace_bytes(int64_t rows, int64_t in, int64_t out, int activation, int backward)
 {
-    (void) in;
     if (!backward)
-        return 0;
+        return product_bytes<T>(rows, out, in, false, false);
     return (activation == MIQ_ACT_NONE ? 0 : up256(rows * out * (int64_t) sizeof(T))) +
-           up256(slope_slices(rows, out) * out * (int64_t) sizeof(float));
+           up256(slope_slices(rows, out) * out * (int64_t) sizeof(float)) +
+           std::max(product_bytes<T>(rows, in, out, false, true), product_bytes<T>(out, in, rows, true, true));
 }
 
 template <typename T>
@@ -181,12 +384,12 @@ int linear_fwd(const T* x, const T* w, const T* bias, const T* residual, int64_t
     if (rows == 0 || out == 0)
         return MIQ_OK;
     MIQ_CHECK_ARG(y && (in == 0 || (x && w)), "null pointer");
-    MIQ_CHECK_ARG(bytes >= workspace_bytes<T>(rows, in, out, activation, 0), "the workspace is too small");
-    (void) workspace;
+    MIQ_CHECK_ARG(bytes >= workspace_bytes<T>(rows, in, out, activation, 0) && (workspace || bytes == 0),
+                  "the workspace is too small");
     int rc = MIQ_OK;
     with_activation(activation, [&](auto act) {
-        rc = product<T, act.value>(x, in, 1, w, in, 1, rows, out, in, bias, residual, y, (Saved<T>*) saved,
-                                   (hipStream_t) stream);
+        rc = product<T, act.value>({x, rows, in, false}, {w, out, in, false}, bias, residual, y, (Saved<T>*) saved,
+                                   (char*) workspace, (hipStream_t) stream);
     });
     return rc;
 }
@@ -201,31 +404,35 @@ int linear_bwd(const T* g, const void* saved, const T* x, const T* w, int64_t ro
     MIQ_CHECK_ARG(rows * out == 0 || (g && (saved || !kept)), "null pointer");
     MIQ_CHECK_ARG(rows * in == 0 || !dw || x, "dweight needs x");
     MIQ_CHECK_ARG(out * in == 0 || !dx || w, "dx needs weight");
-    MIQ_CHECK_ARG(workspace && bytes >= workspace_bytes<T>(rows, in, out, activation, 1),
+    MIQ_CHECK_ARG((workspace || bytes == 0) && bytes >= workspace_bytes<T>(rows, in, out, activation, 1),
                   "the workspace is too small");
     hipStream_t s  = (hipStream_t) stream;
     const T* dz    = g;
-    float* partial = (float*) ((char*) workspace + (kept ? up256(rows * out * (int64_t) sizeof(T)) : 0));
+    char* at       = (char*) workspace;
+    T* own_dz      = (T*) at;
+    at += kept ? up256(rows * out * (int64_t) sizeof(T)) : 0;
+    float* partial = (float*) at;
+    const int64_t slices = slope_slices(rows, out);
+    at += up256(slices * out * (int64_t) sizeof(float));
     if ((kept || db) && out > 0)
     {
-        const int64_t slices = slope_slices(rows, out);
         const dim3 grid((unsigned) ((out + kBlock - 1) / kBlock), (unsigned) slices);
         with_activation(activation, [&](auto act) {
             hipLaunchKernelGGL((slope_kernel<T, act.value>), grid, dim3(kBlock), 0, s, g, (const Saved<T>*) saved,
-                               rows, out, (rows + slices - 1) / slices, (T*) workspace, partial);
+                               rows, out, (rows + slices - 1) / slices, own_dz, partial);
         });
         MIQ_CHECK_LAUNCH();
         if (kept)
-            dz = (const T*) workspace;
+            dz = own_dz;
         if (db)
             hipLaunchKernelGGL(join_columns_kernel<T>, dim3(grid.x), dim3(kBlock), 0, s, partial, slices, out, db);
         MIQ_CHECK_LAUNCH();
     }
     int rc = MIQ_OK;
     if (dx)
-        rc = product<T, MIQ_ACT_NONE>(dz, out, 1, w, 1, in, rows, in, out, nullptr, nullptr, dx, nullptr, s);
+        rc = product<T, MIQ_ACT_NONE>({dz, rows, out, false}, {w, in, out, true}, nullptr, nullptr, dx, nullptr, at, s);
     if (rc == MIQ_OK && dw)
-        rc = product<T, MIQ_ACT_NONE>(dz, 1, out, x, 1, in, out, in, rows, nullptr, nullptr, dw, nullptr, s);
+        rc = product<T, MIQ_ACT_NONE>({dz, out, rows, true}, {x, in, rows, true}, nullptr, nullptr, dw, nullptr, at, s);
     return rc;
 }
 }   // namespace
