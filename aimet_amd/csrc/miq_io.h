@@ -109,6 +109,33 @@ struct IOTraits<uint16_t>
     }
 };
 
+// 16 bytes at any address that its elements allow.  The memory pipeline takes vector accesses at any alignment (one more
+// cache line per kilobyte), so rows that do not start on 16 bytes need no path of their own.
+typedef float any_f4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef unsigned int any_u4 __attribute__((ext_vector_type(4), aligned(2)));
+
+__device__ __forceinline__ void load_any(const float* p, float* f)
+{
+    const any_f4 v = *(const any_f4*) p;
+    f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w;
+}
+__device__ __forceinline__ void load_any(const uint16_t* p, float* f)
+{
+    const any_u4 v = *(const any_u4*) p;
+    IOTraits<uint16_t>::unpack(make_uint4(v.x, v.y, v.z, v.w), f);
+}
+__device__ __forceinline__ void store_any(float* p, const float* f)
+{
+    const any_f4 v = {f[0], f[1], f[2], f[3]};
+    *(any_f4*) p   = v;
+}
+__device__ __forceinline__ void store_any(uint16_t* p, const float* f)
+{
+    const uint4 w  = IOTraits<uint16_t>::pack(f);
+    const any_u4 v = {w.x, w.y, w.z, w.w};
+    *(any_u4*) p   = v;
+}
+
 }   // namespace miq
 
 #endif

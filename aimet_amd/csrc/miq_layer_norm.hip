@@ -13,45 +13,163 @@ namespace miq
 {
 namespace
 {
-// sum over the block, the same in every thread; `lds` holds kBlock / 64 floats and may be used again after the next barrier
-__device__ __forceinline__ float block_sum(float v, float* lds)
+// sum over LANES threads (a wave, or a whole block of LANES), the same in each of them
+template <int LANES>
+__device__ __forceinline__ float lanes_sum(float v, float* lds)
 {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1)
         v += __shfl_xor(v, o, 64);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0)
-        lds[threadIdx.x >> 6] = v;
-    __syncthreads();
-    float s = 0.f;
+    if constexpr (LANES > 64)
+    {
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0)
+            lds[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = 0.f;
 #pragma unroll
-    for (int i = 0; i < kBlock / 64; ++i)
-        s += lds[i];
-    return s;
+        for (int i = 0; i < LANES / 64; ++i)
+            v += lds[i];
+    }
+    return v;
 }
 
+// two sums at once
+template <int LANES>
+__device__ __forceinline__ void lanes_sum2(float& a, float& b, float2* lds)
+{
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1)
+    {
+        a += __shfl_xor(a, o, 64);
+        b += __shfl_xor(b, o, 64);
+    }
+    if constexpr (LANES > 64)
+    {
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0)
+            lds[threadIdx.x >> 6] = make_float2(a, b);
+        __syncthreads();
+        a = b = 0.f;
+#pragma unroll
+        for (int i = 0; i < LANES / 64; ++i)
+        {
+            a += lds[i].x;
+            b += lds[i].y;
+        }
+    }
+}
+
+// A row lies in the registers of LANES threads, PER pieces of 16 bytes in each: piece i of lane l starts at value
+// (i LANES + l) VEC.  What is past the row's end is read as zero and not stored.
 template <typename T>
-__global__ __launch_bounds__(kBlock) void ln_fwd_kernel(const T* __restrict__ x, const T* __restrict__ w,
-                                                        const T* __restrict__ b, int64_t width, float eps,
-                                                        T* __restrict__ y, float* __restrict__ mean,
-                                                        float* __restrict__ rstd)
+__device__ __forceinline__ void load_piece(const T* p, int left, float* v)
+{
+    constexpr int VEC = IOTraits<T>::VEC;
+    if (left >= VEC)
+        load_any(p, v);
+    else
+#pragma unroll
+        for (int u = 0; u < VEC; ++u)
+            v[u] = u < left ? IOTraits<T>::load1(p + u) : 0.f;
+}
+template <typename T>
+__device__ __forceinline__ void store_piece(T* p, int left, const float* v)
+{
+    constexpr int VEC = IOTraits<T>::VEC;
+    if (left >= VEC)
+        store_any(p, v);
+    else
+#pragma unroll
+        for (int u = 0; u < VEC; ++u)
+            if (u < left)
+                IOTraits<T>::store1(p + u, v[u]);
+}
+
+// One pass: the row stays in registers between its mean, its variance (from differences to the mean) and the result.
+template <typename T, int PER, int LANES>
+__global__ __launch_bounds__(LANES < kBlock ? kBlock : LANES) void ln_fwd_kernel(
+    const T* __restrict__ x, const T* __restrict__ w, const T* __restrict__ b, int64_t rows, int width, float eps,
+    T* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd)
+{
+    constexpr int VEC = IOTraits<T>::VEC, kRows = LANES < kBlock ? kBlock / LANES : 1;
+    __shared__ float lds[LANES / 64];
+    const int lane    = threadIdx.x % LANES;
+    const int64_t row = (int64_t) blockIdx.x * kRows + threadIdx.x / LANES;
+    if (row >= rows)
+        return;   // (a whole wave: with one row a block there are as many blocks as rows)
+    const T* px = x + row * width;
+    float v[PER][VEC], s = 0.f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+        load_piece(px + (i * LANES + lane) * VEC, width - (i * LANES + lane) * VEC, v[i]);
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+#pragma unroll
+        for (int u = 0; u < VEC; ++u)
+            s += v[i][u];
+    const float m = lanes_sum<LANES>(s, lds) / (float) width;
+    float q       = 0.f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+#pragma unroll
+        for (int u = 0; u < VEC; ++u)
+        {
+            v[i][u] = (i * LANES + lane) * VEC + u < width ? v[i][u] - m : 0.f;
+            q       = fmaf(v[i][u], v[i][u], q);
+        }
+    const float r = 1.0f / sqrtf(lanes_sum<LANES>(q, lds) / (float) width + eps);
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+    {
+        const int c = (i * LANES + lane) * VEC;
+        if (c >= width)
+            continue;
+        float ww[VEC], bb[VEC];
+        if (w)
+            load_piece(w + c, width - c, ww);
+        if (b)
+            load_piece(b + c, width - c, bb);
+#pragma unroll
+        for (int u = 0; u < VEC; ++u)
+        {
+            float h = v[i][u] * r;
+            if (w)
+                h *= ww[u];
+            v[i][u] = b ? h + bb[u] : h;
+        }
+        store_piece(y + row * width + c, width - c, v[i]);
+    }
+    if (lane == 0 && mean)
+    {
+        mean[row] = m;
+        rstd[row] = r;
+    }
+}
+
+// Rows too long for registers: read three times, the second and third from the caches
+template <typename T>
+__global__ __launch_bounds__(1024) void ln_fwd_long_kernel(const T* __restrict__ x, const T* __restrict__ w,
+                                                           const T* __restrict__ b, int64_t width, float eps,
+                                                           T* __restrict__ y, float* __restrict__ mean,
+                                                           float* __restrict__ rstd)
 {
     using IO = IOTraits<T>;
-    __shared__ float lds[kBlock / 64];
+    __shared__ float lds[1024 / 64];
     const int64_t row = blockIdx.x;
     const T* px       = x + row * width;
     float s           = 0.f;
-    for (int64_t c = threadIdx.x; c < width; c += kBlock)
+    for (int64_t c = threadIdx.x; c < width; c += 1024)
         s += IO::load1(px + c);
-    const float m = block_sum(s, lds) / (float) width;
+    const float m = lanes_sum<1024>(s, lds) / (float) width;
     float q       = 0.f;
-    for (int64_t c = threadIdx.x; c < width; c += kBlock)
+    for (int64_t c = threadIdx.x; c < width; c += 1024)
     {
         const float d = IO::load1(px + c) - m;
-        q += d * d;
+        q             = fmaf(d, d, q);
     }
-    const float r = 1.0f / sqrtf(block_sum(q, lds) / (float) width + eps);
-    for (int64_t c = threadIdx.x; c < width; c += kBlock)
+    const float r = 1.0f / sqrtf(lanes_sum<1024>(q, lds) / (float) width + eps);
+    for (int64_t c = threadIdx.x; c < width; c += 1024)
     {
         const float h = (IO::load1(px + c) - m) * r;
         IO::store1(y + row * width + c, h * (w ? IO::load1(w + c) : 1.f) + (b ? IO::load1(b + c) : 0.f));
@@ -63,42 +181,151 @@ __global__ __launch_bounds__(kBlock) void ln_fwd_kernel(const T* __restrict__ x,
     }
 }
 
+// One pass over x and grad: a block takes rows block, block + blocks, ...; a thread meets the same columns in every row
+// and keeps their sums g xhat and g.  partial[block][0][c] and [1][c] receive them, for ln_join_kernel.
+template <typename T, int PER, int LANES>
+__global__ __launch_bounds__(LANES < kBlock ? kBlock : LANES) void ln_bwd_kernel(
+    const T* __restrict__ x, const T* __restrict__ g, const T* __restrict__ w, const float* __restrict__ mean,
+    const float* __restrict__ rstd, int64_t rows, int width, T* __restrict__ dx, float* __restrict__ partial)
+{
+    constexpr int VEC = IOTraits<T>::VEC, kRows = LANES < kBlock ? kBlock / LANES : 1;
+    __shared__ float2 lds[LANES / 64];
+    const int lane = threadIdx.x % LANES;
+    float sw[PER][VEC] = {}, sb[PER][VEC] = {};
+    for (int64_t row = (int64_t) blockIdx.x * kRows + threadIdx.x / LANES; row < rows;
+         row += (int64_t) gridDim.x * kRows)
+    {
+        const float m = mean[row], r = rstd[row];
+        const T* px = x + row * width;
+        const T* pg = g + row * width;
+        float h[PER][VEC], gv[PER][VEC], s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+        {
+            const int c = (i * LANES + lane) * VEC;
+            load_piece(px + c, width - c, h[i]);
+            load_piece(pg + c, width - c, gv[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+        {
+            const int c = (i * LANES + lane) * VEC;
+            if (c >= width)
+                continue;
+            float ww[VEC];
+            if (w)
+                load_piece(w + c, width - c, ww);
+#pragma unroll
+            for (int u = 0; u < VEC; ++u)
+            {
+                h[i][u] = (h[i][u] - m) * r;   // (past the end: g is 0 there, and so is every sum's term)
+                sw[i][u] = fmaf(gv[i][u], h[i][u], sw[i][u]);
+                sb[i][u] += gv[i][u];
+                if (w)
+                    gv[i][u] *= ww[u];
+                s1 += gv[i][u];
+                s2 = fmaf(gv[i][u], h[i][u], s2);
+            }
+        }
+        if (!dx)
+            continue;
+        lanes_sum2<LANES>(s1, s2, lds);
+        s1 /= (float) width;
+        s2 /= (float) width;
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+        {
+            const int c = (i * LANES + lane) * VEC;
+            if (c >= width)
+                continue;
+#pragma unroll
+            for (int u = 0; u < VEC; ++u)
+                gv[i][u] = r * (gv[i][u] - s1 - h[i][u] * s2);
+            store_piece(dx + row * width + c, width - c, gv[i]);
+        }
+    }
+    if (!partial)
+        return;
+    if constexpr (kRows > 1)
+    {
+        // the block's waves saw the same columns: added wave by wave
+        __shared__ float both[2][PER * LANES * VEC];
+        for (int k = 0; k < kRows; ++k)
+        {
+            if ((int) threadIdx.x / LANES == k)
+#pragma unroll
+                for (int i = 0; i < PER; ++i)
+#pragma unroll
+                    for (int u = 0; u < VEC; ++u)
+                    {
+                        const int c = (i * LANES + lane) * VEC + u;
+                        both[0][c]  = k ? both[0][c] + sw[i][u] : sw[i][u];
+                        both[1][c]  = k ? both[1][c] + sb[i][u] : sb[i][u];
+                    }
+            __syncthreads();
+        }
+        for (int c = threadIdx.x; c < width; c += kBlock)
+        {
+            partial[((int64_t) blockIdx.x * 2) * width + c]     = both[0][c];
+            partial[((int64_t) blockIdx.x * 2 + 1) * width + c] = both[1][c];
+        }
+    }
+    else
+    {
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+        {
+            const int c = (i * LANES + lane) * VEC;
+            if (c >= width)
+                continue;
+#pragma unroll
+            for (int k = 0; k < VEC; k += 4)
+            {
+                store_piece(partial + ((int64_t) blockIdx.x * 2) * width + c + k, width - c - k, sw[i] + k);
+                store_piece(partial + ((int64_t) blockIdx.x * 2 + 1) * width + c + k, width - c - k, sb[i] + k);
+            }
+        }
+    }
+}
+
+// rows too long for registers
 template <typename T>
-__global__ __launch_bounds__(kBlock) void ln_dx_kernel(const T* __restrict__ x, const T* __restrict__ g,
-                                                       const T* __restrict__ w, const float* __restrict__ mean,
-                                                       const float* __restrict__ rstd, int64_t width,
-                                                       T* __restrict__ dx)
+__global__ __launch_bounds__(1024) void ln_dx_long_kernel(const T* __restrict__ x, const T* __restrict__ g,
+                                                          const T* __restrict__ w, const float* __restrict__ mean,
+                                                          const float* __restrict__ rstd, int64_t width,
+                                                          T* __restrict__ dx)
 {
     using IO = IOTraits<T>;
-    __shared__ float lds[kBlock / 64];
+    __shared__ float2 lds[1024 / 64];
     const int64_t row = blockIdx.x;
     const T* px       = x + row * width;
     const T* pg       = g + row * width;
     const float m = mean[row], r = rstd[row];
     float s1 = 0.f, s2 = 0.f;
-    for (int64_t c = threadIdx.x; c < width; c += kBlock)
+    for (int64_t c = threadIdx.x; c < width; c += 1024)
     {
         const float gw = IO::load1(pg + c) * (w ? IO::load1(w + c) : 1.f);
         s1 += gw;
-        s2 += gw * ((IO::load1(px + c) - m) * r);
+        s2 = fmaf(gw, (IO::load1(px + c) - m) * r, s2);
     }
-    const float m1 = block_sum(s1, lds) / (float) width;
-    const float m2 = block_sum(s2, lds) / (float) width;
-    for (int64_t c = threadIdx.x; c < width; c += kBlock)
+    lanes_sum2<1024>(s1, s2, lds);
+    s1 /= (float) width;
+    s2 /= (float) width;
+    for (int64_t c = threadIdx.x; c < width; c += 1024)
     {
         const float gw = IO::load1(pg + c) * (w ? IO::load1(w + c) : 1.f);
         const float h  = (IO::load1(px + c) - m) * r;
-        IO::store1(dx + row * width + c, r * (gw - m1 - h * m2));
+        IO::store1(dx + row * width + c, r * (gw - s1 - h * s2));
     }
 }
 
-// column sums of a slice of the rows: partial[slice][0][c] = sum g xhat, partial[slice][1][c] = sum g
+// column sums of a slice of the rows, for rows too long for registers
 template <typename T>
-__global__ __launch_bounds__(kBlock) void ln_dparams_kernel(const T* __restrict__ x, const T* __restrict__ g,
-                                                            const float* __restrict__ mean,
-                                                            const float* __restrict__ rstd, int64_t rows,
-                                                            int64_t width, int64_t rows_per_slice,
-                                                            float* __restrict__ partial)
+__global__ __launch_bounds__(kBlock) void ln_dparams_long_kernel(const T* __restrict__ x, const T* __restrict__ g,
+                                                                 const float* __restrict__ mean,
+                                                                 const float* __restrict__ rstd, int64_t rows,
+                                                                 int64_t width, int64_t rows_per_slice,
+                                                                 float* __restrict__ partial)
 {
     using IO        = IOTraits<T>;
     const int64_t c = (int64_t) blockIdx.x * kBlock + threadIdx.x;
@@ -110,33 +337,88 @@ __global__ __launch_bounds__(kBlock) void ln_dparams_kernel(const T* __restrict_
     for (int64_t row = first; row < last; ++row)
     {
         const float gv = IO::load1(g + row * width + c);
-        sw += gv * ((IO::load1(x + row * width + c) - mean[row]) * rstd[row]);
+        sw             = fmaf(gv, (IO::load1(x + row * width + c) - mean[row]) * rstd[row], sw);
         sb += gv;
     }
     partial[((int64_t) blockIdx.y * 2) * width + c]     = sw;
     partial[((int64_t) blockIdx.y * 2 + 1) * width + c] = sb;
 }
 
+// adds partial[0 .. slices) of 32 columns, 32 threads a column, in an order that the number of slices alone decides
 template <typename T>
-__global__ __launch_bounds__(kBlock) void ln_join_kernel(const float* __restrict__ partial, int64_t slices,
-                                                         int64_t width, T* __restrict__ dw, T* __restrict__ db)
+__global__ __launch_bounds__(1024) void ln_join_kernel(const float* __restrict__ partial, int64_t slices,
+                                                       int64_t width, T* __restrict__ dw, T* __restrict__ db)
 {
-    const int64_t c = (int64_t) blockIdx.x * kBlock + threadIdx.x;
-    if (c >= width)
-        return;
-    T* out = blockIdx.y == 0 ? dw : db;
+    __shared__ float lds[32][33];
+    const int64_t c = (int64_t) blockIdx.x * 32 + threadIdx.x % 32;
+    const int part  = threadIdx.x / 32;
+    T* out          = blockIdx.y == 0 ? dw : db;
     if (!out)
         return;
     float s = 0.f;
-    for (int64_t k = 0; k < slices; ++k)
-        s += partial[(k * 2 + blockIdx.y) * width + c];
-    IOTraits<T>::store1(out + c, s);
+    if (c < width)
+        for (int64_t k = part; k < slices; k += 32)
+            s += partial[(k * 2 + blockIdx.y) * width + c];
+    lds[part][threadIdx.x % 32] = s;
+    __syncthreads();
+    // thread (part, lane) now adds column `part`: value `lane`
+    float v = lds[threadIdx.x % 32][part];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+        v += __shfl_xor(v, o, 64);
+    const int64_t to = (int64_t) blockIdx.x * 32 + part;
+    if (threadIdx.x % 32 == 0 && to < width)
+        IOTraits<T>::store1(out + to, v);
 }
 
+// How a row is held: 32 values a thread at most, 16 with 1024 threads (the backward pass keeps four registers a value).
+// Rows of up to 2048 values take a wave each, up to 8192 a block of 256, up to 16384 a block of 1024.
+enum class Rows
+{
+    kWave,
+    kBlock,
+    kWide,
+    kLong
+};
+
+Rows rows_of(int64_t width)
+{
+    return width <= 2048 ? Rows::kWave : width <= 8192 ? Rows::kBlock : width <= 16384 ? Rows::kWide : Rows::kLong;
+}
+
+// blocks of the backward pass: as many as the device holds at a time, no more than there are rows for
 int64_t ln_slices(int64_t rows, int64_t width)
 {
-    const int64_t columns = (width + kBlock - 1) / kBlock;
-    return std::max<int64_t>(1, std::min<int64_t>((1024 + columns - 1) / columns, rows / 16));
+    if (rows_of(width) == Rows::kLong)
+    {
+        const int64_t columns = (width + kBlock - 1) / kBlock;
+        return std::max<int64_t>(1, std::min<int64_t>((1024 + columns - 1) / columns, rows / 16));
+    }
+    const int64_t each = rows_of(width) == Rows::kWave ? 4 : 1, most = rows_of(width) == Rows::kWide ? 256 : 512;
+    return std::max<int64_t>(1, std::min<int64_t>(most, (rows + each - 1) / each));
+}
+
+// f(PER, LANES) as integral constants, for a row held in registers
+template <typename T, typename F>
+void with_rows(int64_t width, F&& f)
+{
+    const auto with_lanes = [&](auto lanes, auto most) {
+        // all of a thread's pieces, half or a quarter of them: the fewest that hold the row
+        constexpr int P     = decltype(most)::value / IOTraits<T>::VEC;
+        const int64_t piece = (int64_t) decltype(lanes)::value * IOTraits<T>::VEC, need = (width + piece - 1) / piece;
+        if (need > P / 2)
+            f(std::integral_constant<int, P>(), lanes);
+        else if (need > P / 4)
+            f(std::integral_constant<int, P / 2>(), lanes);
+        else
+            f(std::integral_constant<int, P / 4 ? P / 4 : 1>(), lanes);
+    };
+    if (rows_of(width) == Rows::kWave)
+        with_lanes(std::integral_constant<int, 64>(), std::integral_constant<int, 32>());
+    else if (rows_of(width) == Rows::kBlock)
+        with_lanes(std::integral_constant<int, 256>(), std::integral_constant<int, 32>());
+    else
+        with_lanes(std::integral_constant<int, 1024>(), std::integral_constant<int, 16>());
 }
 
 int check_shape(int64_t rows, int64_t width)
@@ -156,8 +438,17 @@ int layer_norm_fwd(const T* x, const T* w, const T* b, int64_t rows, int64_t wid
         return MIQ_OK;
     MIQ_CHECK_ARG(x && y, "null pointer");
     MIQ_CHECK_ARG((mean != nullptr) == (rstd != nullptr), "mean and rstd go together");
-    hipLaunchKernelGGL(ln_fwd_kernel<T>, dim3((unsigned) rows), dim3(kBlock), 0, (hipStream_t) stream, x, w, b, width,
-                       eps, y, mean, rstd);
+    hipStream_t s  = (hipStream_t) stream;
+    if (rows_of(width) == Rows::kLong)
+        hipLaunchKernelGGL(ln_fwd_long_kernel<T>, dim3((unsigned) rows), dim3(1024), 0, s, x, w, b, width, eps, y, mean,
+                           rstd);
+    else
+        with_rows<T>(width, [&](auto per, auto lanes) {
+            constexpr int P = decltype(per)::value, L = decltype(lanes)::value;
+            constexpr int kRows = L < kBlock ? kBlock / L : 1, kThreads = L < kBlock ? kBlock : L;
+            hipLaunchKernelGGL((ln_fwd_kernel<T, P, L>), dim3((unsigned) ((rows + kRows - 1) / kRows)),
+                               dim3(kThreads), 0, s, x, w, b, rows, (int) width, eps, y, mean, rstd);
+        });
     MIQ_CHECK_LAUNCH();
     return MIQ_OK;
 }
@@ -170,19 +461,35 @@ int layer_norm_bwd(const T* x, const T* g, const T* w, const float* mean, const 
         return rc;
     MIQ_CHECK_ARG(rows == 0 || (x && g && mean && rstd), "null pointer");
     MIQ_CHECK_ARG(!(dw || db) || workspace, "the gradients of weight and bias need the workspace");
-    hipStream_t s = (hipStream_t) stream;
-    if (dx && rows)
+    hipStream_t s        = (hipStream_t) stream;
+    const int64_t slices = ln_slices(rows, width);
+    float* partial       = dw || db ? workspace : nullptr;
+    if (!dx && !partial)
+        return MIQ_OK;
+    if (rows_of(width) == Rows::kLong)
     {
-        hipLaunchKernelGGL(ln_dx_kernel<T>, dim3((unsigned) rows), dim3(kBlock), 0, s, x, g, w, mean, rstd, width, dx);
+        if (dx && rows)
+            hipLaunchKernelGGL(ln_dx_long_kernel<T>, dim3((unsigned) rows), dim3(1024), 0, s, x, g, w, mean, rstd, width,
+                               dx);
+        MIQ_CHECK_LAUNCH();
+        if (partial)
+            hipLaunchKernelGGL(ln_dparams_long_kernel<T>, dim3((unsigned) ((width + kBlock - 1) / kBlock), (unsigned) slices),
+                               dim3(kBlock), 0, s, x, g, mean, rstd, rows, width, (rows + slices - 1) / slices, partial);
         MIQ_CHECK_LAUNCH();
     }
-    if (dw || db)
+    else if (rows || partial)
     {
-        const int64_t slices = ln_slices(rows, width), columns = (width + kBlock - 1) / kBlock;
-        hipLaunchKernelGGL(ln_dparams_kernel<T>, dim3((unsigned) columns, (unsigned) slices), dim3(kBlock), 0, s, x, g,
-                           mean, rstd, rows, width, (rows + slices - 1) / slices, workspace);
+        with_rows<T>(width, [&](auto per, auto lanes) {
+            constexpr int P = decltype(per)::value, L = decltype(lanes)::value;
+            constexpr int kThreads = L < kBlock ? kBlock : L;
+            hipLaunchKernelGGL((ln_bwd_kernel<T, P, L>), dim3((unsigned) slices), dim3(kThreads), 0, s, x, g, w,
+                               mean, rstd, rows, (int) width, dx, partial);
+        });
         MIQ_CHECK_LAUNCH();
-        hipLaunchKernelGGL(ln_join_kernel<T>, dim3((unsigned) columns, 2), dim3(kBlock), 0, s, workspace, slices,
+    }
+    if (partial)
+    {
+        hipLaunchKernelGGL(ln_join_kernel<T>, dim3((unsigned) ((width + 31) / 32), 2), dim3(1024), 0, s, partial, slices,
                            width, dw, db);
         MIQ_CHECK_LAUNCH();
     }

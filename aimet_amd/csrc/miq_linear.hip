@@ -131,43 +131,75 @@ __global__ __launch_bounds__(kBlock) void pack_columns_kernel(const T* __restric
     }
 }
 
-// dz = g act'(z) and its column sums over a slice of the rows
+// dz = g act'(z) and its column sums over a slice of the rows: a thread takes 8 columns, 32 threads across and 8 rows at
+// a time
 template <typename T, int ACT>
 __global__ __launch_bounds__(kBlock) void slope_kernel(const T* __restrict__ g, const Saved<T>* __restrict__ z,
                                                        int64_t rows, int64_t cols, int64_t rows_per_slice,
                                                        T* __restrict__ dz, float* __restrict__ partial)
 {
-    using IO        = IOTraits<T>;
-    const int64_t c = (int64_t) blockIdx.x * kBlock + threadIdx.x;
-    if (c >= cols)
-        return;
+    constexpr int VEC = 8, kAcross = 32, kDown = kBlock / kAcross;
+    __shared__ float lds[kDown][kAcross * VEC];
+    const int across = threadIdx.x % kAcross, down = threadIdx.x / kAcross;
+    const int64_t c     = ((int64_t) blockIdx.x * kAcross + across) * VEC;
     const int64_t first = blockIdx.y * rows_per_slice;
     const int64_t last  = first + rows_per_slice < rows ? first + rows_per_slice : rows;
-    float sum           = 0.f;
-    for (int64_t r = first; r < last; ++r)
-    {
-        float d = IO::load1(g + r * cols + c);
-        if (ACT != MIQ_ACT_NONE)
+    float sum[VEC]      = {};
+    if (c < cols)
+#pragma unroll 2
+        for (int64_t r = first + down; r < last; r += kDown)
         {
-            d *= act_slope<ACT>((float) z[r * cols + c]);
-            IO::store1(dz + r * cols + c, d);
+            const int64_t at = r * cols + c;
+            float d[VEC], s[VEC];
+            load8(g + at, cols - c, d);
+            if constexpr (ACT != MIQ_ACT_NONE)
+            {
+                load8(z + at, cols - c, s);
+#pragma unroll
+                for (int u = 0; u < VEC; ++u)
+                    d[u] *= act_slope<ACT>(s[u]);
+                store8(dz + at, cols - c, d);
+            }
+#pragma unroll
+            for (int u = 0; u < VEC; ++u)
+                sum[u] += d[u];
         }
-        sum += d;
+    if (!partial)
+        return;
+#pragma unroll
+    for (int u = 0; u < VEC; ++u)
+        lds[down][across * VEC + u] = sum[u];
+    __syncthreads();
+    for (int i = threadIdx.x; i < kAcross * VEC; i += kBlock)
+    {
+        const int64_t q = (int64_t) blockIdx.x * kAcross * VEC + i;
+        if (q >= cols)
+            continue;
+        float t = 0.f;
+#pragma unroll
+        for (int k = 0; k < kDown; ++k)
+            t += lds[k][i];
+        partial[(int64_t) blockIdx.y * cols + q] = t;
     }
-    partial[(int64_t) blockIdx.y * cols + c] = sum;
 }
 
+// adds the slices' sums: 64 columns a block, 4 threads a column
 template <typename T>
 __global__ __launch_bounds__(kBlock) void join_columns_kernel(const float* __restrict__ partial, int64_t slices,
                                                               int64_t cols, T* __restrict__ out)
 {
-    const int64_t c = (int64_t) blockIdx.x * kBlock + threadIdx.x;
-    if (c >= cols)
-        return;
-    float s = 0.f;
-    for (int64_t k = 0; k < slices; ++k)
-        s += partial[k * cols + c];
-    IOTraits<T>::store1(out + c, s);
+    __shared__ float lds[4][64];
+    const int64_t c = (int64_t) blockIdx.x * 64 + threadIdx.x % 64;
+    const int part  = threadIdx.x / 64;
+    float s         = 0.f;
+    if (c < cols)
+        for (int64_t k = part; k < slices; k += 4)
+            s += partial[k * cols + c];
+    lds[part][threadIdx.x % 64] = s;
+    __syncthreads();
+    if (part == 0 && c < cols)
+        IOTraits<T>::store1(out + c, (lds[0][threadIdx.x] + lds[1][threadIdx.x]) +
+                                         (lds[2][threadIdx.x] + lds[3][threadIdx.x]));
 }
 
 template <typename F>
@@ -339,8 +371,7 @@ int product(const Matrix<T>& a, const Matrix<T>& b, const T* bias, const T* resi
     p.scale_a = (const int*) sa, p.scale_b = (const int*) sb;
     p.splits  = plan.splits;
     p.partial = (float*) (sb + plan.scale_b);
-    p.e       = {bias, residual, c, saved, a.count, b.count,
-                 b.count % 8 == 0 && aligned(bias) && aligned(residual) && aligned(c) && aligned(saved)};
+    p.e       = {bias, residual, c, saved, a.count, b.count};
     if constexpr (std::is_same<T, float>::value)
         return launch_product<T, ACT, false, false>(p, plan.big, s);
     else
@@ -416,16 +447,16 @@ int linear_bwd(const T* g, const void* saved, const T* x, const T* w, int64_t ro
     at += up256(slices * out * (int64_t) sizeof(float));
     if ((kept || db) && out > 0)
     {
-        const dim3 grid((unsigned) ((out + kBlock - 1) / kBlock), (unsigned) slices);
+        const dim3 grid((unsigned) ((out + 255) / 256), (unsigned) slices);
         with_activation(activation, [&](auto act) {
-            hipLaunchKernelGGL((slope_kernel<T, act.value>), grid, dim3(kBlock), 0, s, g, (const Saved<T>*) saved,
-                               rows, out, (rows + slices - 1) / slices, own_dz, partial);
+            hipLaunchKernelGGL((slope_kernel<T, act.value>), grid, dim3(kBlock), 0, s, g, (const Saved<T>*) saved, rows, out,
+                               (rows + slices - 1) / slices, own_dz, db ? partial : nullptr);
         });
         MIQ_CHECK_LAUNCH();
         if (kept)
             dz = own_dz;
         if (db)
-            hipLaunchKernelGGL(join_columns_kernel<T>, dim3(grid.x), dim3(kBlock), 0, s, partial, slices, out, db);
+            hipLaunchKernelGGL(join_columns_kernel<T>, dim3((unsigned) ((out + 63) / 64)), dim3(kBlock), 0, s, partial, slices, out, db);
         MIQ_CHECK_LAUNCH();
     }
     int rc = MIQ_OK;

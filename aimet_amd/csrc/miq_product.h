@@ -168,33 +168,87 @@ __device__ __forceinline__ _Float16 kept_z(float z, _Float16*)
     return (_Float16) (z > 0.f && z < 0x1p-24f ? 0x1p-24f : c);
 }
 
-// 8 consecutive values between memory and float32
-__device__ __forceinline__ void load8(const float* p, float* v)
+// 8 consecutive values between memory and float32, at any address; of the last of a row only `left`
+typedef _Float16 any_h8 __attribute__((ext_vector_type(8), aligned(2)));
+
+__device__ __forceinline__ float value_at(const float* p)
 {
-    const float4 a = ((const float4*) p)[0], b = ((const float4*) p)[1];
-    IOTraits<float>::unpack(a, v);
-    IOTraits<float>::unpack(b, v + 4);
+    return *p;
 }
-__device__ __forceinline__ void load8(const uint16_t* p, float* v)
+__device__ __forceinline__ float value_at(const uint16_t* p)
 {
-    IOTraits<uint16_t>::unpack(*(const uint4*) p, v);
+    return bf16_to_f32(*p);
 }
-__device__ __forceinline__ void store8(float* p, const float* v)
+__device__ __forceinline__ float value_at(const _Float16* p)
 {
-    ((float4*) p)[0] = IOTraits<float>::pack(v);
-    ((float4*) p)[1] = IOTraits<float>::pack(v + 4);
+    return (float) *p;
 }
-__device__ __forceinline__ void store8(uint16_t* p, const float* v)
+__device__ __forceinline__ void put_at(float* p, float v)
 {
-    *(uint4*) p = IOTraits<uint16_t>::pack(v);
+    *p = v;
 }
-__device__ __forceinline__ void store8(_Float16* p, const float* v)
+__device__ __forceinline__ void put_at(uint16_t* p, float v)
 {
-    h8 h;
+    *p = (uint16_t) f32_to_bf16(v);
+}
+__device__ __forceinline__ void put_at(_Float16* p, float v)
+{
+    *p = kept_z(v, (_Float16*) nullptr);
+}
+__device__ __forceinline__ void load_whole8(const float* p, float* v)
+{
+    load_any(p, v);
+    load_any(p + 4, v + 4);
+}
+__device__ __forceinline__ void load_whole8(const uint16_t* p, float* v)
+{
+    load_any(p, v);
+}
+__device__ __forceinline__ void load_whole8(const _Float16* p, float* v)
+{
+    const any_h8 h = *(const any_h8*) p;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        v[i] = (float) h[i];
+}
+__device__ __forceinline__ void store_whole8(float* p, const float* v)
+{
+    store_any(p, v);
+    store_any(p + 4, v + 4);
+}
+__device__ __forceinline__ void store_whole8(uint16_t* p, const float* v)
+{
+    store_any(p, v);
+}
+__device__ __forceinline__ void store_whole8(_Float16* p, const float* v)
+{
+    any_h8 h;
 #pragma unroll
     for (int i = 0; i < 8; ++i)
         h[i] = kept_z(v[i], (_Float16*) nullptr);
-    *(h8*) p = h;
+    *(any_h8*) p = h;
+}
+
+template <typename S>
+__device__ __forceinline__ void load8(const S* p, int64_t left, float* v)
+{
+    if (left >= 8)
+        load_whole8(p, v);
+    else
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            v[i] = i < left ? value_at(p + i) : 0.f;
+}
+template <typename S>
+__device__ __forceinline__ void store8(S* p, int64_t left, const float* v)
+{
+    if (left >= 8)
+        store_whole8(p, v);
+    else
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < left)
+                put_at(p + i, v[i]);
 }
 
 // Where z goes: y = act(z + bias) + residual, z + bias itself for the backward pass
@@ -206,44 +260,29 @@ struct Epilogue
     T* c;
     Saved<T>* saved;      // or null
     int64_t m, n;
-    bool vec;             // n is a multiple of 8 and every pointer is 16-byte aligned
 };
 
-// z: 8 values of row r from column q on (in the matrix: r < m; q < n, but q + 8 may be past n unless vec)
+// z: 8 values of row r < m from column q < n on
 template <typename T, int ACT>
 __device__ __forceinline__ void finish8(const Epilogue<T>& e, int64_t r, int64_t q, float* z)
 {
-    const int64_t at = r * e.n + q;
+    const int64_t at = r * e.n + q, left = e.n - q;
     float t[8];
-    if (e.vec)
+    if (e.bias)
     {
-        if (e.bias)
-        {
-            load8(e.bias + q, t);
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                z[i] += t[i];
-        }
-        if (e.saved)
-            store8(e.saved + at, z);
-        if (e.residual)
-            load8(e.residual + at, t);
+        load8(e.bias + q, left, t);
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            z[i] = act_value<ACT>(z[i]) + (e.residual ? t[i] : 0.f);
-        store8(e.c + at, z);
-        return;
+            z[i] += t[i];
     }
+    if (e.saved)
+        store8(e.saved + at, left, z);
+    if (e.residual)
+        load8(e.residual + at, left, t);
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-        if (q + i < e.n)
-        {
-            const float v = z[i] + (e.bias ? IOTraits<T>::load1(e.bias + q + i) : 0.f);
-            if (e.saved)
-                e.saved[at + i] = kept_z(v, (Saved<T>*) nullptr);
-            IOTraits<T>::store1(e.c + at + i,
-                                act_value<ACT>(v) + (e.residual ? IOTraits<T>::load1(e.residual + at + i) : 0.f));
-        }
+        z[i] = act_value<ACT>(z[i]) + (e.residual ? t[i] : 0.f);
+    store8(e.c + at, left, z);
 }
 
 template <typename T>
@@ -408,18 +447,7 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(const Product<T> p
             if (p.splits == 1)
                 finish8<T, ACT>(p.e, r, q, z);
             else
-            {
-                float* to = p.partial + ((int64_t) split * p.e.m + r) * p.e.n + q;
-                if (p.e.n % 4 == 0 && q + 8 <= p.e.n)
-                {
-                    ((float4*) to)[0] = make_float4(z[0], z[1], z[2], z[3]);
-                    ((float4*) to)[1] = make_float4(z[4], z[5], z[6], z[7]);
-                }
-                else
-                    for (int u = 0; u < 8; ++u)
-                        if (q + u < p.e.n)
-                            to[u] = z[u];
-            }
+                store8(p.partial + ((int64_t) split * p.e.m + r) * p.e.n + q, p.e.n - q, z);
         }
     }
 }
@@ -436,19 +464,11 @@ __global__ __launch_bounds__(kBlock) void join_kernel(const float* __restrict__ 
     float z[8] = {};
     for (int s = 0; s < splits; ++s)
     {
-        const float* from = partial + ((int64_t) s * e.m + r) * e.n + q;
-        if (e.n % 8 == 0)
-        {
-            float t[8];
-            load8(from, t);
+        float t[8];
+        load8(partial + ((int64_t) s * e.m + r) * e.n + q, e.n - q, t);
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                z[i] += t[i];
-        }
-        else
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                z[i] += q + i < e.n ? from[i] : 0.f;
+        for (int i = 0; i < 8; ++i)
+            z[i] += t[i];
     }
     finish8<T, ACT>(e, r, q, z);
 }
