@@ -52,7 +52,8 @@ struct Operand
 
 // Where the 16-byte chunk `c` of row `r` of a slice lies: exchanged within a row such that the lanes of one LDS access
 // meet different banks.  `KEY` 0: A in rows (lanes read 8 consecutive rows), 1: B in rows (8 rows as row_of_b deals
-// them), 2: columns (lanes read 4 or 8 rows, at the same columns).
+// them), 2: A in columns (lanes read rows k .. k + 3 and k + 8 .. k + 11, at the same columns), 3: B in columns (the
+// same, columns as row_of_b deals them).
 template <int KEY>
 __device__ __forceinline__ int exchanged(int r, int c)
 {
@@ -60,7 +61,7 @@ __device__ __forceinline__ int exchanged(int r, int c)
         return c ^ (r & 7);
     if (KEY == 1)
         return c ^ ((r & 3) | ((r >> 1) & 4));
-    return c ^ ((r & 3) * 4);
+    return c ^ ((r & 3) * 4 + (r >> 3 & 1) * 2);
 }
 
 // row of B's 16 FN row share that lane index i (0..15) of fragment j holds
@@ -69,87 +70,103 @@ __device__ __forceinline__ int row_of_b(int j, int i)
     return 32 * (j / 2) + 8 * (i / 4) + 4 * (j % 2) + i % 4;
 }
 
-// One operand's slices: who loads what, and the fragments.  COUNT rows (m or n) of the tile, WAVES waves load.
+// One operand's slices: who loads what.  COUNT rows (m or n) of the tile, WAVES waves load, 1 KiB each at a time: load i
+// of a wave is the (i WAVES + wave)th KiB of the slice.  A lane's place in its row of LDS is then the same in every load,
+// and so is its offset from the load's first byte: one 32-bit register, everything else is the same for the whole wave.
 template <int COUNT, int WAVES, bool COLUMNS, int KEY>
 struct Loader
 {
     static constexpr int kChunks = (COLUMNS ? COUNT * 2 : kSlice * 2) / 16;   // 16-byte chunks of a row in LDS
-    static constexpr int kRows   = COLUMNS ? kSlice : COUNT;
-    static constexpr int kLoads  = kRows * kChunks / 64 / WAVES;              // 1 KiB loads of a wave
+    static constexpr int kRows   = COLUMNS ? kSlice : COUNT;                  // rows in LDS
+    static constexpr int kAtOnce = 64 / kChunks;                              // rows of a load
+    static constexpr int kLoads  = kRows / kAtOnce / WAVES;                   // loads of a wave
     static constexpr int kBytes  = COUNT * kSlice * 2;
-    static_assert(kRows * kChunks % (64 * WAVES) == 0, "the slice is cut evenly");
+    static_assert(kRows % (kAtOnce * WAVES) == 0 && WAVES * kAtOnce % (KEY == 0 ? 8 : 16) == 0,
+                  "the slice is cut evenly, and rows of one lane exchange their chunks alike");
 
-    const uint16_t* p[kLoads];
-    int k_of[kLoads];   // first k of the lane's chunk, within the slice
-    bool in[kLoads];    // columns: the chunk is inside of the operand
-    int64_t step;
+    const uint16_t* p;   // first value of the slice, of the wave's first row in LDS; the same in all lanes
+    int64_t step;        // to the next slice
+    int64_t apart;       // between the rows of two loads
+    uint32_t offset;     // of the lane's chunk, in bytes
+    bool edge;           // the tile reaches past the operand's end
 
     __device__ __forceinline__ void start(const Operand& o, int64_t first, int wave, int lane)
     {
-        step = COLUMNS ? o.ld * kSlice : kSlice;
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i)
-        {
-            const int at = (wave * kLoads + i) * 64 + lane, r = at / kChunks;
-            const int c = exchanged<KEY>(r, at % kChunks);
-            if (COLUMNS)
-            {
-                in[i]   = first + c * 8 < o.count;
-                k_of[i] = r;
-                p[i]    = in[i] ? o.p + r * o.ld + first + c * 8 : o.p;
-            }
-            else
-            {
-                // rows past the end read the last one: nothing made of them is stored
-                const int64_t row = first + r < o.count ? first + r : o.count - 1;
-                in[i]             = true;
-                k_of[i]           = c * 8;
-                p[i]              = o.p + row * o.ld + c * 8;
-            }
-        }
+        const int r = wave * kAtOnce, c = exchanged<KEY>(r + lane / kChunks, lane % kChunks);
+        step   = COLUMNS ? o.ld * kSlice : kSlice;
+        apart  = o.ld * (kAtOnce * WAVES);
+        p      = o.p + r * o.ld + (COLUMNS ? first : first * o.ld);
+        offset = (uint32_t) (lane / kChunks) * (uint32_t) (o.ld * 2) + c * 16;
+        edge   = first + COUNT > o.count;
     }
 
     // Starts the loads of a slice with `left` values of k remaining (from its first) into `lds`
-    template <bool TAIL>
-    __device__ __forceinline__ void load(char* lds, int wave, int64_t left)
+    __device__ __forceinline__ void load(const Operand& o, int64_t first, char* lds, int wave, int lane, int64_t left)
     {
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i)
+        if (!edge && left >= kSlice)
         {
-            const uint16_t* from = p[i];
-            if ((TAIL && k_of[i] >= left) || (COLUMNS && !in[i]))
-                from = (const uint16_t*) &g_zero16;
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*) from,
-                                             (__attribute__((address_space(3))) void*) (lds + (wave * kLoads + i) * 1024),
-                                             16, 0, 0);
-            p[i] += step;
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i)
+                to_lds((const char*) (p + i * apart) + offset, lds + (i * WAVES + wave) * 1024);
         }
+        else
+        {
+            // What is outside of the operand is read as zeros
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i)
+            {
+                const int r = (i * WAVES + wave) * kAtOnce + lane / kChunks;
+                const int c = exchanged<KEY>(r, lane % kChunks) * 8;
+                const bool in = COLUMNS ? r < left && first + c < o.count : c < left && first + r < o.count;
+                to_lds(in ? (const char*) (p + i * apart) + offset : (const char*) &g_zero16,
+                       lds + (i * WAVES + wave) * 1024);
+            }
+        }
+        p += step;
+    }
+
+    static __device__ __forceinline__ void to_lds(const char* from, char* lds)
+    {
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*) from,
+                                         (__attribute__((address_space(3))) void*) lds, 16, 0, 0);
     }
 };
 
-// fragment of rows row(0..15) of a slice, k from 32 half
+// A wave's fragments of one operand, from row 0 of its share `first` of the tile's rows.  place() is the lane's part of
+// the address, the same for all of them; the fragment's own part is a constant.
 template <bool COLUMNS, int KEY, int CHUNKS>
-__device__ __forceinline__ s8v fragment(const char* lds, int row_i, int row_q, int half, int lane)
+struct Reader
 {
-    if (!COLUMNS)
+    uint32_t at;
+
+    __device__ __forceinline__ void place(int first, int lane)
     {
-        // row_i: this lane's row of the tile
-        const int c = exchanged<KEY>(row_i, half * 4 + lane / 16);
-        return *(const s8v*) (lds + row_i * 128 + c * 16);
+        if (!COLUMNS)
+        {
+            const int r = first + (KEY == 1 ? row_of_b(0, lane % 16) : lane % 16);
+            at          = r * 128 + exchanged<KEY>(r, lane / 16) * 16;
+        }
+        else
+        {
+            // names 4 columns of row k
+            const int k = lane / 16 * 8 + lane % 16 / 4, q = first + (KEY == 3 ? row_of_b(0, lane % 4 * 4) : lane % 4 * 4);
+            at          = k * (CHUNKS * 16) + exchanged<KEY>(k, q / 8) * 16 + q % 8 * 2;
+        }
     }
-    // row_q: first of the 4 columns that this lane names
-    const int k = half * 32 + lane / 16 * 8 + (lane % 16) / 4;
-    s8v out;
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
+
+    // fragment i, k from 32 half
+    __device__ __forceinline__ s8v read(const char* lds, int i, int half) const
     {
-        const int kk = k + 4 * u;
-        const int at = kk * (CHUNKS * 16) + exchanged<KEY>(kk, row_q / 8) * 16 + (row_q % 8) * 2;
-        const s4v v  = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4v*) (lds + at));
-        out[4 * u] = v[0], out[4 * u + 1] = v[1], out[4 * u + 2] = v[2], out[4 * u + 3] = v[3];
+        if (!COLUMNS)   // rows i 16 further (B: where row_of_b has them), which leaves the exchange as it is
+            return *(const s8v*) (lds + (at ^ half * 64) + (KEY == 1 ? row_of_b(i, 0) : i * 16) * 128);
+        // columns further on are other chunks of the same row: bits that the lane's part does not have, exchanged alike
+        const uint32_t from = (at ^ (KEY == 3 ? i / 2 * 64 : i * 32)) + (KEY == 3 ? i % 2 * 8 : 0) + half * (512 * CHUNKS);
+        const s4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4v*) (lds + from));
+        const s4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) s4v*) (lds + from + 64 * CHUNKS));
+        return s8v{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     }
-    return out;
-}
+};
 
 // What the backward pass keeps of z = x w^T + b.  float32 tensors keep it as it is.  bfloat16 ones keep a half: as
 // many bytes, three bits more, and z matters only through act'(z), which is flat far out, so saturating at the
@@ -317,8 +334,9 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(const Product<T> p
 {
     constexpr bool kF32  = std::is_same<T, float>::value;
     constexpr int kWaves = WM * WN, kTM = WM * FM * 16, kTN = WN * FN * 16;
-    using LA             = Loader<kTM, kWaves, AC, AC ? 2 : 0>;
-    using LB             = Loader<kTN, kWaves, BC, BC ? 2 : 1>;
+    constexpr int kKeyA = AC ? 2 : 0, kKeyB = BC ? 3 : 1;
+    using LA             = Loader<kTM, kWaves, AC, kKeyA>;
+    using LB             = Loader<kTN, kWaves, BC, kKeyB>;
     using Kind           = std::integral_constant<bool, !kF32>;
     __shared__ __attribute__((aligned(1024))) char lds[2 * (LA::kBytes + LB::kBytes)];
 
@@ -339,40 +357,22 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(const Product<T> p
     LB lb;
     la.start(p.a, m0, wave, lane);
     lb.start(p.b, n0, wave, lane);
-#pragma unroll
-    for (int i = 0; i < LA::kLoads; ++i)
-        la.p[i] += (int64_t) first * la.step;
-#pragma unroll
-    for (int i = 0; i < LB::kLoads; ++i)
-        lb.p[i] += (int64_t) first * lb.step + (kF32 ? p.k : 0);
+    la.p += (int64_t) first * la.step;
+    lb.p += (int64_t) first * lb.step + (kF32 ? p.k : 0);
     int64_t left = p.k - (int64_t) first * kSlice;
     int issued   = 0;
     const auto issue = [&](int buffer) {
         char* to = lds + buffer * (LA::kBytes + LB::kBytes);
-        if (left >= kSlice)
-        {
-            la.template load<false>(to, wave, left);
-            lb.template load<false>(to + LA::kBytes, wave, left);
-        }
-        else
-        {
-            la.template load<true>(to, wave, left);
-            lb.template load<true>(to + LA::kBytes, wave, left);
-        }
+        la.load(p.a, m0, to, wave, lane, left);
+        lb.load(p.b, n0, to + LA::kBytes, wave, lane, left);
         left -= kSlice;
         ++issued;
         if (kF32 && (issued == last - first || issued == 2 * (last - first)))
         {
             const int64_t back = (int64_t) (last - first) * kSlice;
             left += back;
-            const int64_t ja = (issued == last - first ? p.k : -p.k) - back;
-            const int64_t jb = (issued == last - first ? -p.k : 0) - back;
-#pragma unroll
-            for (int i = 0; i < LA::kLoads; ++i)
-                la.p[i] += ja;
-#pragma unroll
-            for (int i = 0; i < LB::kLoads; ++i)
-                lb.p[i] += jb;
+            la.p += (issued == last - first ? p.k : -p.k) - back;
+            lb.p += (issued == last - first ? -p.k : 0) - back;
         }
     };
 
@@ -383,16 +383,51 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(const Product<T> p
         for (int j = 0; j < FN; ++j)
             acc[i][j] = f4{0.f, 0.f, 0.f, 0.f};
 
-    const int i16 = lane % 16;
-    if (count > 0)
-        issue(0);
-    for (int s = 0; s < count; ++s)
+    Reader<AC, kKeyA, LA::kChunks> ra;
+    Reader<BC, kKeyB, LB::kChunks> rb;
+    ra.place(wm * FM * 16, lane);
+    rb.place(wn * FN * 16, lane);
+    struct Fragments
     {
-        __syncthreads();   // slice s has arrived, and everybody is done with slice s - 1
+        s8v a[FM], b[FN];
+    };
+    const auto fetch = [&](Fragments& f, int buffer, int half) {
+        const char* sa = lds + buffer * (LA::kBytes + LB::kBytes);
+        const char* sb = sa + LA::kBytes;
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+            f.b[j] = rb.read(sb, j, half);
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+            f.a[i] = ra.read(sa, i, half);
+    };
+    const auto multiply = [&](const Fragments& f) {
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+                acc[i][j] = mfma_16x16x32(f.b[j], f.a[i], acc[i][j], Kind());
+    };
+    // Fragments of one half of a slice are read while the other half's are multiplied: across the barrier the second
+    // half of the slice before is at work.
+    Fragments f0, f1;
+    if (count > 0)
+    {
+        issue(0);
+        __syncthreads();
+        if (1 < count)
+            issue(1);
+        fetch(f0, 0, 0);
+        fetch(f1, 0, 1);
+        multiply(f0);
+    }
+    for (int s = 1; s < count; ++s)
+    {
+        __syncthreads();   // slice s has arrived, and everybody has read slice s - 1
+        fetch(f0, s & 1, 0);
         if (s + 1 < count)
             issue((s + 1) & 1);
-        const char* sa = lds + (s & 1) * (LA::kBytes + LB::kBytes);
-        const char* sb = sa + LA::kBytes;
+        multiply(f1);
         // the two passes over fine halves are corrections, finite for finite operands: where an infinity or a NaN
         // made them anything else, the coarse pass alone says what comes out
         if (kF32 && s == 2 * (last - first))
@@ -403,30 +438,16 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(const Product<T> p
 #pragma unroll
                     for (int u = 0; u < 4; ++u)
                         acc[i][j][u] = __builtin_isfinite(acc[i][j][u]) ? acc[i][j][u] : 0.f;
-#pragma unroll
-        for (int half = 0; half < 2; ++half)
-        {
-            s8v fa[FM], fb[FN];
-#pragma unroll
-            for (int i = 0; i < FM; ++i)
-                fa[i] = fragment<AC, AC ? 2 : 0, LA::kChunks>(sa, wm * FM * 16 + i * 16 + i16,
-                                                             wm * FM * 16 + i * 16 + (lane % 4) * 4, half, lane);
-#pragma unroll
-            for (int j = 0; j < FN; ++j)
-                fb[j] = fragment<BC, BC ? 2 : 1, LB::kChunks>(sb, wn * FN * 16 + row_of_b(j, i16),
-                                                             wn * FN * 16 + row_of_b(j, (lane % 4) * 4), half, lane);
-#pragma unroll
-            for (int i = 0; i < FM; ++i)
-#pragma unroll
-                for (int j = 0; j < FN; ++j)
-                    acc[i][j] = mfma_16x16x32(fb[j], fa[i], acc[i][j], Kind());
-        }
+        fetch(f1, s & 1, 1);
+        multiply(f0);
     }
+    if (count > 0)
+        multiply(f1);
 
 #pragma unroll
     for (int i = 0; i < FM; ++i)
     {
-        const int64_t r = m0 + wm * FM * 16 + i * 16 + i16;
+        const int64_t r = m0 + wm * FM * 16 + i * 16 + lane % 16;
         if (r >= p.e.m)
             continue;
         const int sr = kF32 ? p.scale_a[r] : 0;
