@@ -2,7 +2,7 @@
 //
 //   z = x w^T + b, y = act(z) + residual                          x [rows, in], w [out, in], y [rows, out]
 //   dz = g act'(z), dx = dz w, dw = dz^T x, db = sum over rows of dz, dresidual = g
-#include "miq_product.h"
+#include "miq_few_rows.h"
 
 #include <algorithm>
 
@@ -45,89 +45,183 @@ __device__ __forceinline__ uint32_t finite_magnitude(float x)
     return b < 0x7f800000u ? b : 0u;
 }
 
-// out[r][0 .. kp) = src[r][0 .. k), zeros behind; float32: out[r][0 .. kp) coarse, out[r][kp .. 2 kp) fine, scale[r] = -s
-template <typename T>
-__global__ __launch_bounds__(kBlock) void pack_rows_kernel(const T* __restrict__ src, int64_t k, int64_t kp,
-                                                           uint16_t* __restrict__ out, int* __restrict__ scale)
+// 8 values as 16-bit operands
+__device__ __forceinline__ void put_parts(const float* v, int shift, uint16_t* coarse, uint16_t* fine)
 {
-    const int64_t r = blockIdx.x;
-    const T* from   = src + r * k;
-    if constexpr (std::is_same<T, float>::value)
-    {
-        __shared__ uint32_t lds[kBlock / 64];
-        uint32_t largest = 0;
-        for (int64_t c = threadIdx.x; c < k; c += kBlock)
-            largest = max(largest, finite_magnitude(from[c]));
+    uint16_t c[8], f[8];
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1)
-            largest = max(largest, (uint32_t) __shfl_xor((int) largest, o, 64));
+    for (int u = 0; u < 8; ++u)
+        split_value(v[u], shift, c + u, f + u);
+    *(uint4*) coarse = make_uint4(c[0] | c[1] << 16, c[2] | c[3] << 16, c[4] | c[5] << 16, c[6] | c[7] << 16);
+    *(uint4*) fine   = make_uint4(f[0] | f[1] << 16, f[2] | f[3] << 16, f[4] | f[5] << 16, f[6] | f[7] << 16);
+}
+__device__ __forceinline__ void put_values(const uint16_t* v, uint16_t* to)
+{
+    *(uint4*) to = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
+}
+
+// out[r][0 .. kp) = src[r][0 .. k), zeros behind; float32: out[r][0 .. kp) coarse, out[r][kp .. 2 kp) fine, scale[r] = -s.
+// LANES threads hold a row of up to 32 LANES values in registers between its largest value and its halves; of a longer
+// one what is past them is read again.
+template <int LANES>
+__global__ __launch_bounds__(kBlock) void pack_rows_kernel(const float* __restrict__ src, int64_t rows, int64_t k,
+                                                           int64_t kp, uint16_t* __restrict__ out,
+                                                           int* __restrict__ scale)
+{
+    constexpr int kHeld = 4;
+    const int lane  = threadIdx.x % LANES;
+    const int64_t r = (int64_t) blockIdx.x * (kBlock / LANES) + threadIdx.x / LANES;
+    if (r >= rows)
+        return;
+    const float* from = src + r * k;
+    float v[kHeld][8], t[8];
+    uint32_t largest = 0;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+        load8(from + (i * LANES + lane) * 8, k - (i * LANES + lane) * 8, v[i]);
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            largest = max(largest, finite_magnitude(v[i][u]));
+    for (int64_t c = (kHeld * LANES + lane) * 8; c < k; c += LANES * 8)
+    {
+        load8(from + c, k - c, t);
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            largest = max(largest, finite_magnitude(t[u]));
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1)
+        largest = max(largest, (uint32_t) __shfl_xor((int) largest, o, 64));
+    if constexpr (LANES > 64)
+    {
+        __shared__ uint32_t lds[LANES / 64];
         if ((threadIdx.x & 63) == 0)
             lds[threadIdx.x >> 6] = largest;
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < kBlock / 64; ++i)
+        for (int i = 0; i < LANES / 64; ++i)
             largest = max(largest, lds[i]);
-        const int shift = row_shift(largest);
-        uint16_t* to    = out + r * 2 * kp;
-        for (int64_t c = threadIdx.x; c < kp; c += kBlock)
-            split_value(c < k ? from[c] : 0.f, shift, to + c, to + kp + c);
-        if (threadIdx.x == 0)
-            scale[r] = -shift;
     }
-    else
-        for (int64_t c = threadIdx.x; c < kp; c += kBlock)
-            out[r * kp + c] = c < k ? from[c] : (uint16_t) 0;
+    const int shift = row_shift(largest);
+    uint16_t* to    = out + r * 2 * kp;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+    {
+        const int64_t c = (i * LANES + lane) * 8;
+        if (c < kp)
+            put_parts(v[i], shift, to + c, to + kp + c);
+    }
+    for (int64_t c = (kHeld * LANES + lane) * 8; c < kp; c += LANES * 8)
+    {
+        load8(from + c, k - c, t);
+        put_parts(t, shift, to + c, to + kp + c);
+    }
+    if (lane == 0)
+        scale[r] = -shift;
 }
 
-__global__ __launch_bounds__(kBlock) void clear_kernel(uint32_t* p, int64_t n)
+__global__ __launch_bounds__(kBlock) void copy_rows_kernel(const uint16_t* __restrict__ src, int64_t rows, int64_t k,
+                                                           int64_t kp, uint16_t* __restrict__ out)
 {
-    const int64_t i = (int64_t) blockIdx.x * kBlock + threadIdx.x;
-    if (i < n)
-        p[i] = 0;
+    const int64_t per = kp / 8, at = (int64_t) blockIdx.x * kBlock + threadIdx.x;
+    if (at >= rows * per)
+        return;
+    const int64_t r = at / per, c = at % per * 8;
+    uint16_t v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+        v[u] = c + u < k ? src[r * k + c + u] : (uint16_t) 0;
+    put_values(v, out + r * kp + c);
 }
 
-// largest[c] = largest finite magnitude of column c of src [k][count] (bits; cleared before)
+// largest[slice][c] = largest finite magnitude (its bits) in a slice of the rows of column c of src [k][count]: 64 threads
+// of 4 columns across, 4 rows at a time
 __global__ __launch_bounds__(kBlock) void column_max_kernel(const float* __restrict__ src, int64_t k, int64_t count,
                                                             int64_t rows_per_slice, uint32_t* __restrict__ largest)
 {
-    const int64_t c = (int64_t) blockIdx.x * kBlock + threadIdx.x;
-    if (c >= count)
-        return;
+    __shared__ uint32_t lds[4][256];
+    const int across    = threadIdx.x % 64, down = threadIdx.x / 64;
+    const int64_t c     = ((int64_t) blockIdx.x * 64 + across) * 4;
     const int64_t first = blockIdx.y * rows_per_slice;
     const int64_t last  = first + rows_per_slice < k ? first + rows_per_slice : k;
-    uint32_t m          = 0;
-    for (int64_t r = first; r < last; ++r)
-        m = max(m, finite_magnitude(src[r * count + c]));
-    atomicMax(largest + c, m);   // a maximum is the same in any order
+    uint32_t m[4]       = {};
+    if (c + 4 <= count)
+    {
+#pragma unroll 4
+        for (int64_t r = first + down; r < last; r += 4)
+        {
+            float v[4];
+            load_any(src + r * count + c, v);
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                m[u] = max(m[u], finite_magnitude(v[u]));
+        }
+    }
+    else
+        for (int64_t r = first + down; r < last; r += 4)
+            for (int u = 0; u < 4; ++u)
+                if (c + u < count)
+                    m[u] = max(m[u], finite_magnitude(src[r * count + c + u]));
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+        lds[down][u * 64 + across] = m[u];
+    __syncthreads();
+    const int at = threadIdx.x % 4 * 64 + threadIdx.x / 4;   // column threadIdx.x of the block's 256
+    const int64_t q = (int64_t) blockIdx.x * 256 + threadIdx.x;
+    if (q < count)
+        largest[blockIdx.y * count + q] = max(max(lds[0][at], lds[1][at]), max(lds[2][at], lds[3][at]));
 }
 
-// as pack_rows_kernel, of the transpose: src [k][count], row r of the result is column r of src
+// As pack_rows_kernel and copy_rows_kernel, of the transpose: src [k][count], row r of the result is column r of src.
+// 64 x 64 values a block, through LDS.
 template <typename T>
 __global__ __launch_bounds__(kBlock) void pack_columns_kernel(const T* __restrict__ src, int64_t k, int64_t count,
                                                               int64_t kp, const uint32_t* __restrict__ largest,
-                                                              uint16_t* __restrict__ out, int* __restrict__ scale)
+                                                              int slices, uint16_t* __restrict__ out,
+                                                              int* __restrict__ scale)
 {
     __shared__ T tile[64][65];
+    __shared__ int shifts[64];
     const int64_t across = (count + 63) / 64;
     const int64_t r0 = blockIdx.x % across * 64, k0 = blockIdx.x / across * 64;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int i = wave; i < 64; i += kBlock / 64)
-        tile[i][lane] = k0 + i < k && r0 + lane < count ? src[(k0 + i) * count + r0 + lane] : (T) 0;
-    __syncthreads();
-    for (int i = wave; i < 64; i += kBlock / 64)
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
     {
-        const int64_t r = r0 + i, c = k0 + lane;
-        if (r >= count || c >= kp)
+        const int64_t kk = k0 + i * 4 + wave;
+        tile[i * 4 + wave][lane] = kk < k && r0 + lane < count ? src[kk * count + r0 + lane] : (T) 0;
+    }
+    if constexpr (std::is_same<T, float>::value)
+        if (threadIdx.x < 64)
+        {
+            uint32_t m = 0;
+            if (r0 + lane < count)
+                for (int i = 0; i < slices; ++i)
+                    m = max(m, largest[i * count + r0 + lane]);
+            shifts[lane] = row_shift(m);
+            if (k0 == 0 && r0 + lane < count)
+                scale[r0 + lane] = -row_shift(m);
+        }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+    {
+        const int r = (i * kBlock + threadIdx.x) / 8, c = threadIdx.x % 8 * 8;
+        if (r0 + r >= count || k0 + c >= kp)
             continue;
+        T v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            v[u] = tile[c + u][r];
         if constexpr (std::is_same<T, float>::value)
         {
-            const int shift = row_shift(largest[r]);
-            split_value(tile[lane][i], shift, out + r * 2 * kp + c, out + r * 2 * kp + kp + c);
-            if (c == 0)
-                scale[r] = -shift;
+            uint16_t* to = out + (r0 + r) * 2 * kp + k0 + c;
+            put_parts(v, shifts[r], to, to + kp);
         }
         else
-            out[r * kp + c] = tile[lane][i];
+            put_values(v, out + (r0 + r) * kp + k0 + c);
     }
 }
 
@@ -249,8 +343,15 @@ struct Matrix
     bool columns;
 };
 
+int64_t max_slices(int64_t k)
+{
+    return std::max<int64_t>(1, std::min<int64_t>(32, k / 16));
+}
+
 struct Plan
 {
+    bool few, few_columns;    // few rows: b is read as it lies, by the kernels of miq_few_rows.h
+    bool short_sum;           // float32, both in columns, k short
     bool pack_a, pack_b;
     int64_t kp;               // length of packed rows
     bool big;                 // 256 x 256 tiles, else 128 x 128
@@ -266,6 +367,25 @@ Plan plan_product(const Matrix<T>& a, const Matrix<T>& b, bool at_any_address)
     constexpr bool kF32 = std::is_same<T, float>::value;
     Plan p              = {};
     const int64_t m = a.count, n = b.count, k = a.k;
+    const auto ragged = [&](const Matrix<T>& x) {
+        return (x.columns ? x.count : x.k) % 8 != 0 || (x.p && !aligned(x.p));
+    };
+    p.few       = !a.columns && !b.columns && m <= (kF32 ? 64 : 16);
+    p.short_sum = kF32 && a.columns && b.columns && k <= 64;
+    if (p.few || p.short_sum)
+        return p;
+    // about 2048 waves in blocks of 8; pieces of k of 128 at least
+    const bool low         = !a.columns && b.columns && m <= (kF32 ? 64 : 16);
+    const int64_t wide     = (n + 16 * IOTraits<T>::VEC - 1) / (16 * IOTraits<T>::VEC);
+    const int64_t pieces   = std::max<int64_t>(1, std::min<int64_t>(256 / std::max<int64_t>(wide, 1), k / 128));
+    const int64_t low_size = low && pieces > 1 ? up256(pieces * m * n * 4) : 0;
+    p.few_columns          = low && (kF32 || ragged(b));
+    if (p.few_columns)
+    {
+        p.splits  = (int) pieces;
+        p.partial = p.total = low_size;
+        return p;
+    }
     const auto odd = [&](const Matrix<T>& x) {
         return kF32 || (x.columns ? x.count : x.k) % 8 != 0 || at_any_address || !aligned(x.p);
     };
@@ -279,9 +399,12 @@ Plan plan_product(const Matrix<T>& a, const Matrix<T>& b, bool at_any_address)
     p.splits = p.big ? 1 : (int) std::max<int64_t>(1, std::min<int64_t>(512 / std::max<int64_t>(small, 1), slices / 8));
     const int64_t each = (kF32 ? 2 : 1) * p.kp * 2;
     p.a_bytes = p.pack_a ? up256(m * each) : 0, p.b_bytes = p.pack_b ? up256(n * each) : 0;
-    p.scale_a = kF32 ? up256(m * 8) : 0, p.scale_b = kF32 ? up256(n * 8) : 0;
+    p.scale_a = kF32 ? up256(m * 4 * (1 + (a.columns ? max_slices(k) : 0))) : 0;
+    p.scale_b = kF32 ? up256(n * 4 * (1 + (b.columns ? max_slices(k) : 0))) : 0;
     p.partial = p.splits > 1 ? up256(p.splits * m * n * 4) : 0;
     p.total   = p.a_bytes + p.b_bytes + p.scale_a + p.scale_b + p.partial;
+    if (at_any_address)
+        p.total = std::max(p.total, low_size);
     return p;
 }
 
@@ -294,25 +417,36 @@ int pack(const Matrix<T>& x, int64_t kp, char* to, char* scale, hipStream_t s)
     uint32_t* largest = (uint32_t*) scale + x.count;
     if (!x.columns)
     {
-        hipLaunchKernelGGL(pack_rows_kernel<T>, dim3((unsigned) x.count), dim3(kBlock), 0, s, x.p, x.k, kp,
-                           (uint16_t*) to, exponents);
+        if constexpr (std::is_same<T, float>::value)
+        {
+            if (x.k <= 2048)
+                hipLaunchKernelGGL(pack_rows_kernel<64>, dim3((unsigned) ((x.count + 3) / 4)), dim3(kBlock), 0, s, x.p,
+                                   x.count, x.k, kp, (uint16_t*) to, exponents);
+            else
+                hipLaunchKernelGGL(pack_rows_kernel<256>, dim3((unsigned) x.count), dim3(kBlock), 0, s, x.p, x.count,
+                                   x.k, kp, (uint16_t*) to, exponents);
+        }
+        else
+        {
+            const int64_t blocks = (x.count * (kp / 8) + kBlock - 1) / kBlock;
+            MIQ_CHECK_ARG(blocks <= INT32_MAX, "an operand is too large");
+            hipLaunchKernelGGL(copy_rows_kernel, dim3((unsigned) blocks), dim3(kBlock), 0, s, x.p, x.count, x.k, kp,
+                               (uint16_t*) to);
+        }
         MIQ_CHECK_LAUNCH();
         return MIQ_OK;
     }
+    const int64_t slices = max_slices(x.k);
     if constexpr (std::is_same<T, float>::value)
     {
-        const unsigned columns = (unsigned) ((x.count + kBlock - 1) / kBlock);
-        hipLaunchKernelGGL(clear_kernel, dim3(columns), dim3(kBlock), 0, s, largest, x.count);
-        MIQ_CHECK_LAUNCH();
-        const int64_t slices = slope_slices(x.k, x.count);
-        hipLaunchKernelGGL(column_max_kernel, dim3(columns, (unsigned) slices), dim3(kBlock), 0, s, x.p, x.k, x.count,
-                           (x.k + slices - 1) / slices, largest);
+        hipLaunchKernelGGL(column_max_kernel, dim3((unsigned) ((x.count + 255) / 256), (unsigned) slices), dim3(kBlock), 0,
+                           s, x.p, x.k, x.count, (x.k + slices - 1) / slices, largest);
         MIQ_CHECK_LAUNCH();
     }
     const int64_t tiles = ((x.count + 63) / 64) * ((kp + 63) / 64);
     MIQ_CHECK_ARG(tiles <= INT32_MAX, "an operand has too many tiles");
     hipLaunchKernelGGL(pack_columns_kernel<T>, dim3((unsigned) tiles), dim3(kBlock), 0, s, x.p, x.k, x.count, kp,
-                       largest, (uint16_t*) to, exponents);
+                       largest, (int) slices, (uint16_t*) to, exponents);
     MIQ_CHECK_LAUNCH();
     return MIQ_OK;
 }
@@ -339,6 +473,39 @@ int launch_product(Product<T>& p, bool big, hipStream_t s)
     return MIQ_OK;
 }
 
+template <typename T, int ACT, int MT, int NT>
+int launch_few_rows(const T* a, const T* b, int64_t k, const Epilogue<T>& e, hipStream_t s)
+{
+    // about 2048 waves, each with 8 steps of k or more
+    const int64_t blocks = (e.n + 16 * NT - 1) / (16 * NT);
+    int waves            = 4;
+    while (waves < (MT == 1 ? 16 : 8) && blocks * waves < 2048 && k / (4 * Chunk<T>::VEC) / (2 * waves) >= 8)
+        waves *= 2;
+    hipLaunchKernelGGL((few_rows_kernel<T, ACT, MT, NT>), dim3((unsigned) blocks), dim3(waves * 64),
+                       waves * MT * NT * 1024, s, a, b, k, e);
+    MIQ_CHECK_LAUNCH();
+    return MIQ_OK;
+}
+
+template <typename T, int MT>
+int launch_few_rows_columns(const Matrix<T>& a, const Matrix<T>& b, const Plan& plan, float* partial,
+                            const Epilogue<T>& e, hipStream_t s)
+{
+    constexpr int VEC  = IOTraits<T>::VEC, kWaves = 8;
+    const int64_t wide = (b.count + 16 * VEC - 1) / (16 * VEC), per = (a.k + plan.splits - 1) / plan.splits;
+    hipLaunchKernelGGL((few_rows_columns_kernel<T, MT>), dim3((unsigned) wide, (unsigned) plan.splits), dim3(kWaves * 64),
+                       kWaves * MT * VEC * 1024, s, a.p, b.p, a.k, per, plan.splits > 1 ? partial : nullptr, e);
+    MIQ_CHECK_LAUNCH();
+    if (plan.splits > 1)
+    {
+        const int64_t groups = (e.n + 7) / 8 * e.m;
+        hipLaunchKernelGGL((join_kernel<T, MIQ_ACT_NONE>), dim3((unsigned) ((groups + kBlock - 1) / kBlock)),
+                           dim3(kBlock), 0, s, partial, plan.splits, e);
+        MIQ_CHECK_LAUNCH();
+    }
+    return MIQ_OK;
+}
+
 // c[m, n] = act(sum over k of a(m, k) b(n, k) + bias) + residual
 template <typename T, int ACT>
 int product(const Matrix<T>& a, const Matrix<T>& b, const T* bias, const T* residual, T* c, Saved<T>* saved,
@@ -348,6 +515,36 @@ int product(const Matrix<T>& a, const Matrix<T>& b, const T* bias, const T* resi
         return MIQ_OK;
     const Plan plan = plan_product(a, b, false);
     Product<T> p    = {};
+    p.e             = {bias, residual, c, saved, a.count, b.count};
+    if (plan.few)
+    {
+        if (a.count <= 16)
+            return launch_few_rows<T, ACT, 1, 1>(a.p, b.p, a.k, p.e, s);
+        if constexpr (std::is_same<T, float>::value)
+            return a.count <= 32 ? launch_few_rows<T, ACT, 2, 2>(a.p, b.p, a.k, p.e, s)
+                                 : launch_few_rows<T, ACT, 4, 2>(a.p, b.p, a.k, p.e, s);
+    }
+    if constexpr (ACT == MIQ_ACT_NONE)
+    {
+        if (plan.few_columns)
+        {
+            if (a.count <= 16)
+                return launch_few_rows_columns<T, 1>(a, b, plan, (float*) workspace, p.e, s);
+            if constexpr (std::is_same<T, float>::value)
+                return a.count <= 32 ? launch_few_rows_columns<T, 2>(a, b, plan, (float*) workspace, p.e, s)
+                                     : launch_few_rows_columns<T, 4>(a, b, plan, (float*) workspace, p.e, s);
+        }
+        if constexpr (std::is_same<T, float>::value)
+            if (plan.short_sum)
+            {
+                const int64_t tiles = ((p.e.m + 127) / 128) * ((p.e.n + 127) / 128);
+                MIQ_CHECK_ARG(tiles <= INT32_MAX, "the product has too many tiles");
+                hipLaunchKernelGGL(short_sum_kernel, dim3((unsigned) tiles), dim3(kBlock), 0, s, a.p, b.p, (int) a.k,
+                                   p.e);
+                MIQ_CHECK_LAUNCH();
+                return MIQ_OK;
+            }
+    }
     char* const pa = workspace;
     char* const pb = pa + plan.a_bytes;
     char* const sa = pb + plan.b_bytes;
@@ -371,7 +568,6 @@ int product(const Matrix<T>& a, const Matrix<T>& b, const T* bias, const T* resi
     p.scale_a = (const int*) sa, p.scale_b = (const int*) sb;
     p.splits  = plan.splits;
     p.partial = (float*) (sb + plan.scale_b);
-    p.e       = {bias, residual, c, saved, a.count, b.count};
     if constexpr (std::is_same<T, float>::value)
         return launch_product<T, ACT, false, false>(p, plan.big, s);
     else
