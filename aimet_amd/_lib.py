@@ -151,7 +151,7 @@ _SIGNATURES = {
     "miq_layer_norm_fwd_bf16": ([_p, _p, _p, _i64, _i64, _flt, _p, _p, _p, _p], _int),
     "miq_layer_norm_bwd_f32": ([_p, _p, _p, _p, _p, _i64, _i64, _p, _p, _p, _p, _p], _int),
     "miq_layer_norm_bwd_bf16": ([_p, _p, _p, _p, _p, _i64, _i64, _p, _p, _p, _p, _p], _int),
-    "miq_linear_workspace_bytes": ([_i64, _i64, _i64, _int, _int, _int], _i64),
+    "miq_linear_workspace_bytes": ([_i64, _i64, _i64, _int, _int, _int, _int], _i64),
     "miq_linear_fwd_f32": ([_p, _p, _p, _p, _i64, _i64, _i64, _int, _p, _p, _p, _i64, _p], _int),
     "miq_linear_fwd_bf16": ([_p, _p, _p, _p, _i64, _i64, _i64, _int, _p, _p, _p, _i64, _p], _int),
     "miq_linear_bwd_f32": ([_p, _p, _p, _p, _i64, _i64, _i64, _int, _p, _p, _p, _p, _i64, _p], _int),

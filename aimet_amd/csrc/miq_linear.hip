@@ -2,6 +2,7 @@
 //
 //   z = x w^T + b, y = act(z) + residual                          x [rows, in], w [out, in], y [rows, out]
 //   dz = g act'(z), dx = dz w, dw = dz^T x, db = sum over rows of dz, dresidual = g
+#include "miq_direct.h"
 #include "miq_few_rows.h"
 
 #include <algorithm>
@@ -122,18 +123,24 @@ __global__ __launch_bounds__(kBlock) void pack_rows_kernel(const float* __restri
         scale[r] = -shift;
 }
 
-__global__ __launch_bounds__(kBlock) void copy_rows_kernel(const uint16_t* __restrict__ src, int64_t rows, int64_t k,
-                                                           int64_t kp, uint16_t* __restrict__ out)
+// out[r][0 .. kp) = src[r][0 .. k), zeros behind
+template <typename T>
+__global__ __launch_bounds__(kBlock) void copy_rows_kernel(const T* __restrict__ src, int64_t rows, int64_t k,
+                                                           int64_t kp, T* __restrict__ out)
 {
-    const int64_t per = kp / 8, at = (int64_t) blockIdx.x * kBlock + threadIdx.x;
+    constexpr int VEC = IOTraits<T>::VEC;
+    const int64_t per = kp / VEC, at = (int64_t) blockIdx.x * kBlock + threadIdx.x;
     if (at >= rows * per)
         return;
-    const int64_t r = at / per, c = at % per * 8;
-    uint16_t v[8];
+    const int64_t r = at / per, c = at % per * VEC;
+    T v[VEC];
 #pragma unroll
-    for (int u = 0; u < 8; ++u)
-        v[u] = c + u < k ? src[r * k + c + u] : (uint16_t) 0;
-    put_values(v, out + r * kp + c);
+    for (int u = 0; u < VEC; ++u)
+        v[u] = c + u < k ? src[r * k + c + u] : (T) 0;
+    if constexpr (VEC == 8)
+        put_values(v, out + r * kp + c);
+    else
+        *(float4*) (out + r * kp + c) = make_float4(v[0], v[1], v[2], v[3]);
 }
 
 // largest[slice][c] = largest finite magnitude (its bits) in a slice of the rows of column c of src [k][count]: 64 threads
@@ -341,71 +348,123 @@ struct Matrix
     const T* p;
     int64_t count, k;
     bool columns;
+    bool at16;   // p is a multiple of 16 bytes
+
+    int64_t inner() const
+    {
+        return columns ? count : k;
+    }
+    int64_t outer() const
+    {
+        return columns ? k : count;
+    }
+    bool whole() const   // every row is whole 16-byte chunks
+    {
+        return at16 && inner() * (int64_t) sizeof(T) % 16 == 0;
+    }
 };
+
+int64_t up4(int64_t n)
+{
+    return (n + 3) / 4 * 4;
+}
 
 int64_t max_slices(int64_t k)
 {
     return std::max<int64_t>(1, std::min<int64_t>(32, k / 16));
 }
 
+#ifdef MIQ_TUNE
+int64_t direct_most() { static const char* e = getenv("DIRECT"); return e ? atoi(e) : 500; }
+#else
+int64_t direct_most() { return 500; }
+#endif
+
+enum class Way
+{
+    kFewRows,      // few rows: b is read as it lies, by the kernels of miq_few_rows.h
+    kFewColumns,   // the same, b in columns
+    kShortSum,     // float32, both in columns, k short
+    kDirect,       // float32, from the operands as they lie
+    kTiles         // 16-bit operands
+};
+
 struct Plan
 {
-    bool few, few_columns;    // few rows: b is read as it lies, by the kernels of miq_few_rows.h
-    bool short_sum;           // float32, both in columns, k short
+    Way way;
     bool pack_a, pack_b;
-    int64_t kp;               // length of packed rows
-    bool big;                 // 256 x 256 tiles, else 128 x 128
+    int64_t kp;   // length of packed rows
+    bool big;     // 256 x 256 tiles, else 128 x 128 (kDirect: 128 x 128, else 64 x 128)
     int splits;
     int64_t a_bytes, b_bytes, scale_a, scale_b, partial, total;   // of the workspace
 };
 
-// bfloat16 operands whose rows are whole 16-byte chunks are read as they lie.  `at_any_address`: for the size of a
-// workspace, which is asked for before the addresses are known.
 template <typename T>
-Plan plan_product(const Matrix<T>& a, const Matrix<T>& b, bool at_any_address)
+Plan plan_product(const Matrix<T>& a, const Matrix<T>& b)
 {
     constexpr bool kF32 = std::is_same<T, float>::value;
     Plan p              = {};
+    p.splits            = 1;
     const int64_t m = a.count, n = b.count, k = a.k;
-    const auto ragged = [&](const Matrix<T>& x) {
-        return (x.columns ? x.count : x.k) % 8 != 0 || (x.p && !aligned(x.p));
-    };
-    p.few       = !a.columns && !b.columns && m <= (kF32 ? 64 : 16);
-    p.short_sum = kF32 && a.columns && b.columns && k <= 64;
-    if (p.few || p.short_sum)
+    const auto done = [&] {
+        p.partial = p.splits > 1 ? up256(p.splits * m * n * 4) : 0;
+        p.total   = p.a_bytes + p.b_bytes + p.scale_a + p.scale_b + p.partial;
         return p;
-    // about 2048 waves in blocks of 8; pieces of k of 128 at least
-    const bool low         = !a.columns && b.columns && m <= (kF32 ? 64 : 16);
-    const int64_t wide     = (n + 16 * IOTraits<T>::VEC - 1) / (16 * IOTraits<T>::VEC);
-    const int64_t pieces   = std::max<int64_t>(1, std::min<int64_t>(256 / std::max<int64_t>(wide, 1), k / 128));
-    const int64_t low_size = low && pieces > 1 ? up256(pieces * m * n * 4) : 0;
-    p.few_columns          = low && (kF32 || ragged(b));
-    if (p.few_columns)
+    };
+    const auto tiles = [&](int64_t tm, int64_t tn) { return (m + tm - 1) / tm * ((n + tn - 1) / tn); };
+    if (!a.columns && !b.columns && m <= 16)
     {
-        p.splits  = (int) pieces;
-        p.partial = p.total = low_size;
-        return p;
+        p.way = Way::kFewRows;
+        return done();
     }
-    const auto odd = [&](const Matrix<T>& x) {
-        return kF32 || (x.columns ? x.count : x.k) % 8 != 0 || at_any_address || !aligned(x.p);
-    };
-    p.pack_a = odd(a), p.pack_b = odd(b);
+    if (!a.columns && b.columns && m <= 16 && (kF32 || !b.whole()))
+    {
+        // about 2048 waves in blocks of 8; pieces of k of 128 at least
+        const int64_t wide = (n + 16 * IOTraits<T>::VEC - 1) / (16 * IOTraits<T>::VEC);
+        p.way    = Way::kFewColumns;
+        p.splits = (int) std::max<int64_t>(1, std::min<int64_t>(256 / std::max<int64_t>(wide, 1), k / 128));
+        return done();
+    }
+    if (kF32 && a.columns && b.columns && k <= 16)
+    {
+        p.way = Way::kShortSum;
+        return done();
+    }
+    if (kF32 && m * n <= direct_most() * (m + n))
+    {
+        p.way = Way::kDirect;
+        // rows that are not whole chunks are copied, with zeros behind them
+        const auto copied = [&](const Matrix<T>& x) { return x.whole() ? 0 : up256(x.outer() * up4(x.inner()) * 4); };
+        p.a_bytes = copied(a), p.b_bytes = copied(b);
+        p.big = m > 64;
+        p.splits = (int) std::max<int64_t>(1, std::min<int64_t>(512 / std::max<int64_t>(tiles(p.big ? 128 : 64, 128), 1), k / 256));
+        return done();
+    }
+    p.way    = Way::kTiles;
+    p.pack_a = kF32 || !a.whole(), p.pack_b = kF32 || !b.whole();
     if (a.columns && (p.pack_a || p.pack_b))
         p.pack_a = p.pack_b = true;   // both in columns, or both in rows
-    p.kp = kF32 ? (k + kSlice - 1) / kSlice * kSlice : (k + 7) / 8 * 8;
-    const int64_t big = ((m + 255) / 256) * ((n + 255) / 256), small = ((m + 127) / 128) * ((n + 127) / 128);
-    p.big               = big >= 200;
-    const int64_t slices = (k + kSlice - 1) / kSlice;
-    p.splits = p.big ? 1 : (int) std::max<int64_t>(1, std::min<int64_t>(512 / std::max<int64_t>(small, 1), slices / 8));
+    p.kp  = kF32 ? (k + kSlice - 1) / kSlice * kSlice : (k + 7) / 8 * 8;
+    p.big = tiles(256, 256) >= 200;
+    if (!p.big)
+        p.splits = (int) std::max<int64_t>(1, std::min<int64_t>(512 / std::max<int64_t>(tiles(128, 128), 1), (k + kSlice - 1) / kSlice / 8));
     const int64_t each = (kF32 ? 2 : 1) * p.kp * 2;
     p.a_bytes = p.pack_a ? up256(m * each) : 0, p.b_bytes = p.pack_b ? up256(n * each) : 0;
     p.scale_a = kF32 ? up256(m * 4 * (1 + (a.columns ? max_slices(k) : 0))) : 0;
     p.scale_b = kF32 ? up256(n * 4 * (1 + (b.columns ? max_slices(k) : 0))) : 0;
-    p.partial = p.splits > 1 ? up256(p.splits * m * n * 4) : 0;
-    p.total   = p.a_bytes + p.b_bytes + p.scale_a + p.scale_b + p.partial;
-    if (at_any_address)
-        p.total = std::max(p.total, low_size);
-    return p;
+    return done();
+}
+
+template <typename T>
+int copy_rows(const T* src, int64_t rows, int64_t k, int64_t kp, T* to, hipStream_t s)
+{
+    const int64_t blocks = (rows * (kp / IOTraits<T>::VEC) + kBlock - 1) / kBlock;
+    if (blocks == 0)
+        return MIQ_OK;
+    MIQ_CHECK_ARG(blocks <= INT32_MAX, "an operand is too large");
+    hipLaunchKernelGGL(copy_rows_kernel<T>, dim3((unsigned) blocks), dim3(kBlock), 0, s, src, rows, k, kp, to);
+    MIQ_CHECK_LAUNCH();
+    return MIQ_OK;
 }
 
 template <typename T>
@@ -428,10 +487,8 @@ int pack(const Matrix<T>& x, int64_t kp, char* to, char* scale, hipStream_t s)
         }
         else
         {
-            const int64_t blocks = (x.count * (kp / 8) + kBlock - 1) / kBlock;
-            MIQ_CHECK_ARG(blocks <= INT32_MAX, "an operand is too large");
-            hipLaunchKernelGGL(copy_rows_kernel, dim3((unsigned) blocks), dim3(kBlock), 0, s, x.p, x.count, x.k, kp,
-                               (uint16_t*) to);
+            if (int rc = copy_rows(x.p, x.count, x.k, kp, (uint16_t*) to, s))
+                return rc;
         }
         MIQ_CHECK_LAUNCH();
         return MIQ_OK;
@@ -451,6 +508,18 @@ int pack(const Matrix<T>& x, int64_t kp, char* to, char* scale, hipStream_t s)
     return MIQ_OK;
 }
 
+template <typename T, int ACT>
+int launch_join(const float* partial, int splits, const Epilogue<T>& e, hipStream_t s)
+{
+    if (splits == 1)
+        return MIQ_OK;
+    const int64_t groups = (e.n + 7) / 8 * e.m;
+    hipLaunchKernelGGL((join_kernel<T, ACT>), dim3((unsigned) ((groups + kBlock - 1) / kBlock)), dim3(kBlock), 0, s,
+                       partial, splits, e);
+    MIQ_CHECK_LAUNCH();
+    return MIQ_OK;
+}
+
 template <typename T, int ACT, bool AC, bool BC>
 int launch_product(Product<T>& p, bool big, hipStream_t s)
 {
@@ -463,14 +532,21 @@ int launch_product(Product<T>& p, bool big, hipStream_t s)
     else
         hipLaunchKernelGGL((product_kernel<T, ACT, 2, 2, 4, 4, AC, BC>), dim3((unsigned) blocks), dim3(256), 0, s, p);
     MIQ_CHECK_LAUNCH();
-    if (p.splits > 1)
-    {
-        const int64_t groups = (p.e.n + 7) / 8 * p.e.m;
-        hipLaunchKernelGGL((join_kernel<T, ACT>), dim3((unsigned) ((groups + kBlock - 1) / kBlock)), dim3(kBlock), 0, s,
-                           p.partial, p.splits, p.e);
-        MIQ_CHECK_LAUNCH();
-    }
-    return MIQ_OK;
+    return launch_join<T, ACT>(p.partial, p.splits, p.e, s);
+}
+
+template <int ACT, bool AC, bool BC>
+int launch_direct(DirectProduct& p, bool big, hipStream_t s)
+{
+    p.tiles_m = (int) ((p.e.m + (big ? 127 : 63)) / (big ? 128 : 64)), p.tiles_n = (int) ((p.e.n + 127) / 128);
+    const int64_t blocks = (int64_t) p.tiles_m * p.tiles_n * p.splits;
+    MIQ_CHECK_ARG(blocks <= INT32_MAX, "the product has too many tiles");
+    if (big)
+        hipLaunchKernelGGL((direct_kernel<ACT, 2, 2, 4, 4, AC, BC>), dim3((unsigned) blocks), dim3(256), 0, s, p);
+    else
+        hipLaunchKernelGGL((direct_kernel<ACT, 1, 4, 4, 2, AC, BC>), dim3((unsigned) blocks), dim3(256), 0, s, p);
+    MIQ_CHECK_LAUNCH();
+    return launch_join<float, ACT>(p.partial, p.splits, p.e, s);
 }
 
 template <typename T, int ACT, int MT, int NT>
@@ -496,14 +572,7 @@ int launch_few_rows_columns(const Matrix<T>& a, const Matrix<T>& b, const Plan& 
     hipLaunchKernelGGL((few_rows_columns_kernel<T, MT>), dim3((unsigned) wide, (unsigned) plan.splits), dim3(kWaves * 64),
                        kWaves * MT * VEC * 1024, s, a.p, b.p, a.k, per, plan.splits > 1 ? partial : nullptr, e);
     MIQ_CHECK_LAUNCH();
-    if (plan.splits > 1)
-    {
-        const int64_t groups = (e.n + 7) / 8 * e.m;
-        hipLaunchKernelGGL((join_kernel<T, MIQ_ACT_NONE>), dim3((unsigned) ((groups + kBlock - 1) / kBlock)),
-                           dim3(kBlock), 0, s, partial, plan.splits, e);
-        MIQ_CHECK_LAUNCH();
-    }
-    return MIQ_OK;
+    return launch_join<T, MIQ_ACT_NONE>(partial, plan.splits, e, s);
 }
 
 // c[m, n] = act(sum over k of a(m, k) b(n, k) + bias) + residual
@@ -513,45 +582,60 @@ int product(const Matrix<T>& a, const Matrix<T>& b, const T* bias, const T* resi
 {
     if (a.count == 0 || b.count == 0)
         return MIQ_OK;
-    const Plan plan = plan_product(a, b, false);
-    Product<T> p    = {};
-    p.e             = {bias, residual, c, saved, a.count, b.count};
-    if (plan.few)
-    {
-        if (a.count <= 16)
-            return launch_few_rows<T, ACT, 1, 1>(a.p, b.p, a.k, p.e, s);
-        if constexpr (std::is_same<T, float>::value)
-            return a.count <= 32 ? launch_few_rows<T, ACT, 2, 2>(a.p, b.p, a.k, p.e, s)
-                                 : launch_few_rows<T, ACT, 4, 2>(a.p, b.p, a.k, p.e, s);
-    }
-    if constexpr (ACT == MIQ_ACT_NONE)
-    {
-        if (plan.few_columns)
+    constexpr bool kF32    = std::is_same<T, float>::value;
+    const Plan plan        = plan_product(a, b);
+    const Epilogue<T> e    = {bias, residual, c, saved, a.count, b.count};
+    [[maybe_unused]] constexpr bool kPlain = ACT == MIQ_ACT_NONE;   // products of the backward pass, and some of the forward's
+    if (plan.way == Way::kFewRows)
+        return launch_few_rows<T, ACT, 1, 1>(a.p, b.p, a.k, e, s);
+    if constexpr (kPlain)
+        if (plan.way == Way::kFewColumns)
+            return launch_few_rows_columns<T, 1>(a, b, plan, (float*) workspace, e, s);
+    if constexpr (kPlain && kF32)
+        if (plan.way == Way::kShortSum)
         {
-            if (a.count <= 16)
-                return launch_few_rows_columns<T, 1>(a, b, plan, (float*) workspace, p.e, s);
-            if constexpr (std::is_same<T, float>::value)
-                return a.count <= 32 ? launch_few_rows_columns<T, 2>(a, b, plan, (float*) workspace, p.e, s)
-                                     : launch_few_rows_columns<T, 4>(a, b, plan, (float*) workspace, p.e, s);
+            const int64_t tiles = ((e.m + 127) / 128) * ((e.n + 127) / 128);
+            MIQ_CHECK_ARG(tiles <= INT32_MAX, "the product has too many tiles");
+            hipLaunchKernelGGL(short_sum_kernel, dim3((unsigned) tiles), dim3(kBlock), 0, s, a.p, b.p, (int) a.k, e);
+            MIQ_CHECK_LAUNCH();
+            return MIQ_OK;
         }
-        if constexpr (std::is_same<T, float>::value)
-            if (plan.short_sum)
+    if constexpr (kF32)
+        if (plan.way == Way::kDirect)
+        {
+            char* at        = workspace;
+            const auto as_read = [&](const Matrix<T>& x, int64_t bytes, Operand<float>* o) {
+                *o = {x.p, x.inner(), x.count};
+                if (x.whole())
+                    return MIQ_OK;
+                *o = {(const float*) at, up4(x.inner()), x.count};
+                at += bytes;
+                return copy_rows(x.p, x.outer(), x.inner(), o->ld, (float*) o->p, s);
+            };
+            DirectProduct p = {{}, {}, a.k, 0, 0, plan.splits, nullptr, e};
+            if (int rc = as_read(a, plan.a_bytes, &p.a))
+                return rc;
+            if (int rc = as_read(b, plan.b_bytes, &p.b))
+                return rc;
+            p.partial = (float*) at;
+            if constexpr (kPlain)
             {
-                const int64_t tiles = ((p.e.m + 127) / 128) * ((p.e.n + 127) / 128);
-                MIQ_CHECK_ARG(tiles <= INT32_MAX, "the product has too many tiles");
-                hipLaunchKernelGGL(short_sum_kernel, dim3((unsigned) tiles), dim3(kBlock), 0, s, a.p, b.p, (int) a.k,
-                                   p.e);
-                MIQ_CHECK_LAUNCH();
-                return MIQ_OK;
+                if (a.columns)
+                    return launch_direct<ACT, true, true>(p, plan.big, s);
+                if (b.columns)
+                    return launch_direct<ACT, false, true>(p, plan.big, s);
             }
-    }
+            return launch_direct<ACT, false, false>(p, plan.big, s);
+        }
+    Product<T> p   = {};
+    p.e            = e;
     char* const pa = workspace;
     char* const pb = pa + plan.a_bytes;
     char* const sa = pb + plan.b_bytes;
     char* const sb = sa + plan.scale_a;
     p.a = {(const uint16_t*) a.p, a.columns ? a.count : a.k, a.count};
     p.b = {(const uint16_t*) b.p, b.columns ? b.count : b.k, b.count};
-    const int64_t ld = (std::is_same<T, float>::value ? 2 : 1) * plan.kp;
+    const int64_t ld = (kF32 ? 2 : 1) * plan.kp;
     if (plan.pack_a)
     {
         if (int rc = pack(a, plan.kp, pa, sa, s))
@@ -568,12 +652,12 @@ int product(const Matrix<T>& a, const Matrix<T>& b, const T* bias, const T* resi
     p.scale_a = (const int*) sa, p.scale_b = (const int*) sb;
     p.splits  = plan.splits;
     p.partial = (float*) (sb + plan.scale_b);
-    if constexpr (std::is_same<T, float>::value)
+    if constexpr (kF32)
         return launch_product<T, ACT, false, false>(p, plan.big, s);
     else
     {
         const bool ac = a.columns && !plan.pack_a, bc = b.columns && !plan.pack_b;
-        if constexpr (ACT == MIQ_ACT_NONE)
+        if constexpr (kPlain)
         {
             if (ac && bc)
                 return launch_product<T, ACT, true, true>(p, plan.big, s);
@@ -584,22 +668,23 @@ int product(const Matrix<T>& a, const Matrix<T>& b, const T* bias, const T* resi
     }
 }
 
+// bytes of the workspace; `at16`: every tensor starts on a multiple of 16 bytes
 template <typename T>
-int64_t product_bytes(int64_t m, int64_t n, int64_t k, bool ac, bool bc)
+int64_t product_bytes(int64_t m, int64_t n, int64_t k, bool ac, bool bc, bool a16, bool b16)
 {
-    if (m == 0 || n == 0)
-        return 0;
-    return plan_product<T>({nullptr, m, k, ac}, {nullptr, n, k, bc}, true).total;
+    return m == 0 || n == 0 ? 0 : plan_product<T>({nullptr, m, k, ac, a16}, {nullptr, n, k, bc, b16}).total;
 }
 
 template <typename T>
-int64_t workspace_bytes(int64_t rows, int64_t in, int64_t out, int activation, int backward)
+int64_t workspace_bytes(int64_t rows, int64_t in, int64_t out, int activation, bool backward, bool at16)
 {
     if (!backward)
-        return product_bytes<T>(rows, out, in, false, false);
-    return (activation == MIQ_ACT_NONE ? 0 : up256(rows * out * (int64_t) sizeof(T))) +
+        return product_bytes<T>(rows, out, in, false, false, at16, at16);
+    const bool kept = activation != MIQ_ACT_NONE;   // dz is the workspace's then
+    return (kept ? up256(rows * out * (int64_t) sizeof(T)) : 0) +
            up256(slope_slices(rows, out) * out * (int64_t) sizeof(float)) +
-           std::max(product_bytes<T>(rows, in, out, false, true), product_bytes<T>(out, in, rows, true, true));
+           std::max(product_bytes<T>(rows, in, out, false, true, kept || at16, at16),
+                    product_bytes<T>(out, in, rows, true, true, kept || at16, at16));
 }
 
 template <typename T>
@@ -611,11 +696,11 @@ int linear_fwd(const T* x, const T* w, const T* bias, const T* residual, int64_t
     if (rows == 0 || out == 0)
         return MIQ_OK;
     MIQ_CHECK_ARG(y && (in == 0 || (x && w)), "null pointer");
-    MIQ_CHECK_ARG(bytes >= workspace_bytes<T>(rows, in, out, activation, 0) && (workspace || bytes == 0),
-                  "the workspace is too small");
+    const int64_t need = workspace_bytes<T>(rows, in, out, activation, false, aligned(x) && aligned(w));
+    MIQ_CHECK_ARG(bytes >= need && (workspace || need == 0), "the workspace is too small");
     int rc = MIQ_OK;
     with_activation(activation, [&](auto act) {
-        rc = product<T, act.value>({x, rows, in, false}, {w, out, in, false}, bias, residual, y, (Saved<T>*) saved,
+        rc = product<T, act.value>({x, rows, in, false, aligned(x)}, {w, out, in, false, aligned(w)}, bias, residual, y, (Saved<T>*) saved,
                                    (char*) workspace, (hipStream_t) stream);
     });
     return rc;
@@ -631,8 +716,9 @@ int linear_bwd(const T* g, const void* saved, const T* x, const T* w, int64_t ro
     MIQ_CHECK_ARG(rows * out == 0 || (g && (saved || !kept)), "null pointer");
     MIQ_CHECK_ARG(rows * in == 0 || !dw || x, "dweight needs x");
     MIQ_CHECK_ARG(out * in == 0 || !dx || w, "dx needs weight");
-    MIQ_CHECK_ARG((workspace || bytes == 0) && bytes >= workspace_bytes<T>(rows, in, out, activation, 1),
-                  "the workspace is too small");
+    const bool at16    = aligned(g) && aligned(x) && aligned(w);
+    const int64_t need = workspace_bytes<T>(rows, in, out, activation, true, at16);
+    MIQ_CHECK_ARG(bytes >= need && (workspace || need == 0), "the workspace is too small");
     hipStream_t s  = (hipStream_t) stream;
     const T* dz    = g;
     char* at       = (char*) workspace;
@@ -657,9 +743,11 @@ int linear_bwd(const T* g, const void* saved, const T* x, const T* w, int64_t ro
     }
     int rc = MIQ_OK;
     if (dx)
-        rc = product<T, MIQ_ACT_NONE>({dz, rows, out, false}, {w, in, out, true}, nullptr, nullptr, dx, nullptr, at, s);
+        rc = product<T, MIQ_ACT_NONE>({dz, rows, out, false, kept || at16}, {w, in, out, true, at16}, nullptr, nullptr, dx,
+                                      nullptr, at, s);
     if (rc == MIQ_OK && dw)
-        rc = product<T, MIQ_ACT_NONE>({dz, out, rows, true}, {x, in, rows, true}, nullptr, nullptr, dw, nullptr, at, s);
+        rc = product<T, MIQ_ACT_NONE>({dz, out, rows, true, kept || at16}, {x, in, rows, true, at16}, nullptr, nullptr, dw,
+                                      nullptr, at, s);
     return rc;
 }
 }   // namespace
@@ -670,12 +758,12 @@ using namespace miq;
 extern "C"
 {
 int64_t miq_linear_workspace_bytes(int64_t rows, int64_t in_features, int64_t out_features, int activation, int bf16,
-                                   int backward)
+                                   int backward, int aligned)
 {
     if (rows < 0 || in_features < 0 || out_features < 0)
         return 0;
-    return bf16 ? workspace_bytes<uint16_t>(rows, in_features, out_features, activation, backward)
-                : workspace_bytes<float>(rows, in_features, out_features, activation, backward);
+    return bf16 ? workspace_bytes<uint16_t>(rows, in_features, out_features, activation, backward != 0, aligned != 0)
+                : workspace_bytes<float>(rows, in_features, out_features, activation, backward != 0, aligned != 0);
 }
 
 int miq_linear_fwd_f32(const float* x, const float* weight, const float* bias, const float* residual, int64_t rows,

@@ -43,9 +43,10 @@ constexpr int kSlice = 64;   // values of k in a slice: 128 bytes of a row
 // 16 zero bytes: what lanes outside of an operand load
 __device__ const uint4 g_zero16 = {0u, 0u, 0u, 0u};
 
+template <typename E>
 struct Operand
 {
-    const uint16_t* p;
+    const E* p;
     int64_t ld;      // elements between rows ("rows") or between values of k ("columns"); a multiple of 8
     int64_t count;   // m or n
 };
@@ -53,7 +54,7 @@ struct Operand
 // Where the 16-byte chunk `c` of row `r` of a slice lies: exchanged within a row such that the lanes of one LDS access
 // meet different banks.  `KEY` 0: A in rows (lanes read 8 consecutive rows), 1: B in rows (8 rows as row_of_b deals
 // them), 2: A in columns (lanes read rows k .. k + 3 and k + 8 .. k + 11, at the same columns), 3: B in columns (the
-// same, columns as row_of_b deals them).
+// same, columns as row_of_b deals them).  float32: 4: rows (16 rows at a time), 5: columns (rows k, k + 8, k + 16, k + 24).
 template <int KEY>
 __device__ __forceinline__ int exchanged(int r, int c)
 {
@@ -61,7 +62,17 @@ __device__ __forceinline__ int exchanged(int r, int c)
         return c ^ (r & 7);
     if (KEY == 1)
         return c ^ ((r & 3) | ((r >> 1) & 4));
+    if (KEY == 4)
+        return c ^ (r >> 1 & 7);
+    if (KEY == 5)
+        return c ^ (r >> 3 & 3) * 4;
     return c ^ ((r & 3) * 4 + (r >> 3 & 1) * 2);
+}
+// rows this far apart exchange their chunks alike
+template <int KEY>
+constexpr int period()
+{
+    return KEY == 0 ? 8 : KEY == 5 ? 32 : 16;
 }
 
 // row of B's 16 FN row share that lane index i (0..15) of fragment j holds
@@ -71,43 +82,46 @@ __device__ __forceinline__ int row_of_b(int j, int i)
 }
 
 // One operand's slices: who loads what.  COUNT rows (m or n) of the tile, WAVES waves load, 1 KiB each at a time: load i
-// of a wave is the (i WAVES + wave)th KiB of the slice.  A lane's place in its row of LDS is then the same in every load,
-// and so is its offset from the load's first byte: one 32-bit register, everything else is the same for the whole wave.
-template <int COUNT, int WAVES, bool COLUMNS, int KEY>
+// of a wave is the (i WAVES + wave)th KiB of the slice.  A lane's place in its row of LDS is then the same in every load
+// (but in float32 columns), and so is its offset from the load's first byte: one 32-bit register, everything else is the
+// same for the whole wave.
+template <typename E, int COUNT, int WAVES, bool COLUMNS, int KEY>
 struct Loader
 {
-    static constexpr int kChunks = (COLUMNS ? COUNT * 2 : kSlice * 2) / 16;   // 16-byte chunks of a row in LDS
-    static constexpr int kRows   = COLUMNS ? kSlice : COUNT;                  // rows in LDS
+    static constexpr int kVec    = 16 / sizeof(E);
+    static constexpr int kDeep   = 128 / sizeof(E);                           // values of k in a slice
+    static constexpr int kChunks = COLUMNS ? COUNT / kVec : 8;                // 16-byte chunks of a row in LDS
+    static constexpr int kRows   = COLUMNS ? kDeep : COUNT;                   // rows in LDS
     static constexpr int kAtOnce = 64 / kChunks;                              // rows of a load
     static constexpr int kLoads  = kRows / kAtOnce / WAVES;                   // loads of a wave
-    static constexpr int kBytes  = COUNT * kSlice * 2;
-    static_assert(kRows % (kAtOnce * WAVES) == 0 && WAVES * kAtOnce % (KEY == 0 ? 8 : 16) == 0,
-                  "the slice is cut evenly, and rows of one lane exchange their chunks alike");
+    static constexpr int kBytes  = COUNT * 128;
+    static constexpr bool kAlike = WAVES * kAtOnce % period<KEY>() == 0;      // a lane's chunk is the same in every load
+    static_assert(kRows % (kAtOnce * WAVES) == 0, "the slice is cut evenly");
 
-    const uint16_t* p;   // first value of the slice, of the wave's first row in LDS; the same in all lanes
+    const E* p;          // first value of the slice, of the wave's first row in LDS; the same in all lanes
     int64_t step;        // to the next slice
     int64_t apart;       // between the rows of two loads
     uint32_t offset;     // of the lane's chunk, in bytes
     bool edge;           // the tile reaches past the operand's end
 
-    __device__ __forceinline__ void start(const Operand& o, int64_t first, int wave, int lane)
+    __device__ __forceinline__ void start(const Operand<E>& o, int64_t first, int wave, int lane)
     {
         const int r = wave * kAtOnce, c = exchanged<KEY>(r + lane / kChunks, lane % kChunks);
-        step   = COLUMNS ? o.ld * kSlice : kSlice;
+        step   = COLUMNS ? o.ld * kDeep : kDeep;
         apart  = o.ld * (kAtOnce * WAVES);
         p      = o.p + r * o.ld + (COLUMNS ? first : first * o.ld);
-        offset = (uint32_t) (lane / kChunks) * (uint32_t) (o.ld * 2) + c * 16;
+        offset = (uint32_t) (lane / kChunks) * (uint32_t) (o.ld * sizeof(E)) + c * 16;
         edge   = first + COUNT > o.count;
     }
 
     // Starts the loads of a slice with `left` values of k remaining (from its first) into `lds`
-    __device__ __forceinline__ void load(const Operand& o, int64_t first, char* lds, int wave, int lane, int64_t left)
+    __device__ __forceinline__ void load(const Operand<E>& o, int64_t first, char* lds, int wave, int lane, int64_t left)
     {
-        if (!edge && left >= kSlice)
+        if (!edge && left >= kDeep)
         {
 #pragma unroll
             for (int i = 0; i < kLoads; ++i)
-                to_lds((const char*) (p + i * apart) + offset, lds + (i * WAVES + wave) * 1024);
+                to_lds((const char*) (p + i * apart) + offset_of(i, wave, lane), lds + (i * WAVES + wave) * 1024);
         }
         else
         {
@@ -116,13 +130,21 @@ struct Loader
             for (int i = 0; i < kLoads; ++i)
             {
                 const int r = (i * WAVES + wave) * kAtOnce + lane / kChunks;
-                const int c = exchanged<KEY>(r, lane % kChunks) * 8;
+                const int c = exchanged<KEY>(r, lane % kChunks) * kVec;
                 const bool in = COLUMNS ? r < left && first + c < o.count : c < left && first + r < o.count;
-                to_lds(in ? (const char*) (p + i * apart) + offset : (const char*) &g_zero16,
+                to_lds(in ? (const char*) (p + i * apart) + offset_of(i, wave, lane) : (const char*) &g_zero16,
                        lds + (i * WAVES + wave) * 1024);
             }
         }
         p += step;
+    }
+
+    __device__ __forceinline__ uint32_t offset_of(int i, int wave, int lane) const
+    {
+        if (kAlike)
+            return offset;
+        const int r = wave * kAtOnce + lane / kChunks, c = lane % kChunks;
+        return offset + (exchanged<KEY>(r + i * WAVES * kAtOnce, c) - exchanged<KEY>(r, c)) * 16;
     }
 
     static __device__ __forceinline__ void to_lds(const char* from, char* lds)
@@ -302,10 +324,52 @@ __device__ __forceinline__ void finish8(const Epilogue<T>& e, int64_t r, int64_t
     store8(e.c + at, left, z);
 }
 
+// the same for 4 values of a float32 matrix
+__device__ __forceinline__ void load4(const float* p, int64_t left, float* v)
+{
+    if (left >= 4)
+        load_any(p, v);
+    else
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            v[i] = i < left ? p[i] : 0.f;
+}
+__device__ __forceinline__ void store4(float* p, int64_t left, const float* v)
+{
+    if (left >= 4)
+        store_any(p, v);
+    else
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i < left)
+                p[i] = v[i];
+}
+template <int ACT>
+__device__ __forceinline__ void finish4(const Epilogue<float>& e, int64_t r, int64_t q, float* z)
+{
+    const int64_t at = r * e.n + q, left = e.n - q;
+    float t[4];
+    if (e.bias)
+    {
+        load4(e.bias + q, left, t);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            z[i] += t[i];
+    }
+    if (e.saved)
+        store4(e.saved + at, left, z);
+    if (e.residual)
+        load4(e.residual + at, left, t);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        z[i] = act_value<ACT>(z[i]) + (e.residual ? t[i] : 0.f);
+    store4(e.c + at, left, z);
+}
+
 template <typename T>
 struct Product
 {
-    Operand a, b;
+    Operand<uint16_t> a, b;
     int64_t k;             // length of the sum (float32: padded to whole slices)
     int tiles_m, tiles_n;
     int splits;            // the sum over k is cut into this many pieces, whose results go to `partial`
@@ -335,8 +399,8 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(const Product<T> p
     constexpr bool kF32  = std::is_same<T, float>::value;
     constexpr int kWaves = WM * WN, kTM = WM * FM * 16, kTN = WN * FN * 16;
     constexpr int kKeyA = AC ? 2 : 0, kKeyB = BC ? 3 : 1;
-    using LA             = Loader<kTM, kWaves, AC, kKeyA>;
-    using LB             = Loader<kTN, kWaves, BC, kKeyB>;
+    using LA             = Loader<uint16_t, kTM, kWaves, AC, kKeyA>;
+    using LB             = Loader<uint16_t, kTN, kWaves, BC, kKeyB>;
     using Kind           = std::integral_constant<bool, !kF32>;
     __shared__ __attribute__((aligned(1024))) char lds[2 * (LA::kBytes + LB::kBytes)];
 

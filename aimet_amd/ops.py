@@ -633,9 +633,9 @@ def _linear_sizes(x, weight):
     return rows, weight.shape[1], weight.shape[0]
 
 
-def _linear_workspace(rows, n_in, n_out, activation, bf16, backward, device):
-    """(tensor or None, bytes)"""
-    n = int(lib.miq_linear_workspace_bytes(rows, n_in, n_out, activation, bf16, backward))
+def _linear_workspace(rows, n_in, n_out, activation, bf16, backward, addresses, device):
+    """(tensor or None, bytes); `addresses`: those of the call's operands, or-ed together"""
+    n = lib.miq_linear_workspace_bytes(rows, n_in, n_out, activation, bf16, backward, addresses & 15 == 0)
     return (torch.empty(n, dtype=torch.uint8, device=device) if n else None), n
 
 
@@ -660,7 +660,7 @@ def linear_fwd(x, weight, bias=None, activation="none", residual=None, want_save
     saved = None
     if want_saved and act:
         saved = torch.empty(shape, dtype=torch.float16 if bf16 else _F32, device=x.device)
-    ws, ws_bytes = _linear_workspace(rows, n_in, n_out, act, bf16, 0, x.device)
+    ws, ws_bytes = _linear_workspace(rows, n_in, n_out, act, bf16, 0, x.data_ptr() | weight.data_ptr(), x.device)
     with _OnDevice(x.device):
         check(fn(x.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(residual), rows, n_in, n_out, act, y.data_ptr(),
                  _ptr(saved), _ptr(ws), ws_bytes, _stream(x)))
@@ -686,7 +686,8 @@ def linear_bwd(grad, saved, x, weight, activation="none", want_dx=True, want_dwe
     dx = torch.empty_like(x) if want_dx else None
     dw = torch.empty_like(weight) if want_dweight else None
     db = torch.empty(n_out, dtype=x.dtype, device=x.device) if want_dbias else None
-    ws, ws_bytes = _linear_workspace(rows, n_in, n_out, act, bf16, 1, x.device)
+    ws, ws_bytes = _linear_workspace(rows, n_in, n_out, act, bf16, 1,
+                                     grad.data_ptr() | x.data_ptr() | weight.data_ptr(), x.device)
     with _OnDevice(x.device):
         check(fn(grad.data_ptr(), _ptr(saved) if act else None, x.data_ptr(), weight.data_ptr(), rows, n_in, n_out,
                  act, _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), ws_bytes, _stream(x)))

@@ -735,14 +735,15 @@ int miq_layer_norm_bwd_bf16(const uint16_t* x, const uint16_t* grad, const uint1
  * pass needs of z, [rows, out], float for the f32 entry points and half for the bf16 ones.  dx, dweight, dbias may each
  * be NULL where that gradient is not wanted.
  * workspace: miq_linear_workspace_bytes() bytes, 256-byte aligned (may be NULL where that is 0); nothing in it outlives
- * the call on its stream.  out == in is not allowed. */
+ * the call on its stream.  `aligned`: every tensor of the call starts on a multiple of 16 bytes (some then need less).
+ * out == in is not allowed. */
 #define MIQ_ACT_NONE 0
 #define MIQ_ACT_RELU 1
 #define MIQ_ACT_SILU 2
 #define MIQ_ACT_GELU 3      /* z Phi(z) */
 #define MIQ_ACT_GELU_TANH 4 /* z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2 */
 int64_t miq_linear_workspace_bytes(int64_t rows, int64_t in_features, int64_t out_features, int activation, int bf16,
-                                   int backward);
+                                   int backward, int aligned);
 int miq_linear_fwd_f32(const float* x, const float* weight, const float* bias, const float* residual, int64_t rows,
                        int64_t in_features, int64_t out_features, int activation, float* y, float* saved,
                        void* workspace, int64_t workspace_bytes, void* stream);

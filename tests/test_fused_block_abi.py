@@ -49,11 +49,11 @@ def test_linear_refusals(lib, suffix):
     _refused(lib, bwd(P, None, P, None, 4, 8, 8, 0, P, P, P, P, big, None), "weight")
     _refused(lib, bwd(P, P, P, P, 4, 8, 8, 3, P, P, P, P, 0, None), "workspace")
     for rows, n_in, n_out in ((1, 64, 64), (300, 1000, 77), (5000, 512, 4096)):
-        need = lib.miq_linear_workspace_bytes(rows, n_in, n_out, 3, int(suffix == "bf16"), 0)
+        need = lib.miq_linear_workspace_bytes(rows, n_in, n_out, 3, int(suffix == "bf16"), 0, 1)
         if need:
             _refused(lib, fwd(P, P, None, None, rows, n_in, n_out, 3, P, None, P, need - 1, None), "workspace")
     assert fwd(None, None, None, None, 0, 8, 8, 0, None, None, None, 0, None) == 0
-    assert lib.miq_linear_workspace_bytes(-1, 8, 8, 0, 0, 1) == 0
+    assert lib.miq_linear_workspace_bytes(-1, 8, 8, 0, 0, 1, 1) == 0
 
 
 def test_functions_refuse_before_any_launch():
