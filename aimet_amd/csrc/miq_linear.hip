@@ -374,11 +374,17 @@ int64_t max_slices(int64_t k)
     return std::max<int64_t>(1, std::min<int64_t>(32, k / 16));
 }
 
-#ifdef MIQ_TUNE
-int64_t direct_most() { static const char* e = getenv("DIRECT"); return e ? atoi(e) : 500; }
-#else
-int64_t direct_most() { return 500; }
-#endif
+// Whether a float32 product is formed from its operands as they lie (miq_direct.h) or from halves made beforehand.
+// Measured: the first runs at about 170 TFLOP/s, the second at up to 380 once the halves are there; making them takes
+// about 22 us of launches and 3 ps a value of an operand in rows, 5 ps in columns (one more pass).  E.g. [512, 4096] x
+// [4096, 4096]^T: 115 us and 107 us, [256, 4096] x [11008, 4096]^T: 177 us and 192 us, [1024, 4096] x [4096, 4096]^T:
+// 204 us and 171 us.
+template <typename T>
+bool direct_pays(const Matrix<T>& a, const Matrix<T>& b)
+{
+    const auto halves = [](const Matrix<T>& x) { return (double) x.count * x.k * (x.columns ? 5e-12 : 3e-12); };
+    return 3.5e-15 * 2.0 * a.count * b.count * a.k <= 22e-6 + halves(a) + halves(b);
+}
 
 enum class Way
 {
@@ -430,7 +436,7 @@ Plan plan_product(const Matrix<T>& a, const Matrix<T>& b)
         p.way = Way::kShortSum;
         return done();
     }
-    if (kF32 && m * n <= direct_most() * (m + n))
+    if (kF32 && direct_pays(a, b))
     {
         p.way = Way::kDirect;
         // rows that are not whole chunks are copied, with zeros behind them
