@@ -182,6 +182,21 @@ def _load():
 lib = _load()
 
 
+def _load_native():
+    """The torch binding of some of the entry points (csrc/miq_torch.cpp).  torch comes first: it loads the libraries
+    the binding is linked against."""
+    import torch  # noqa: F401  pylint: disable=import-outside-toplevel,unused-import
+    try:
+        from . import _native  # pylint: disable=import-outside-toplevel
+    except ImportError as exc:
+        raise ImportError(f"aimet_amd/_native.so cannot be loaded ({exc}). Build it with `make -C aimet_amd/csrc`.") \
+            from exc
+    return _native
+
+
+native = _load_native()
+
+
 def check(status):
     """Raise MiqError for a non-zero status (RuntimeError subclass, like the reference's pybind exceptions)."""
     if status != OK:

@@ -10,7 +10,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._lib import Encoding, check, lib
+from ._lib import Encoding, check, lib, native as _native
 
 _F32, _BF16 = torch.float32, torch.bfloat16
 
@@ -561,137 +561,32 @@ def column_error(a, b, kind):
 
 
 # --------------------------------------------------------------- transformer block: layer norm, product with epilogue
+# These are bound in C++ (csrc/miq_torch.cpp), so that their autograd nodes run without the interpreter.
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
-
-
-def _require_like(x, **others):
-    """Every tensor given lives on x's GPU and has x's type."""
-    _require_gpu(x, *others.values())
-    for name, t in others.items():
-        if t is not None and t.dtype is not x.dtype:
-            raise RuntimeError(f"{name} is {t.dtype} but the input is {x.dtype}: one type is expected")
 
 
 def layer_norm_fwd(x, width, weight=None, bias=None, eps=1e-5, want_stats=False):
     """Layer norm over the last `width` values of x: (y, stats), stats a float32 [2, rows] tensor (mean and
     1 / sqrt(variance + eps) of every row) for layer_norm_bwd, or None unless `want_stats`."""
-    _require_like(x, weight=weight, bias=bias)
-    width = int(width)
-    if width < 1 or x.numel() % width:
-        raise RuntimeError(f"a tensor of {x.numel()} elements has no rows of {width}")
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None and t.numel() != width:
-            raise RuntimeError(f"{name} has {t.numel()} elements, a row has {width}")
-    fn = lib.miq_layer_norm_fwd_f32 if _suffix(x) == "f32" else lib.miq_layer_norm_fwd_bf16
-    x = x.contiguous()
-    weight = weight.contiguous() if weight is not None else None
-    bias = bias.contiguous() if bias is not None else None
-    rows = x.numel() // width
-    y = torch.empty_like(x)
-    stats = torch.empty(2, rows, dtype=_F32, device=x.device) if want_stats else None
-    mean = stats.data_ptr() if want_stats else None
-    with _OnDevice(x.device):
-        check(fn(x.data_ptr(), _ptr(weight), _ptr(bias), rows, width, float(eps), y.data_ptr(), mean,
-                 mean + 4 * rows if want_stats else None, _stream(x)))
-    return y, stats
+    return _native.layer_norm_fwd(x, width, weight, bias, eps, want_stats)
 
 
 def layer_norm_bwd(x, grad, width, weight, stats, want_dx=True, want_dweight=True, want_dbias=True):
     """(dx, dweight, dbias) of layer_norm_fwd, None where not wanted; `stats` as the forward pass returned it."""
-    _require_like(x, grad=grad, weight=weight)
-    _require_gpu(x, stats)
-    width = int(width)
-    if width < 1 or x.numel() % width or grad.numel() != x.numel():
-        raise RuntimeError(f"x has {x.numel()} and grad {grad.numel()} elements, a row {width}")
-    rows = x.numel() // width
-    if stats.dtype is not _F32 or tuple(stats.shape) != (2, rows) or not stats.is_contiguous():
-        raise RuntimeError("stats is not what layer_norm_fwd returned for these rows")
-    if weight is not None and weight.numel() != width:
-        raise RuntimeError(f"weight has {weight.numel()} elements, a row has {width}")
-    fn = lib.miq_layer_norm_bwd_f32 if _suffix(x) == "f32" else lib.miq_layer_norm_bwd_bf16
-    x, grad = x.contiguous(), grad.contiguous()
-    weight = weight.contiguous() if weight is not None else None
-    dx = torch.empty_like(x) if want_dx else None
-    dw = torch.empty(width, dtype=x.dtype, device=x.device) if want_dweight else None
-    db = torch.empty(width, dtype=x.dtype, device=x.device) if want_dbias else None
-    ws = None
-    if want_dweight or want_dbias:
-        ws = torch.empty(int(lib.miq_layer_norm_bwd_workspace_bytes(rows, width)), dtype=torch.uint8, device=x.device)
-    with _OnDevice(x.device):
-        check(fn(x.data_ptr(), grad.data_ptr(), _ptr(weight), stats.data_ptr(), stats.data_ptr() + 4 * rows, rows,
-                 width, _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), _stream(x)))
-    return dx, dw, db
-
-
-def _linear_sizes(x, weight):
-    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
-        raise RuntimeError(f"an input of shape {tuple(x.shape)} does not go with a weight of shape "
-                           f"{tuple(weight.shape)}: [..., in] and [out, in] are expected")
-    rows = 1
-    for d in x.shape[:-1]:
-        rows *= d
-    return rows, weight.shape[1], weight.shape[0]
-
-
-def _linear_workspace(rows, n_in, n_out, activation, bf16, backward, addresses, device):
-    """(tensor or None, bytes); `addresses`: those of the call's operands, or-ed together"""
-    n = lib.miq_linear_workspace_bytes(rows, n_in, n_out, activation, bf16, backward, addresses & 15 == 0)
-    return (torch.empty(n, dtype=torch.uint8, device=device) if n else None), n
+    return _native.layer_norm_bwd(x, grad, width, weight, stats, want_dx, want_dweight, want_dbias)
 
 
 def linear_fwd(x, weight, bias=None, activation="none", residual=None, want_saved=False):
     """act(x weight^T + bias) + residual for x [..., in], weight [out, in], bias [out], residual [..., out], in one
     launch sequence: (y, saved), `saved` what linear_bwd needs of the product (None unless `want_saved`, and for
     activation "none")."""
-    _require_like(x, weight=weight, bias=bias, residual=residual)
-    rows, n_in, n_out = _linear_sizes(x, weight)
-    act = ACTIVATIONS[activation]
-    shape = (*x.shape[:-1], n_out)
-    if bias is not None and tuple(bias.shape) != (n_out,):
-        raise RuntimeError(f"bias has shape {tuple(bias.shape)}, ({n_out},) is expected")
-    if residual is not None and tuple(residual.shape) != shape:
-        raise RuntimeError(f"residual has shape {tuple(residual.shape)}, {shape} is expected")
-    bf16 = _suffix(x) == "bf16"
-    fn = lib.miq_linear_fwd_bf16 if bf16 else lib.miq_linear_fwd_f32
-    x, weight = x.contiguous(), weight.contiguous()
-    bias = bias.contiguous() if bias is not None else None
-    residual = residual.contiguous() if residual is not None else None
-    y = torch.empty(shape, dtype=x.dtype, device=x.device)
-    saved = None
-    if want_saved and act:
-        saved = torch.empty(shape, dtype=torch.float16 if bf16 else _F32, device=x.device)
-    ws, ws_bytes = _linear_workspace(rows, n_in, n_out, act, bf16, 0, x.data_ptr() | weight.data_ptr(), x.device)
-    with _OnDevice(x.device):
-        check(fn(x.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(residual), rows, n_in, n_out, act, y.data_ptr(),
-                 _ptr(saved), _ptr(ws), ws_bytes, _stream(x)))
-    return y, saved
+    return _native.linear_fwd(x, weight, bias, ACTIVATIONS[activation], residual, want_saved)
 
 
 def linear_bwd(grad, saved, x, weight, activation="none", want_dx=True, want_dweight=True, want_dbias=True):
     """(dx, dweight, dbias) of linear_fwd, None where not wanted; `saved` as the forward pass returned it.  The
     residual's gradient is `grad` itself."""
-    _require_like(x, weight=weight, grad=grad)
-    rows, n_in, n_out = _linear_sizes(x, weight)
-    act = ACTIVATIONS[activation]
-    bf16 = _suffix(x) == "bf16"
-    if grad.numel() != rows * n_out:
-        raise RuntimeError(f"grad has {grad.numel()} elements, the output {rows * n_out}")
-    if act:
-        _require_gpu(x, saved)
-        if saved.dtype is not (torch.float16 if bf16 else _F32) or saved.numel() != rows * n_out or \
-                not saved.is_contiguous():
-            raise RuntimeError("saved is not what linear_fwd returned for these shapes")
-    fn = lib.miq_linear_bwd_bf16 if bf16 else lib.miq_linear_bwd_f32
-    grad, x, weight = grad.contiguous(), x.contiguous(), weight.contiguous()
-    dx = torch.empty_like(x) if want_dx else None
-    dw = torch.empty_like(weight) if want_dweight else None
-    db = torch.empty(n_out, dtype=x.dtype, device=x.device) if want_dbias else None
-    ws, ws_bytes = _linear_workspace(rows, n_in, n_out, act, bf16, 1,
-                                     grad.data_ptr() | x.data_ptr() | weight.data_ptr(), x.device)
-    with _OnDevice(x.device):
-        check(fn(grad.data_ptr(), _ptr(saved) if act else None, x.data_ptr(), weight.data_ptr(), rows, n_in, n_out,
-                 act, _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), ws_bytes, _stream(x)))
-    return dx, dw, db
+    return _native.linear_bwd(grad, saved, x, weight, ACTIVATIONS[activation], want_dx, want_dweight, want_dbias)
 
 
 # ---------------------------------------------------------------------------------------------------- range learning

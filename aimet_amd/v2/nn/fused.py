@@ -6,102 +6,36 @@ default_config.json) but runs its members as separate torch modules.  FusedLinea
 bias, activation and residual in one pass over the output, with one output quantizer behind it.  FusedLayerNorm is
 nn.LayerNorm on one pass over the input.  Both train: gradients of input, weight, bias and residual.
 
-float32 and bfloat16 tensors on the GPU; sums and statistics are float32.  Under torch.autocast the functions follow
+float32 and bfloat16 tensors on the GPU; sums and statistics are float32; differentiable once.  Under torch.autocast the functions follow
 torch's own: linear() computes in the autocast type, layer_norm() in float32.
 """
 from typing import Optional, Sequence
 
 import torch
 from torch import nn
-from torch.autograd.function import once_differentiable
 
 from ... import ops
+from ..._lib import native as _native
 from .base import QuantizationMixin
 
 ACTIVATIONS = tuple(ops.ACTIVATIONS)
-
-
-class _LayerNormFunc(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, width, eps):  # pylint: disable=arguments-differ
-        x = x.contiguous()
-        y, stats = ops.layer_norm_fwd(x, width, weight, bias, eps, want_stats=True)
-        ctx.width = width
-        ctx.shapes = (None if weight is None else weight.shape, None if bias is None else bias.shape)
-        ctx.save_for_backward(x, weight, stats)
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):  # pylint: disable=arguments-differ
-        x, weight, stats = ctx.saved_tensors
-        want_dx, want_dw, want_db = ctx.needs_input_grad[:3]
-        dx, dw, db = ops.layer_norm_bwd(x, grad, ctx.width, weight, stats, want_dx, want_dw, want_db)
-        w_shape, b_shape = ctx.shapes
-        return dx, (dw.view(w_shape) if want_dw else None), (db.view(b_shape) if want_db else None), None, None
-
-
-class _LinearFunc(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, residual, activation):  # pylint: disable=arguments-differ
-        x, weight = x.contiguous(), weight.contiguous()
-        wants = any(ctx.needs_input_grad[:3])
-        y, saved = ops.linear_fwd(x, weight, bias, activation, residual, want_saved=wants)
-        ctx.activation = activation
-        if wants:
-            ctx.save_for_backward(x, weight, saved)
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):  # pylint: disable=arguments-differ
-        want_dx, want_dw, want_db, want_dr = ctx.needs_input_grad[:4]
-        dx = dw = db = None
-        if want_dx or want_dw or want_db:
-            x, weight, saved = ctx.saved_tensors
-            dx, dw, db = ops.linear_bwd(grad, saved, x, weight, ctx.activation, want_dx, want_dw, want_db)
-        return dx, dw, db, (grad if want_dr else None), None
-
-
-def _differentiates(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
-def _cast(dtype, *tensors):
-    return [t if t is None or t.dtype is dtype or not t.is_floating_point() else t.to(dtype) for t in tensors]
 
 
 def layer_norm(input: torch.Tensor, normalized_shape: Sequence[int], weight: Optional[torch.Tensor] = None,  # pylint: disable=redefined-builtin
                bias: Optional[torch.Tensor] = None, eps: float = 1e-5) -> torch.Tensor:
     """torch.nn.functional.layer_norm on the HIP kernels: normalizes over the trailing `normalized_shape`, then scales
     and shifts.  `weight` and `bias` have that shape and the input's type."""
-    shape = (normalized_shape,) if isinstance(normalized_shape, int) else tuple(normalized_shape)
-    if not shape or tuple(input.shape[-len(shape):]) != shape:
-        raise RuntimeError(f"normalized_shape {shape} is not the end of the input's shape {tuple(input.shape)}")
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None and tuple(t.shape) != shape:
-            raise RuntimeError(f"{name} has shape {tuple(t.shape)}, {shape} is expected")
-    if torch.is_autocast_enabled("cuda"):
-        input, weight, bias = _cast(torch.float32, input, weight, bias)
-    width = 1
-    for d in shape:
-        width *= d
-    if _differentiates(input, weight, bias):
-        return _LayerNormFunc.apply(input, weight, bias, width, eps)
-    return ops.layer_norm_fwd(input, width, weight, bias, eps)[0]
+    return _native.layer_norm(input, normalized_shape, weight, bias, eps)
 
 
 def linear(input: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,  # pylint: disable=redefined-builtin
            activation: str = "none", residual: Optional[torch.Tensor] = None) -> torch.Tensor:
     """activation(input weight^T + bias) + residual.  input [..., in], weight [out, in], bias [out], residual of the
     output's shape [..., out]; all of one type.  activation: "none", "relu", "silu", "gelu" (exact) or "gelu_tanh"."""
-    if activation not in ops.ACTIVATIONS:
+    code = ops.ACTIVATIONS.get(activation)
+    if code is None:
         raise ValueError(f"unknown activation {activation!r}: one of {', '.join(ACTIVATIONS)} is expected")
-    if torch.is_autocast_enabled("cuda"):
-        input, weight, bias, residual = _cast(torch.get_autocast_dtype("cuda"), input, weight, bias, residual)
-    if _differentiates(input, weight, bias, residual):
-        return _LinearFunc.apply(input, weight, bias, residual, activation)
-    return ops.linear_fwd(input, weight, bias, activation, residual)[0]
+    return _native.linear(input, weight, bias, code, residual)
 
 
 class FusedLayerNorm(nn.LayerNorm):
