@@ -137,7 +137,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void direct_kernel(const DirectProd
             issue(0);
         for (int s = 0; s < last - first; ++s)
         {
-            __syncthreads();   // slice s has arrived, and everybody has read slice s - 1
+            arrived();   // slice s has arrived, and everybody has read slice s - 1
             if (s + 1 < last - first)
                 issue((s + 1) & 1);
             const char* sa = lds + (s & 1) * (LA::kBytes + LB::kBytes);

@@ -81,6 +81,18 @@ __device__ __forceinline__ int row_of_b(int j, int i)
     return 32 * (j / 2) + 8 * (i / 4) + 4 * (j % 2) + i % 4;
 }
 
+// Loads from memory to LDS are written out as instructions: to the compiler the builtin is a store that any LDS read
+// after it may depend on, and it puts a wait for the load before the read.  Nothing is returned in registers.  What makes
+// the loads' results visible is arrived() alone: every wave waits for its own loads and reads, then for the other waves.
+__device__ __forceinline__ uint32_t lds_address(const char* p)
+{
+    return (uint32_t) (uintptr_t) (__attribute__((address_space(3))) const char*) p;
+}
+__device__ __forceinline__ void arrived()
+{
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
 // One operand's slices: who loads what.  COUNT rows (m or n) of the tile, WAVES waves load, 1 KiB each at a time: load i
 // of a wave is the (i WAVES + wave)th KiB of the slice.  A lane's place in its row of LDS is then the same in every load
 // (but in float32 columns), and so is its offset from the load's first byte: one 32-bit register, everything else is the
@@ -114,28 +126,37 @@ struct Loader
         edge   = first + COUNT > o.count;
     }
 
-    // Starts the loads of a slice with `left` values of k remaining (from its first) into `lds`
-    __device__ __forceinline__ void load(const Operand<E>& o, int64_t first, char* lds, int wave, int lane, int64_t left)
+    // Starts load i of a slice with `left` values of k remaining (from its first) into `lds`.  INSIDE: all of the slice is
+    // inside of the operand; otherwise what is not is read as zeros.
+    template <bool INSIDE>
+    __device__ __forceinline__ void load_one(int i, const Operand<E>& o, int64_t first, char* lds, int wave, int lane,
+                                             int64_t left)
     {
-        if (!edge && left >= kDeep)
-        {
-#pragma unroll
-            for (int i = 0; i < kLoads; ++i)
-                to_lds((const char*) (p + i * apart) + offset_of(i, wave, lane), lds + (i * WAVES + wave) * 1024);
-        }
+        const uint32_t to = __builtin_amdgcn_readfirstlane(lds_address(lds + (i * WAVES + wave) * 1024));
+        if (INSIDE)
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to),
+                         "v"(offset_of(i, wave, lane)), "s"(p + i * apart)
+                         : "memory");
         else
         {
-            // What is outside of the operand is read as zeros
-#pragma unroll
-            for (int i = 0; i < kLoads; ++i)
-            {
-                const int r = (i * WAVES + wave) * kAtOnce + lane / kChunks;
-                const int c = exchanged<KEY>(r, lane % kChunks) * kVec;
-                const bool in = COLUMNS ? r < left && first + c < o.count : c < left && first + r < o.count;
-                to_lds(in ? (const char*) (p + i * apart) + offset_of(i, wave, lane) : (const char*) &g_zero16,
-                       lds + (i * WAVES + wave) * 1024);
-            }
+            const int r   = (i * WAVES + wave) * kAtOnce + lane / kChunks;
+            const int c   = exchanged<KEY>(r, lane % kChunks) * kVec;
+            const bool in = COLUMNS ? r < left && first + c < o.count : c < left && first + r < o.count;
+            const char* from =
+                in ? (const char*) (p + i * apart) + offset_of(i, wave, lane) : (const char*) &g_zero16;
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from)
+                         : "memory");
         }
+    }
+    __device__ __forceinline__ void load(const Operand<E>& o, int64_t first, char* lds, int wave, int lane, int64_t left)
+    {
+        const bool inside = !edge && left >= kDeep;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i)
+            if (inside)
+                load_one<true>(i, o, first, lds, wave, lane, left);
+            else
+                load_one<false>(i, o, first, lds, wave, lane, left);
         p += step;
     }
 
@@ -145,12 +166,6 @@ struct Loader
             return offset;
         const int r = wave * kAtOnce + lane / kChunks, c = lane % kChunks;
         return offset + (exchanged<KEY>(r + i * WAVES * kAtOnce, c) - exchanged<KEY>(r, c)) * 16;
-    }
-
-    static __device__ __forceinline__ void to_lds(const char* from, char* lds)
-    {
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*) from,
-                                         (__attribute__((address_space(3))) void*) lds, 16, 0, 0);
     }
 };
 
@@ -186,7 +201,11 @@ struct Reader
         const s4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4v*) (lds + from));
         const s4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
             (__attribute__((address_space(3))) s4v*) (lds + from + 64 * CHUNKS));
-        return s8v{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        // (as pairs of 32-bit registers, that the two reads fill the halves of one operand without a move)
+        typedef int i2 __attribute__((ext_vector_type(2)));
+        typedef int i4 __attribute__((ext_vector_type(4)));
+        const i2 l = __builtin_bit_cast(i2, lo), h = __builtin_bit_cast(i2, hi);
+        return __builtin_bit_cast(s8v, i4{l[0], l[1], h[0], h[1]});
     }
 };
 
@@ -414,8 +433,6 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(const Product<T> p
 
     const int slices = (int) ((p.k + kSlice - 1) / kSlice);
     const int first = (int) ((int64_t) slices * split / p.splits), last = (int) ((int64_t) slices * (split + 1) / p.splits);
-    // float32: three passes over k, A's coarse halves with B's fine ones, fine with coarse, coarse with coarse
-    const int count = (last - first) * (kF32 ? 3 : 1);
 
     LA la;
     LB lb;
@@ -425,10 +442,11 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(const Product<T> p
     lb.p += (int64_t) first * lb.step + (kF32 ? p.k : 0);
     int64_t left = p.k - (int64_t) first * kSlice;
     int issued   = 0;
-    const auto issue = [&](int buffer) {
-        char* to = lds + buffer * (LA::kBytes + LB::kBytes);
-        la.load(p.a, m0, to, wave, lane, left);
-        lb.load(p.b, n0, to + LA::kBytes, wave, lane, left);
+    // After a slice's loads: on to the next one.  float32: three times over k, A's coarse halves with B's fine ones, fine
+    // with coarse, coarse with coarse.
+    const auto advance = [&] {
+        la.p += la.step;
+        lb.p += lb.step;
         left -= kSlice;
         ++issued;
         if (kF32 && (issued == last - first || issued == 2 * (last - first)))
@@ -455,46 +473,85 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(const Product<T> p
     {
         s8v a[FM], b[FN];
     };
-    const auto fetch = [&](Fragments& f, int buffer, int half) {
-        const char* sa = lds + buffer * (LA::kBytes + LB::kBytes);
-        const char* sb = sa + LA::kBytes;
-#pragma unroll
-        for (int j = 0; j < FN; ++j)
-            f.b[j] = rb.read(sb, j, half);
-#pragma unroll
-        for (int i = 0; i < FM; ++i)
-            f.a[i] = ra.read(sa, i, half);
-    };
-    const auto multiply = [&](const Fragments& f) {
-#pragma unroll
-        for (int i = 0; i < FM; ++i)
-#pragma unroll
-            for (int j = 0; j < FN; ++j)
-                acc[i][j] = mfma_16x16x32(f.b[j], f.a[i], acc[i][j], Kind());
-    };
-    // Fragments of one half of a slice are read while the other half's are multiplied: across the barrier the second
-    // half of the slice before is at work.
+    // What a wave does between two barriers, in steps of FN matrix instructions each: the rows of one half of a slice are
+    // multiplied (fragments `f`), the other half's fragments (`next`) are read from LDS meanwhile, two or three a step and
+    // none in the last quarter, so that they are there when the half ends; and the next slice's loads are started, spread
+    // over the steps, for a wave that finds the load path full waits with its matrix instructions behind it.  The order
+    // is fixed step by step: left to itself the compiler starts all loads first and waits for all reads at once.
+    constexpr int kReads = (FM + FN + FM - FM / 4 - 1) / (FM - FM / 4), kAll = LA::kLoads + LB::kLoads,
+                  kStarts = (kAll + FM - 1) / FM;
     Fragments f0, f1;
-    if (count > 0)
+    const auto half_slice = [&](auto multiplies, const Fragments& f, auto reads, Fragments& next, const char* from, int half,
+                                auto starts, auto inside, char* to) {
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+        {
+            if constexpr (decltype(starts)::value)
+#pragma unroll
+                for (int u = i * kStarts; u < (i + 1) * kStarts && u < kAll; ++u)
+                {
+                    if (u < LA::kLoads)
+                        la.template load_one<decltype(inside)::value>(u, p.a, m0, to, wave, lane, left);
+                    else
+                        lb.template load_one<decltype(inside)::value>(u - LA::kLoads, p.b, n0, to + LA::kBytes, wave, lane,
+                                                                      left);
+                }
+            if constexpr (decltype(multiplies)::value)
+#pragma unroll
+                for (int j = 0; j < FN; ++j)
+                    acc[i][j] = mfma_16x16x32(f.b[j], f.a[i], acc[i][j], Kind());
+            if constexpr (decltype(reads)::value)
+#pragma unroll
+                for (int u = i * kReads; u < (i + 1) * kReads && u < FM + FN; ++u)
+                {
+                    if (u < FN)
+                        next.b[u] = rb.read(from + LA::kBytes, u, half);
+                    else
+                        next.a[u - FN] = ra.read(from, u - FN, half);
+                }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if constexpr (decltype(starts)::value)
+            advance();
+    };
+    const auto sum = [&](int count, auto inside) {
+        constexpr auto yes = std::true_type();
+        constexpr auto no  = std::false_type();
+        const auto buffer  = [&](int s) { return lds + (s & 1) * (LA::kBytes + LB::kBytes); };
+        half_slice(no, f0, no, f0, nullptr, 0, yes, inside, buffer(0));
+        arrived();
+        if (count > 1)
+            half_slice(no, f0, yes, f0, buffer(0), 0, yes, inside, buffer(1));
+        else
+            half_slice(no, f0, yes, f0, buffer(0), 0, no, inside, nullptr);
+        half_slice(yes, f0, yes, f1, buffer(0), 1, no, inside, nullptr);
+        for (int s = 1; s + 1 < count; ++s)
+        {
+            arrived();   // slice s has arrived, and everybody has read slice s - 1
+            half_slice(yes, f1, yes, f0, buffer(s), 0, yes, inside, buffer(s + 1));
+            half_slice(yes, f0, yes, f1, buffer(s), 1, no, inside, nullptr);
+        }
+        if (count > 1)
+        {
+            arrived();
+            half_slice(yes, f1, yes, f0, buffer(count - 1), 0, no, inside, nullptr);
+            half_slice(yes, f0, yes, f1, buffer(count - 1), 1, no, inside, nullptr);
+        }
+        half_slice(yes, f1, no, f1, nullptr, 0, no, inside, nullptr);
+    };
+    const bool inside = !la.edge && !lb.edge && p.k % kSlice == 0;
+    for (int pass = 0; pass < (kF32 ? 2 : 1) && first < last; ++pass)
     {
-        issue(0);
-        __syncthreads();
-        if (1 < count)
-            issue(1);
-        fetch(f0, 0, 0);
-        fetch(f1, 0, 1);
-        multiply(f0);
-    }
-    for (int s = 1; s < count; ++s)
-    {
-        __syncthreads();   // slice s has arrived, and everybody has read slice s - 1
-        fetch(f0, s & 1, 0);
-        if (s + 1 < count)
-            issue((s + 1) & 1);
-        multiply(f1);
-        // the two passes over fine halves are corrections, finite for finite operands: where an infinity or a NaN
-        // made them anything else, the coarse pass alone says what comes out
-        if (kF32 && s == 2 * (last - first))
+        // float32: the corrections, then the coarse halves
+        const int count = (last - first) * (kF32 && pass == 0 ? 2 : 1);
+        if (inside)
+            sum(count, std::true_type());
+        else
+            sum(count, std::false_type());
+        if (kF32 && pass == 0)
+        {
+            // Corrections are finite for finite operands: where an infinity or a NaN made them anything else, the coarse
+            // halves alone say what comes out.
 #pragma unroll
             for (int i = 0; i < FM; ++i)
 #pragma unroll
@@ -502,11 +559,9 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(const Product<T> p
 #pragma unroll
                     for (int u = 0; u < 4; ++u)
                         acc[i][j][u] = __builtin_isfinite(acc[i][j][u]) ? acc[i][j][u] : 0.f;
-        fetch(f1, s & 1, 1);
-        multiply(f0);
+            arrived();   // everybody has read the last slice
+        }
     }
-    if (count > 0)
-        multiply(f1);
 
 #pragma unroll
     for (int i = 0; i < FM; ++i)

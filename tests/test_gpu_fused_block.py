@@ -304,6 +304,12 @@ def test_linear(fused, dtype, rows, k, n):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,k,n", [(3584, 256, 3840), (3700, 200, 3801), (3601, 77, 3912)])
+def test_linear_of_many_rows_and_columns(fused, dtype, rows, k, n):
+    check_linear(fused, *linear_case(rows, k, n, dtype, True), "silu")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("act", ACTIVATIONS)
 @pytest.mark.parametrize("rows,k,n", [(1, 96, 40), (50, 160, 136), (300, 328, 264)])
 def test_linear_activations(fused, dtype, act, rows, k, n):
@@ -330,8 +336,8 @@ def test_linear_without_rows_or_features(fused):
 def test_linear_keeps_bad_rows_to_themselves(fused):
     """An infinity or a NaN in a row of x reaches that row of the output alone, as what float32 arithmetic makes of it."""
     for dtype in DTYPES:
-        for rows in (7, 300):
-            x, w, b, _, _ = linear_case(rows, 200, 264, dtype, False)
+        for rows, n in ((7, 264), (300, 264), (2000, 264), (3700, 3700)):
+            x, w, b, _, _ = linear_case(rows, 200, n, dtype, False)
             good = fused.linear(x, w, b)
             x[1, 3], x[2, 199], x[4, 0] = float("inf"), -float("inf"), float("nan")
             y = fused.linear(x, w, b)
