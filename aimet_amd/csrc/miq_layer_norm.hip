@@ -34,7 +34,7 @@ __device__ __forceinline__ float lanes_sum(float v, float* lds)
     return v;
 }
 
-// two sums at once
+// Two sums at once.  The caller sees to it that everybody has read what `lds` held before.
 template <int LANES>
 __device__ __forceinline__ void lanes_sum2(float& a, float& b, float2* lds)
 {
@@ -46,7 +46,6 @@ __device__ __forceinline__ void lanes_sum2(float& a, float& b, float2* lds)
     }
     if constexpr (LANES > 64)
     {
-        __syncthreads();
         if ((threadIdx.x & 63) == 0)
             lds[threadIdx.x >> 6] = make_float2(a, b);
         __syncthreads();
@@ -61,31 +60,78 @@ __device__ __forceinline__ void lanes_sum2(float& a, float& b, float2* lds)
 }
 
 // A row lies in the registers of LANES threads, PER pieces of 16 bytes in each: piece i of lane l starts at value
-// (i LANES + l) VEC.  What is past the row's end is read as zero and not stored.
+// (i LANES + l) VEC.  The piece that reaches past the end starts earlier instead, so that it is whole, too: its first
+// `twice` values are also those of the piece before, and are left out where the row is summed up (what is stored for them
+// is stored twice, and the same).  Pieces altogether past the end are empty.  Only rows shorter than a piece are read value
+// by value.
+template <int VEC>
+struct Piece
+{
+    int at, twice;
+    bool has;
+
+    __device__ __forceinline__ Piece(int c, int width)
+    {
+        has   = c < width;
+        at    = c + VEC <= width || width < VEC ? c : width - VEC;
+        twice = c - at;
+    }
+};
+
 template <typename T>
-__device__ __forceinline__ void load_piece(const T* p, int left, float* v)
+__device__ __forceinline__ void load_piece(const T* p, int width, float* v)
 {
     constexpr int VEC = IOTraits<T>::VEC;
-    if (left >= VEC)
+    if (width >= VEC)
         load_any(p, v);
     else
 #pragma unroll
         for (int u = 0; u < VEC; ++u)
-            v[u] = u < left ? IOTraits<T>::load1(p + u) : 0.f;
+            v[u] = u < width ? IOTraits<T>::load1(p + u) : 0.f;
 }
 template <typename T>
-__device__ __forceinline__ void store_piece(T* p, int left, const float* v)
+__device__ __forceinline__ void store_piece(T* p, int width, const float* v)
 {
     constexpr int VEC = IOTraits<T>::VEC;
-    if (left >= VEC)
+    if (width >= VEC)
         store_any(p, v);
     else
 #pragma unroll
         for (int u = 0; u < VEC; ++u)
-            if (u < left)
+            if (u < width)
                 IOTraits<T>::store1(p + u, v[u]);
 }
 
+// the same as it lies in memory, and its values
+template <typename T>
+__device__ __forceinline__ any_u4 raw_piece(const T* p, int width)
+{
+    constexpr int VEC = IOTraits<T>::VEC;
+    if (width >= VEC)
+        return *(const any_u4*) p;
+    T t[VEC];
+#pragma unroll
+    for (int u = 0; u < VEC; ++u)
+        t[u] = u < width ? p[u] : (T) 0;
+    any_u4 v;
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+        if constexpr (VEC == 4)
+            v[u] = __float_as_uint(t[u]);
+        else
+            v[u] = (uint32_t) t[2 * u] | (uint32_t) t[2 * u + 1] << 16;
+    return v;
+}
+__device__ __forceinline__ void values_of(any_u4 v, float (&f)[4])
+{
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+        f[u] = __uint_as_float(v[u]);
+}
+__device__ __forceinline__ void values_of(any_u4 v, float (&f)[8])
+{
+    IOTraits<uint16_t>::unpack(make_uint4(v[0], v[1], v[2], v[3]), f);
+}
 // One pass: the row stays in registers between its mean, its variance (from differences to the mean) and the result.
 template <typename T, int PER, int LANES>
 __global__ __launch_bounds__(LANES < kBlock ? kBlock : LANES) void ln_fwd_kernel(
@@ -102,34 +148,48 @@ __global__ __launch_bounds__(LANES < kBlock ? kBlock : LANES) void ln_fwd_kernel
     float v[PER][VEC], s = 0.f;
 #pragma unroll
     for (int i = 0; i < PER; ++i)
-        load_piece(px + (i * LANES + lane) * VEC, width - (i * LANES + lane) * VEC, v[i]);
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
+    {
+        const Piece<VEC> piece((i * LANES + lane) * VEC, width);
 #pragma unroll
         for (int u = 0; u < VEC; ++u)
-            s += v[i][u];
+            v[i][u] = 0.f;
+        if (piece.has)
+            load_piece(px + piece.at, width, v[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+    {
+        const Piece<VEC> piece((i * LANES + lane) * VEC, width);
+#pragma unroll
+        for (int u = 0; u < VEC; ++u)
+            s += u < piece.twice ? 0.f : v[i][u];
+    }
     const float m = lanes_sum<LANES>(s, lds) / (float) width;
     float q       = 0.f;
 #pragma unroll
     for (int i = 0; i < PER; ++i)
+    {
+        const Piece<VEC> piece((i * LANES + lane) * VEC, width);
 #pragma unroll
         for (int u = 0; u < VEC; ++u)
         {
-            v[i][u] = (i * LANES + lane) * VEC + u < width ? v[i][u] - m : 0.f;
-            q       = fmaf(v[i][u], v[i][u], q);
+            v[i][u] -= m;
+            const bool counts = piece.has && u >= piece.twice && (width >= VEC || u < width);
+            q                 = counts ? fmaf(v[i][u], v[i][u], q) : q;
         }
+    }
     const float r = 1.0f / sqrtf(lanes_sum<LANES>(q, lds) / (float) width + eps);
 #pragma unroll
     for (int i = 0; i < PER; ++i)
     {
-        const int c = (i * LANES + lane) * VEC;
-        if (c >= width)
+        const Piece<VEC> piece((i * LANES + lane) * VEC, width);
+        if (!piece.has)
             continue;
         float ww[VEC], bb[VEC];
         if (w)
-            load_piece(w + c, width - c, ww);
+            load_piece(w + piece.at, width, ww);
         if (b)
-            load_piece(b + c, width - c, bb);
+            load_piece(b + piece.at, width, bb);
 #pragma unroll
         for (int u = 0; u < VEC; ++u)
         {
@@ -138,7 +198,7 @@ __global__ __launch_bounds__(LANES < kBlock ? kBlock : LANES) void ln_fwd_kernel
                 h *= ww[u];
             v[i][u] = b ? h + bb[u] : h;
         }
-        store_piece(y + row * width + c, width - c, v[i]);
+        store_piece(y + row * width + piece.at, width, v[i]);
     }
     if (lane == 0 && mean)
     {
@@ -183,65 +243,99 @@ __global__ __launch_bounds__(1024) void ln_fwd_long_kernel(const T* __restrict__
 
 // One pass over x and grad: a block takes rows block, block + blocks, ...; a thread meets the same columns in every row
 // and keeps their sums g xhat and g.  partial[block][0][c] and [1][c] receive them, for ln_join_kernel.
+// The next row is on its way while this one is worked on: as it lies in memory, which in bfloat16 takes half the registers.
 template <typename T, int PER, int LANES>
 __global__ __launch_bounds__(LANES < kBlock ? kBlock : LANES) void ln_bwd_kernel(
     const T* __restrict__ x, const T* __restrict__ g, const T* __restrict__ w, const float* __restrict__ mean,
     const float* __restrict__ rstd, int64_t rows, int width, T* __restrict__ dx, float* __restrict__ partial)
 {
     constexpr int VEC = IOTraits<T>::VEC, kRows = LANES < kBlock ? kBlock / LANES : 1;
-    __shared__ float2 lds[LANES / 64];
+    __shared__ float2 lds[2][LANES / 64];
     const int lane = threadIdx.x % LANES;
+    int odd        = 0;   // rows use the two halves of `lds` in turn: one barrier a row
     float sw[PER][VEC] = {}, sb[PER][VEC] = {};
-    for (int64_t row = (int64_t) blockIdx.x * kRows + threadIdx.x / LANES; row < rows;
-         row += (int64_t) gridDim.x * kRows)
+    constexpr bool kHold = LANES < 1024 && PER <= 4;   // the weight stays in registers, where they allow it
+    any_u4 nx[PER], ng[PER], rw[PER];
+    float nm = 0.f, nr = 0.f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
     {
-        const float m = mean[row], r = rstd[row];
-        const T* px = x + row * width;
-        const T* pg = g + row * width;
+        const Piece<VEC> piece((i * LANES + lane) * VEC, width);
+        rw[i] = any_u4{0u, 0u, 0u, 0u};
+        if (kHold && w && piece.has)
+            rw[i] = raw_piece(w + piece.at, width);
+    }
+    const int64_t apart = (int64_t) gridDim.x * kRows;
+    int64_t row         = (int64_t) blockIdx.x * kRows + threadIdx.x / LANES;
+    const auto ask      = [&](int64_t at) {
+        nm = mean[at];
+        nr = rstd[at];
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+        {
+            const Piece<VEC> piece((i * LANES + lane) * VEC, width);
+            nx[i] = ng[i] = any_u4{0u, 0u, 0u, 0u};
+            if (piece.has)
+            {
+                nx[i] = raw_piece(x + at * width + piece.at, width);
+                ng[i] = raw_piece(g + at * width + piece.at, width);
+            }
+        }
+    };
+    if (row < rows)
+        ask(row);
+    for (; row < rows; row += apart)
+    {
+        const float m = nm, r = nr;
         float h[PER][VEC], gv[PER][VEC], s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int i = 0; i < PER; ++i)
         {
-            const int c = (i * LANES + lane) * VEC;
-            load_piece(px + c, width - c, h[i]);
-            load_piece(pg + c, width - c, gv[i]);
+            values_of(nx[i], h[i]);
+            values_of(ng[i], gv[i]);
         }
+        if (row + apart < rows)
+            ask(row + apart);
 #pragma unroll
         for (int i = 0; i < PER; ++i)
         {
-            const int c = (i * LANES + lane) * VEC;
-            if (c >= width)
+            const Piece<VEC> piece((i * LANES + lane) * VEC, width);
+            if (!piece.has)
                 continue;
             float ww[VEC];
-            if (w)
-                load_piece(w + c, width - c, ww);
+            if (kHold)
+                values_of(rw[i], ww);
+            else if (w)
+                load_piece(w + piece.at, width, ww);
 #pragma unroll
             for (int u = 0; u < VEC; ++u)
             {
-                h[i][u] = (h[i][u] - m) * r;   // (past the end: g is 0 there, and so is every sum's term)
+                h[i][u] = (h[i][u] - m) * r;   // (past the end of a short row g is 0, and so is every sum's term)
                 sw[i][u] = fmaf(gv[i][u], h[i][u], sw[i][u]);
                 sb[i][u] += gv[i][u];
                 if (w)
                     gv[i][u] *= ww[u];
-                s1 += gv[i][u];
-                s2 = fmaf(gv[i][u], h[i][u], s2);
+                const float once = u < piece.twice ? 0.f : gv[i][u];
+                s1 += once;
+                s2 = fmaf(once, h[i][u], s2);
             }
         }
         if (!dx)
             continue;
-        lanes_sum2<LANES>(s1, s2, lds);
+        lanes_sum2<LANES>(s1, s2, lds[odd]);
+        odd ^= 1;
         s1 /= (float) width;
         s2 /= (float) width;
 #pragma unroll
         for (int i = 0; i < PER; ++i)
         {
-            const int c = (i * LANES + lane) * VEC;
-            if (c >= width)
+            const Piece<VEC> piece((i * LANES + lane) * VEC, width);
+            if (!piece.has)
                 continue;
 #pragma unroll
             for (int u = 0; u < VEC; ++u)
                 gv[i][u] = r * (gv[i][u] - s1 - h[i][u] * s2);
-            store_piece(dx + row * width + c, width - c, gv[i]);
+            store_piece(dx + row * width + piece.at, width, gv[i]);
         }
     }
     if (!partial)
@@ -255,13 +349,17 @@ __global__ __launch_bounds__(LANES < kBlock ? kBlock : LANES) void ln_bwd_kernel
             if ((int) threadIdx.x / LANES == k)
 #pragma unroll
                 for (int i = 0; i < PER; ++i)
+                {
+                    const Piece<VEC> piece((i * LANES + lane) * VEC, width);
 #pragma unroll
                     for (int u = 0; u < VEC; ++u)
-                    {
-                        const int c = (i * LANES + lane) * VEC + u;
-                        both[0][c]  = k ? both[0][c] + sw[i][u] : sw[i][u];
-                        both[1][c]  = k ? both[1][c] + sb[i][u] : sb[i][u];
-                    }
+                        if (piece.has && u >= piece.twice)
+                        {
+                            const int c = piece.at + u;
+                            both[0][c]  = k ? both[0][c] + sw[i][u] : sw[i][u];
+                            both[1][c]  = k ? both[1][c] + sb[i][u] : sb[i][u];
+                        }
+                }
             __syncthreads();
         }
         for (int c = threadIdx.x; c < width; c += kBlock)
@@ -275,14 +373,14 @@ __global__ __launch_bounds__(LANES < kBlock ? kBlock : LANES) void ln_bwd_kernel
 #pragma unroll
         for (int i = 0; i < PER; ++i)
         {
-            const int c = (i * LANES + lane) * VEC;
-            if (c >= width)
+            const Piece<VEC> piece((i * LANES + lane) * VEC, width);
+            if (!piece.has)
                 continue;
 #pragma unroll
             for (int k = 0; k < VEC; k += 4)
             {
-                store_piece(partial + ((int64_t) blockIdx.x * 2) * width + c + k, width - c - k, sw[i] + k);
-                store_piece(partial + ((int64_t) blockIdx.x * 2 + 1) * width + c + k, width - c - k, sb[i] + k);
+                store_any(partial + ((int64_t) blockIdx.x * 2) * width + piece.at + k, sw[i] + k);
+                store_any(partial + ((int64_t) blockIdx.x * 2 + 1) * width + piece.at + k, sb[i] + k);
             }
         }
     }
@@ -386,7 +484,9 @@ Rows rows_of(int64_t width)
     return width <= 2048 ? Rows::kWave : width <= 8192 ? Rows::kBlock : width <= 16384 ? Rows::kWide : Rows::kLong;
 }
 
-// blocks of the backward pass: as many as the device holds at a time, no more than there are rows for
+// Blocks of the backward pass.  512 fill the device (16384 x 4096 bfloat16: 175 us with 256, 91 with 512, 93 with 768,
+// 104 with 1024, whose partial sums cost more than they hide; blocks of 1024 threads: half as many), and no more than give
+// each wave or block two rows (2048 x 1024 float32: 21 us with one row, 17 with two, 18 with four, 24 with eight).
 int64_t ln_slices(int64_t rows, int64_t width)
 {
     if (rows_of(width) == Rows::kLong)
@@ -394,7 +494,7 @@ int64_t ln_slices(int64_t rows, int64_t width)
         const int64_t columns = (width + kBlock - 1) / kBlock;
         return std::max<int64_t>(1, std::min<int64_t>((1024 + columns - 1) / columns, rows / 16));
     }
-    const int64_t each = rows_of(width) == Rows::kWave ? 4 : 1, most = rows_of(width) == Rows::kWide ? 256 : 512;
+    const int64_t each = rows_of(width) == Rows::kWave ? 8 : 2, most = rows_of(width) == Rows::kWide ? 256 : 512;
     return std::max<int64_t>(1, std::min<int64_t>(most, (rows + each - 1) / each));
 }
 
