@@ -205,8 +205,8 @@ __global__ __launch_bounds__(MT == 1 ? 1024 : 512) void few_rows_kernel(const T*
 // As float32 they are the first factor of v_mfma_f32_16x16x4: value u of all lanes makes columns VEC r + u, r = 0 .. 15,
 // so that a lane ends up with 4 VEC consecutive columns of one m.  A block makes 16 VEC columns; its waves share the sum.
 template <typename T, int MT>
-__global__ __launch_bounds__(512) void few_rows_columns_kernel(const T* __restrict__ a, const T* __restrict__ b,
-                                                               int64_t k, int64_t per_split, float* __restrict__ partial,
+__global__ __launch_bounds__(512) void few_rows_columns_kernel(const T* __restrict__ a, int64_t lda,
+                                                               const T* __restrict__ b, int64_t k, int64_t per_split, float* __restrict__ partial,
                                                                const Epilogue<T> e)
 {
     constexpr int VEC = IOTraits<T>::VEC, kUnroll = MT * VEC >= 16 ? 1 : 2;
@@ -222,7 +222,7 @@ __global__ __launch_bounds__(512) void few_rows_columns_kernel(const T* __restri
     for (int i = 0; i < MT; ++i)
     {
         const int64_t m = i * 16 + lane % 16;
-        pa[i]           = a + (m < e.m ? m : e.m - 1) * k;
+        pa[i]           = a + (m < e.m ? m : e.m - 1) * lda;
     }
     const bool inside = c + VEC <= e.n;
     f4 acc[MT][VEC];
@@ -298,8 +298,8 @@ __global__ __launch_bounds__(512) void few_rows_columns_kernel(const T* __restri
 
 // C[m, n] = sum over k of a[k][m] b[k][n] for a short k (the weight's gradient of a small batch), float32: writing C is
 // all that counts.  A wave makes 64 x 64 values from operands read straight from the caches.
-__global__ __launch_bounds__(kBlock) void short_sum_kernel(const float* __restrict__ a, const float* __restrict__ b,
-                                                           int k, const Epilogue<float> e)
+__global__ __launch_bounds__(kBlock) void short_sum_kernel(const float* __restrict__ a, int64_t lda,
+                                                           const float* __restrict__ b, int k, const Epilogue<float> e)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t tiles_n = (e.n + 127) / 128;
@@ -318,7 +318,7 @@ __global__ __launch_bounds__(kBlock) void short_sum_kernel(const float* __restri
         for (int i = 0; i < 4; ++i)
         {
             const int64_t m = m0 + i * 16 + lane % 16, n = n0 + i * 16 + lane % 16;
-            fa[i] = kk < k && m < e.m ? a[kk * e.m + m] : 0.f;
+            fa[i] = kk < k && m < e.m ? a[kk * lda + m] : 0.f;
             fb[i] = kk < k && n < e.n ? b[kk * e.n + n] : 0.f;
         }
 #pragma unroll

@@ -56,17 +56,12 @@ __device__ __forceinline__ void put_parts(const float* v, int shift, uint16_t* c
     *(uint4*) coarse = make_uint4(c[0] | c[1] << 16, c[2] | c[3] << 16, c[4] | c[5] << 16, c[6] | c[7] << 16);
     *(uint4*) fine   = make_uint4(f[0] | f[1] << 16, f[2] | f[3] << 16, f[4] | f[5] << 16, f[6] | f[7] << 16);
 }
-__device__ __forceinline__ void put_values(const uint16_t* v, uint16_t* to)
-{
-    *(uint4*) to = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
-}
-
 // out[r][0 .. kp) = src[r][0 .. k), zeros behind; float32: out[r][0 .. kp) coarse, out[r][kp .. 2 kp) fine, scale[r] = -s.
 // LANES threads hold a row of up to 32 LANES values in registers between its largest value and its halves; of a longer
 // one what is past them is read again.
 template <int LANES>
-__global__ __launch_bounds__(kBlock) void pack_rows_kernel(const float* __restrict__ src, int64_t rows, int64_t k,
-                                                           int64_t kp, uint16_t* __restrict__ out,
+__global__ __launch_bounds__(kBlock) void pack_rows_kernel(const float* __restrict__ src, int64_t ld, int64_t rows,
+                                                           int64_t k, int64_t kp, uint16_t* __restrict__ out,
                                                            int* __restrict__ scale)
 {
     constexpr int kHeld = 4;
@@ -74,7 +69,7 @@ __global__ __launch_bounds__(kBlock) void pack_rows_kernel(const float* __restri
     const int64_t r = (int64_t) blockIdx.x * (kBlock / LANES) + threadIdx.x / LANES;
     if (r >= rows)
         return;
-    const float* from = src + r * k;
+    const float* from = src + r * ld;
     float v[kHeld][8], t[8];
     uint32_t largest = 0;
 #pragma unroll
@@ -133,19 +128,25 @@ __global__ __launch_bounds__(kBlock) void copy_rows_kernel(const T* __restrict__
     if (at >= rows * per)
         return;
     const int64_t r = at / per, c = at % per * VEC;
-    T v[VEC];
-#pragma unroll
-    for (int u = 0; u < VEC; ++u)
-        v[u] = c + u < k ? src[r * k + c + u] : (T) 0;
-    if constexpr (VEC == 8)
-        put_values(v, out + r * kp + c);
+    any_u4 v          = {0u, 0u, 0u, 0u};
+    if (c + VEC <= k)
+        v = *(const any_u4*) (src + r * k + c);
     else
-        *(float4*) (out + r * kp + c) = make_float4(v[0], v[1], v[2], v[3]);
+#pragma unroll
+        for (int u = 0; u < VEC; ++u)
+            if (c + u < k)
+            {
+                if constexpr (VEC == 4)
+                    v[u] = __float_as_uint(src[r * k + c + u]);
+                else
+                    v[u / 2] |= (uint32_t) src[r * k + c + u] << (u % 2 * 16);
+            }
+    *(uint4*) (out + r * kp + c) = make_uint4(v[0], v[1], v[2], v[3]);
 }
 
 // largest[slice][c] = largest finite magnitude (its bits) in a slice of the rows of column c of src [k][count]: 64 threads
 // of 4 columns across, 4 rows at a time
-__global__ __launch_bounds__(kBlock) void column_max_kernel(const float* __restrict__ src, int64_t k, int64_t count,
+__global__ __launch_bounds__(kBlock) void column_max_kernel(const float* __restrict__ src, int64_t ld, int64_t k, int64_t count,
                                                             int64_t rows_per_slice, uint32_t* __restrict__ largest)
 {
     __shared__ uint32_t lds[4][256];
@@ -160,7 +161,7 @@ __global__ __launch_bounds__(kBlock) void column_max_kernel(const float* __restr
         for (int64_t r = first + down; r < last; r += 4)
         {
             float v[4];
-            load_any(src + r * count + c, v);
+            load_any(src + r * ld + c, v);
 #pragma unroll
             for (int u = 0; u < 4; ++u)
                 m[u] = max(m[u], finite_magnitude(v[u]));
@@ -170,7 +171,7 @@ __global__ __launch_bounds__(kBlock) void column_max_kernel(const float* __restr
         for (int64_t r = first + down; r < last; r += 4)
             for (int u = 0; u < 4; ++u)
                 if (c + u < count)
-                    m[u] = max(m[u], finite_magnitude(src[r * count + c + u]));
+                    m[u] = max(m[u], finite_magnitude(src[r * ld + c + u]));
 #pragma unroll
     for (int u = 0; u < 4; ++u)
         lds[down][u * 64 + across] = m[u];
@@ -181,15 +182,14 @@ __global__ __launch_bounds__(kBlock) void column_max_kernel(const float* __restr
         largest[blockIdx.y * count + q] = max(max(lds[0][at], lds[1][at]), max(lds[2][at], lds[3][at]));
 }
 
-// As pack_rows_kernel and copy_rows_kernel, of the transpose: src [k][count], row r of the result is column r of src.
-// 64 x 64 values a block, through LDS.
-template <typename T>
-__global__ __launch_bounds__(kBlock) void pack_columns_kernel(const T* __restrict__ src, int64_t k, int64_t count,
-                                                              int64_t kp, const uint32_t* __restrict__ largest,
-                                                              int slices, uint16_t* __restrict__ out,
-                                                              int* __restrict__ scale)
+// As pack_rows_kernel, of the transpose: src [k][count], row r of the result is column r of src.  64 x 64 values a block,
+// through LDS.
+__global__ __launch_bounds__(kBlock) void pack_columns_kernel(const float* __restrict__ src, int64_t ld, int64_t k,
+                                                              int64_t count, int64_t kp,
+                                                              const uint32_t* __restrict__ largest, int slices,
+                                                              uint16_t* __restrict__ out, int* __restrict__ scale)
 {
-    __shared__ T tile[64][65];
+    __shared__ float tile[64][65];
     __shared__ int shifts[64];
     const int64_t across = (count + 63) / 64;
     const int64_t r0 = blockIdx.x % across * 64, k0 = blockIdx.x / across * 64;
@@ -198,19 +198,18 @@ __global__ __launch_bounds__(kBlock) void pack_columns_kernel(const T* __restric
     for (int i = 0; i < 16; ++i)
     {
         const int64_t kk = k0 + i * 4 + wave;
-        tile[i * 4 + wave][lane] = kk < k && r0 + lane < count ? src[kk * count + r0 + lane] : (T) 0;
+        tile[i * 4 + wave][lane] = kk < k && r0 + lane < count ? src[kk * ld + r0 + lane] : 0.f;
     }
-    if constexpr (std::is_same<T, float>::value)
-        if (threadIdx.x < 64)
-        {
-            uint32_t m = 0;
-            if (r0 + lane < count)
-                for (int i = 0; i < slices; ++i)
-                    m = max(m, largest[i * count + r0 + lane]);
-            shifts[lane] = row_shift(m);
-            if (k0 == 0 && r0 + lane < count)
-                scale[r0 + lane] = -row_shift(m);
-        }
+    if (threadIdx.x < 64)
+    {
+        uint32_t m = 0;
+        if (r0 + lane < count)
+            for (int i = 0; i < slices; ++i)
+                m = max(m, largest[i * count + r0 + lane]);
+        shifts[lane] = row_shift(m);
+        if (k0 == 0 && r0 + lane < count)
+            scale[r0 + lane] = -row_shift(m);
+    }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -218,25 +217,20 @@ __global__ __launch_bounds__(kBlock) void pack_columns_kernel(const T* __restric
         const int r = (i * kBlock + threadIdx.x) / 8, c = threadIdx.x % 8 * 8;
         if (r0 + r >= count || k0 + c >= kp)
             continue;
-        T v[8];
+        float v[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u)
             v[u] = tile[c + u][r];
-        if constexpr (std::is_same<T, float>::value)
-        {
-            uint16_t* to = out + (r0 + r) * 2 * kp + k0 + c;
-            put_parts(v, shifts[r], to, to + kp);
-        }
-        else
-            put_values(v, out + (r0 + r) * kp + k0 + c);
+        uint16_t* to = out + (r0 + r) * 2 * kp + k0 + c;
+        put_parts(v, shifts[r], to, to + kp);
     }
 }
 
 // dz = g act'(z) and its column sums over a slice of the rows: a thread takes 8 columns, 32 threads across and 8 rows at
-// a time
+// a time.  dz may be null for ACT none; its rows are `ld` values apart, zeros behind the last column.
 template <typename T, int ACT>
 __global__ __launch_bounds__(kBlock) void slope_kernel(const T* __restrict__ g, const Saved<T>* __restrict__ z,
-                                                       int64_t rows, int64_t cols, int64_t rows_per_slice,
+                                                       int64_t rows, int64_t cols, int64_t ld, int64_t rows_per_slice,
                                                        T* __restrict__ dz, float* __restrict__ partial)
 {
     constexpr int VEC = 8, kAcross = 32, kDown = kBlock / kAcross;
@@ -259,8 +253,9 @@ __global__ __launch_bounds__(kBlock) void slope_kernel(const T* __restrict__ g, 
 #pragma unroll
                 for (int u = 0; u < VEC; ++u)
                     d[u] *= act_slope<ACT>(s[u]);
-                store8(dz + at, cols - c, d);
             }
+            if (dz)
+                store8(dz + r * ld + c, ld - c, d);
 #pragma unroll
             for (int u = 0; u < VEC; ++u)
                 sum[u] += d[u];
@@ -348,7 +343,8 @@ struct Matrix
     const T* p;
     int64_t count, k;
     bool columns;
-    bool at16;   // p is a multiple of 16 bytes
+    bool at16;    // p is a multiple of 16 bytes
+    int64_t ld;   // values from one row of memory to the next; what is past a row's end is zeros, if anything
 
     int64_t inner() const
     {
@@ -360,13 +356,16 @@ struct Matrix
     }
     bool whole() const   // every row is whole 16-byte chunks
     {
-        return at16 && inner() * (int64_t) sizeof(T) % 16 == 0;
+        return at16 && ld * (int64_t) sizeof(T) % 16 == 0;
     }
 };
 
-int64_t up4(int64_t n)
+// rows of whole 16-byte chunks
+template <typename T>
+int64_t padded(int64_t n)
 {
-    return (n + 3) / 4 * 4;
+    constexpr int VEC = 16 / sizeof(T);
+    return (n + VEC - 1) / VEC * VEC;
 }
 
 int64_t max_slices(int64_t k)
@@ -398,12 +397,40 @@ enum class Way
 struct Plan
 {
     Way way;
-    bool pack_a, pack_b;
-    int64_t kp;   // length of packed rows
-    bool big;     // 256 x 256 tiles, else 128 x 128 (kDirect: 128 x 128, else 64 x 128)
+    int64_t kp;   // kTiles, float32: length of the rows of halves
+    bool big;     // kTiles: 256 x 256, else 128 x 128; kDirect: 128 x 128, else 64 x 128
     int splits;
     int64_t a_bytes, b_bytes, scale_a, scale_b, partial, total;   // of the workspace
 };
+
+// Tiles and pieces of the sum for a product of `slices` slices a pass.  What a launch costs, in us, as measured on many
+// shapes (within 10 % for most): 5, and for each round of tiles that the device holds at a time and each slice of theirs
+//   256 x 256, one a CU: 1.5, 1.25 when half of the CUs have none    128 x 128, two a CU: 1.05, 0.6 when there is one
+// and to join the pieces 4 and 1 for each million of partial values.  E.g. [4096, 1024] x [1024, 1024]^T: 15 whole, 26 in two
+// pieces; [512, 4096] x [4096, 4096]^T: 42, 32 and 32 in two and four; [2048, 11008] x [4096, 11008]^T: 191 in 128 x 128
+// tiles, 165 in 256 x 256 in two pieces.
+void choose_tiles(int64_t m, int64_t n, int64_t slices, int passes, Plan* p)
+{
+    double best = 1e30;
+    for (const bool big : {false, true})
+    {
+        const int64_t side = big ? 256 : 128, tiles = (m + side - 1) / side * ((n + side - 1) / side);
+        for (int64_t splits = 1; splits <= 32 && (splits == 1 || slices >= 4 * splits); splits *= 2)
+        {
+            const int64_t blocks = tiles * splits, at_once = big ? 256 : 512, rounds = (blocks + at_once - 1) / at_once;
+            const bool sparse    = rounds == 1 && blocks <= at_once / 2;
+            const double slice   = big ? (sparse ? 1.25 : 1.5) : (sparse ? 0.6 : 1.05);
+            const double cost    = 5 + (double) rounds * ((slices + splits - 1) / splits) * passes * slice +
+                                (splits > 1 ? 4 + 1e-6 * splits * m * n : 0);
+            if (cost < best)
+            {
+                best      = cost;
+                p->big    = big;
+                p->splits = (int) splits;
+            }
+        }
+    }
+}
 
 template <typename T>
 Plan plan_product(const Matrix<T>& a, const Matrix<T>& b)
@@ -416,6 +443,10 @@ Plan plan_product(const Matrix<T>& a, const Matrix<T>& b)
         p.partial = p.splits > 1 ? up256(p.splits * m * n * 4) : 0;
         p.total   = p.a_bytes + p.b_bytes + p.scale_a + p.scale_b + p.partial;
         return p;
+    };
+    // rows that are not whole chunks are copied, with zeros behind them
+    const auto copied = [&](const Matrix<T>& x) {
+        return x.whole() ? 0 : up256(x.outer() * padded<T>(x.inner()) * (int64_t) sizeof(T));
     };
     const auto tiles = [&](int64_t tm, int64_t tn) { return (m + tm - 1) / tm * ((n + tn - 1) / tn); };
     if (!a.columns && !b.columns && m <= 16)
@@ -439,25 +470,21 @@ Plan plan_product(const Matrix<T>& a, const Matrix<T>& b)
     if (kF32 && direct_pays(a, b))
     {
         p.way = Way::kDirect;
-        // rows that are not whole chunks are copied, with zeros behind them
-        const auto copied = [&](const Matrix<T>& x) { return x.whole() ? 0 : up256(x.outer() * up4(x.inner()) * 4); };
         p.a_bytes = copied(a), p.b_bytes = copied(b);
         p.big = m > 64;
         p.splits = (int) std::max<int64_t>(1, std::min<int64_t>(512 / std::max<int64_t>(tiles(p.big ? 128 : 64, 128), 1), k / 256));
         return done();
     }
-    p.way    = Way::kTiles;
-    p.pack_a = kF32 || !a.whole(), p.pack_b = kF32 || !b.whole();
-    if (a.columns && (p.pack_a || p.pack_b))
-        p.pack_a = p.pack_b = true;   // both in columns, or both in rows
-    p.kp  = kF32 ? (k + kSlice - 1) / kSlice * kSlice : (k + 7) / 8 * 8;
-    p.big = tiles(256, 256) >= 200;
-    if (!p.big)
-        p.splits = (int) std::max<int64_t>(1, std::min<int64_t>(512 / std::max<int64_t>(tiles(128, 128), 1), (k + kSlice - 1) / kSlice / 8));
-    const int64_t each = (kF32 ? 2 : 1) * p.kp * 2;
-    p.a_bytes = p.pack_a ? up256(m * each) : 0, p.b_bytes = p.pack_b ? up256(n * each) : 0;
-    p.scale_a = kF32 ? up256(m * 4 * (1 + (a.columns ? max_slices(k) : 0))) : 0;
-    p.scale_b = kF32 ? up256(n * 4 * (1 + (b.columns ? max_slices(k) : 0))) : 0;
+    p.way = Way::kTiles;
+    choose_tiles(m, n, (k + kSlice - 1) / kSlice, kF32 ? 3 : 1, &p);
+    p.a_bytes = copied(a), p.b_bytes = copied(b);
+    if (kF32)
+    {
+        p.kp      = (k + kSlice - 1) / kSlice * kSlice;
+        p.a_bytes = up256(m * 2 * p.kp * 2), p.b_bytes = up256(n * 2 * p.kp * 2);
+        p.scale_a = up256(m * 4 * (1 + (a.columns ? max_slices(k) : 0)));
+        p.scale_b = up256(n * 4 * (1 + (b.columns ? max_slices(k) : 0)));
+    }
     return done();
 }
 
@@ -473,8 +500,7 @@ int copy_rows(const T* src, int64_t rows, int64_t k, int64_t kp, T* to, hipStrea
     return MIQ_OK;
 }
 
-template <typename T>
-int pack(const Matrix<T>& x, int64_t kp, char* to, char* scale, hipStream_t s)
+int pack(const Matrix<float>& x, int64_t kp, char* to, char* scale, hipStream_t s)
 {
     if (x.count == 0 || kp == 0)
         return MIQ_OK;
@@ -482,36 +508,38 @@ int pack(const Matrix<T>& x, int64_t kp, char* to, char* scale, hipStream_t s)
     uint32_t* largest = (uint32_t*) scale + x.count;
     if (!x.columns)
     {
-        if constexpr (std::is_same<T, float>::value)
-        {
-            if (x.k <= 2048)
-                hipLaunchKernelGGL(pack_rows_kernel<64>, dim3((unsigned) ((x.count + 3) / 4)), dim3(kBlock), 0, s, x.p,
-                                   x.count, x.k, kp, (uint16_t*) to, exponents);
-            else
-                hipLaunchKernelGGL(pack_rows_kernel<256>, dim3((unsigned) x.count), dim3(kBlock), 0, s, x.p, x.count,
-                                   x.k, kp, (uint16_t*) to, exponents);
-        }
+        if (x.k <= 2048)
+            hipLaunchKernelGGL(pack_rows_kernel<64>, dim3((unsigned) ((x.count + 3) / 4)), dim3(kBlock), 0, s, x.p, x.ld,
+                               x.count, x.k, kp, (uint16_t*) to, exponents);
         else
-        {
-            if (int rc = copy_rows(x.p, x.count, x.k, kp, (uint16_t*) to, s))
-                return rc;
-        }
+            hipLaunchKernelGGL(pack_rows_kernel<256>, dim3((unsigned) x.count), dim3(kBlock), 0, s, x.p, x.ld, x.count,
+                               x.k, kp, (uint16_t*) to, exponents);
         MIQ_CHECK_LAUNCH();
         return MIQ_OK;
     }
     const int64_t slices = max_slices(x.k);
-    if constexpr (std::is_same<T, float>::value)
-    {
-        hipLaunchKernelGGL(column_max_kernel, dim3((unsigned) ((x.count + 255) / 256), (unsigned) slices), dim3(kBlock), 0,
-                           s, x.p, x.k, x.count, (x.k + slices - 1) / slices, largest);
-        MIQ_CHECK_LAUNCH();
-    }
+    hipLaunchKernelGGL(column_max_kernel, dim3((unsigned) ((x.count + 255) / 256), (unsigned) slices), dim3(kBlock), 0, s,
+                       x.p, x.ld, x.k, x.count, (x.k + slices - 1) / slices, largest);
+    MIQ_CHECK_LAUNCH();
     const int64_t tiles = ((x.count + 63) / 64) * ((kp + 63) / 64);
     MIQ_CHECK_ARG(tiles <= INT32_MAX, "an operand has too many tiles");
-    hipLaunchKernelGGL(pack_columns_kernel<T>, dim3((unsigned) tiles), dim3(kBlock), 0, s, x.p, x.k, x.count, kp,
+    hipLaunchKernelGGL(pack_columns_kernel, dim3((unsigned) tiles), dim3(kBlock), 0, s, x.p, x.ld, x.k, x.count, kp,
                        largest, (int) slices, (uint16_t*) to, exponents);
     MIQ_CHECK_LAUNCH();
     return MIQ_OK;
+}
+
+// The operand as a kernel of 16-byte chunks reads it: as it lies, or copied to `at`, which then moves on
+template <typename T, typename E>
+int as_read(const Matrix<T>& x, int64_t bytes, char** at, Operand<E>* o, hipStream_t s)
+{
+    *o = {(const E*) x.p, x.ld, x.count};
+    if (x.whole())
+        return MIQ_OK;
+    T* const to = (T*) *at;
+    *o          = {(const E*) to, padded<T>(x.inner()), x.count};
+    *at += bytes;
+    return copy_rows(x.p, x.outer(), x.inner(), o->ld, to, s);
 }
 
 template <typename T, int ACT>
@@ -576,7 +604,7 @@ int launch_few_rows_columns(const Matrix<T>& a, const Matrix<T>& b, const Plan& 
     constexpr int VEC  = IOTraits<T>::VEC, kWaves = 8;
     const int64_t wide = (b.count + 16 * VEC - 1) / (16 * VEC), per = (a.k + plan.splits - 1) / plan.splits;
     hipLaunchKernelGGL((few_rows_columns_kernel<T, MT>), dim3((unsigned) wide, (unsigned) plan.splits), dim3(kWaves * 64),
-                       kWaves * MT * VEC * 1024, s, a.p, b.p, a.k, per, plan.splits > 1 ? partial : nullptr, e);
+                       kWaves * MT * VEC * 1024, s, a.p, a.ld, b.p, a.k, per, plan.splits > 1 ? partial : nullptr, e);
     MIQ_CHECK_LAUNCH();
     return launch_join<T, MIQ_ACT_NONE>(partial, plan.splits, e, s);
 }
@@ -602,26 +630,18 @@ int product(const Matrix<T>& a, const Matrix<T>& b, const T* bias, const T* resi
         {
             const int64_t tiles = ((e.m + 127) / 128) * ((e.n + 127) / 128);
             MIQ_CHECK_ARG(tiles <= INT32_MAX, "the product has too many tiles");
-            hipLaunchKernelGGL(short_sum_kernel, dim3((unsigned) tiles), dim3(kBlock), 0, s, a.p, b.p, (int) a.k, e);
+            hipLaunchKernelGGL(short_sum_kernel, dim3((unsigned) tiles), dim3(kBlock), 0, s, a.p, a.ld, b.p, (int) a.k, e);
             MIQ_CHECK_LAUNCH();
             return MIQ_OK;
         }
     if constexpr (kF32)
         if (plan.way == Way::kDirect)
         {
-            char* at        = workspace;
-            const auto as_read = [&](const Matrix<T>& x, int64_t bytes, Operand<float>* o) {
-                *o = {x.p, x.inner(), x.count};
-                if (x.whole())
-                    return MIQ_OK;
-                *o = {(const float*) at, up4(x.inner()), x.count};
-                at += bytes;
-                return copy_rows(x.p, x.outer(), x.inner(), o->ld, (float*) o->p, s);
-            };
             DirectProduct p = {{}, {}, a.k, 0, 0, plan.splits, nullptr, e};
-            if (int rc = as_read(a, plan.a_bytes, &p.a))
+            char* at        = workspace;
+            if (int rc = as_read(a, plan.a_bytes, &at, &p.a, s))
                 return rc;
-            if (int rc = as_read(b, plan.b_bytes, &p.b))
+            if (int rc = as_read(b, plan.b_bytes, &at, &p.b, s))
                 return rc;
             p.partial = (float*) at;
             if constexpr (kPlain)
@@ -633,65 +653,107 @@ int product(const Matrix<T>& a, const Matrix<T>& b, const T* bias, const T* resi
             }
             return launch_direct<ACT, false, false>(p, plan.big, s);
         }
-    Product<T> p   = {};
-    p.e            = e;
-    char* const pa = workspace;
-    char* const pb = pa + plan.a_bytes;
-    char* const sa = pb + plan.b_bytes;
-    char* const sb = sa + plan.scale_a;
-    p.a = {(const uint16_t*) a.p, a.columns ? a.count : a.k, a.count};
-    p.b = {(const uint16_t*) b.p, b.columns ? b.count : b.k, b.count};
-    const int64_t ld = (kF32 ? 2 : 1) * plan.kp;
-    if (plan.pack_a)
+    Product<T> p = {};
+    p.e          = e;
+    p.splits     = plan.splits;
+    char* at     = workspace;
+    if constexpr (kF32)
     {
-        if (int rc = pack(a, plan.kp, pa, sa, s))
+        char* const pb = at + plan.a_bytes;
+        char* const sa = pb + plan.b_bytes;
+        char* const sb = sa + plan.scale_a;
+        if (int rc = pack(a, plan.kp, at, sa, s))
             return rc;
-        p.a = {(const uint16_t*) pa, ld, a.count};
-    }
-    if (plan.pack_b)
-    {
         if (int rc = pack(b, plan.kp, pb, sb, s))
             return rc;
-        p.b = {(const uint16_t*) pb, ld, b.count};
-    }
-    p.k       = plan.pack_a && plan.pack_b ? plan.kp : a.k;
-    p.scale_a = (const int*) sa, p.scale_b = (const int*) sb;
-    p.splits  = plan.splits;
-    p.partial = (float*) (sb + plan.scale_b);
-    if constexpr (kF32)
+        p.a       = {(const uint16_t*) at, 2 * plan.kp, a.count};
+        p.b       = {(const uint16_t*) pb, 2 * plan.kp, b.count};
+        p.k       = plan.kp;
+        p.scale_a = (const int*) sa, p.scale_b = (const int*) sb;
+        p.partial = (float*) (sb + plan.scale_b);
         return launch_product<T, ACT, false, false>(p, plan.big, s);
+    }
     else
     {
-        const bool ac = a.columns && !plan.pack_a, bc = b.columns && !plan.pack_b;
+        if (int rc = as_read(a, plan.a_bytes, &at, &p.a, s))
+            return rc;
+        if (int rc = as_read(b, plan.b_bytes, &at, &p.b, s))
+            return rc;
+        p.k       = a.k;
+        p.partial = (float*) at;
         if constexpr (kPlain)
         {
-            if (ac && bc)
+            if (a.columns)
                 return launch_product<T, ACT, true, true>(p, plan.big, s);
-            if (bc)
+            if (b.columns)
                 return launch_product<T, ACT, false, true>(p, plan.big, s);
         }
         return launch_product<T, ACT, false, false>(p, plan.big, s);
     }
 }
 
-// bytes of the workspace; `at16`: every tensor starts on a multiple of 16 bytes
 template <typename T>
-int64_t product_bytes(int64_t m, int64_t n, int64_t k, bool ac, bool bc, bool a16, bool b16)
+int64_t product_bytes(const Matrix<T>& a, const Matrix<T>& b)
 {
-    return m == 0 || n == 0 ? 0 : plan_product<T>({nullptr, m, k, ac, a16}, {nullptr, n, k, bc, b16}).total;
+    return a.count == 0 || b.count == 0 ? 0 : plan_product(a, b).total;
 }
 
+// The operands of the three products.  at16: x, w and grad start on multiples of 16 bytes.
 template <typename T>
-int64_t workspace_bytes(int64_t rows, int64_t in, int64_t out, int activation, bool backward, bool at16)
+struct Operands
 {
-    if (!backward)
-        return product_bytes<T>(rows, out, in, false, false, at16, at16);
-    const bool kept = activation != MIQ_ACT_NONE;   // dz is the workspace's then
-    return (kept ? up256(rows * out * (int64_t) sizeof(T)) : 0) +
-           up256(slope_slices(rows, out) * out * (int64_t) sizeof(float)) +
-           std::max(product_bytes<T>(rows, in, out, false, true, kept || at16, at16),
-                    product_bytes<T>(out, in, rows, true, true, kept || at16, at16));
-}
+    int64_t rows, in, out;
+    int activation;
+    bool at16;
+
+    Matrix<T> x_rows(const T* x) const
+    {
+        return {x, rows, in, false, at16, in};
+    }
+    Matrix<T> w_rows(const T* w) const
+    {
+        return {w, out, in, false, at16, in};
+    }
+    Matrix<T> x_columns(const T* x) const
+    {
+        return {x, in, rows, true, at16, in};
+    }
+    Matrix<T> w_columns(const T* w) const
+    {
+        return {w, in, out, true, at16, in};
+    }
+    // dz is grad itself, or is written to the workspace, in rows of whole chunks: where there is an activation, and where
+    // grad would have to be copied anyway
+    bool own_dz() const
+    {
+        return activation != MIQ_ACT_NONE || !at16 || padded<T>(out) != out;
+    }
+    int64_t dz_bytes() const
+    {
+        return own_dz() ? up256(rows * padded<T>(out) * (int64_t) sizeof(T)) : 0;
+    }
+    int64_t sums_bytes() const
+    {
+        return up256(slope_slices(rows, out) * out * (int64_t) sizeof(float));
+    }
+    Matrix<T> dz_rows(const T* dz) const
+    {
+        return {dz, rows, out, false, true, padded<T>(out)};
+    }
+    Matrix<T> dz_columns(const T* dz) const
+    {
+        return {dz, out, rows, true, true, padded<T>(out)};
+    }
+    int64_t forward_bytes() const
+    {
+        return product_bytes(x_rows(nullptr), w_rows(nullptr));
+    }
+    int64_t backward_bytes() const
+    {
+        return dz_bytes() + sums_bytes() + std::max(product_bytes(dz_rows(nullptr), w_columns(nullptr)),
+                                                    product_bytes(dz_columns(nullptr), x_columns(nullptr)));
+    }
+};
 
 template <typename T>
 int linear_fwd(const T* x, const T* w, const T* bias, const T* residual, int64_t rows, int64_t in, int64_t out,
@@ -702,11 +764,13 @@ int linear_fwd(const T* x, const T* w, const T* bias, const T* residual, int64_t
     if (rows == 0 || out == 0)
         return MIQ_OK;
     MIQ_CHECK_ARG(y && (in == 0 || (x && w)), "null pointer");
-    const int64_t need = workspace_bytes<T>(rows, in, out, activation, false, aligned(x) && aligned(w));
+    const Operands<T> o = {rows, in, out, activation, aligned(x) && aligned(w)};
+    const int64_t need  = o.forward_bytes();
     MIQ_CHECK_ARG(bytes >= need && (workspace || need == 0), "the workspace is too small");
+    MIQ_CHECK_ARG(need == 0 || (uintptr_t) workspace % 256 == 0, "the workspace is not aligned to 256 bytes");
     int rc = MIQ_OK;
     with_activation(activation, [&](auto act) {
-        rc = product<T, act.value>({x, rows, in, false, aligned(x)}, {w, out, in, false, aligned(w)}, bias, residual, y, (Saved<T>*) saved,
+        rc = product<T, act.value>(o.x_rows(x), o.w_rows(w), bias, residual, y, (Saved<T>*) saved,
                                    (char*) workspace, (hipStream_t) stream);
     });
     return rc;
@@ -722,38 +786,34 @@ int linear_bwd(const T* g, const void* saved, const T* x, const T* w, int64_t ro
     MIQ_CHECK_ARG(rows * out == 0 || (g && (saved || !kept)), "null pointer");
     MIQ_CHECK_ARG(rows * in == 0 || !dw || x, "dweight needs x");
     MIQ_CHECK_ARG(out * in == 0 || !dx || w, "dx needs weight");
-    const bool at16    = aligned(g) && aligned(x) && aligned(w);
-    const int64_t need = workspace_bytes<T>(rows, in, out, activation, true, at16);
+    const Operands<T> o = {rows, in, out, activation, aligned(g) && aligned(x) && aligned(w)};
+    const int64_t need  = o.backward_bytes();
     MIQ_CHECK_ARG(bytes >= need && (workspace || need == 0), "the workspace is too small");
+    MIQ_CHECK_ARG(need == 0 || (uintptr_t) workspace % 256 == 0, "the workspace is not aligned to 256 bytes");
     hipStream_t s  = (hipStream_t) stream;
-    const T* dz    = g;
     char* at       = (char*) workspace;
-    T* own_dz      = (T*) at;
-    at += kept ? up256(rows * out * (int64_t) sizeof(T)) : 0;
-    float* partial = (float*) at;
+    T* own_dz      = o.own_dz() ? (T*) at : nullptr;
+    const T* dz    = own_dz ? own_dz : g;
+    float* partial = (float*) (at + o.dz_bytes());
+    at += o.dz_bytes() + o.sums_bytes();
     const int64_t slices = slope_slices(rows, out);
-    at += up256(slices * out * (int64_t) sizeof(float));
-    if ((kept || db) && out > 0)
+    if ((own_dz || db) && out > 0)
     {
         const dim3 grid((unsigned) ((out + 255) / 256), (unsigned) slices);
         with_activation(activation, [&](auto act) {
             hipLaunchKernelGGL((slope_kernel<T, act.value>), grid, dim3(kBlock), 0, s, g, (const Saved<T>*) saved, rows, out,
-                               (rows + slices - 1) / slices, own_dz, db ? partial : nullptr);
+                               padded<T>(out), (rows + slices - 1) / slices, own_dz, db ? partial : nullptr);
         });
         MIQ_CHECK_LAUNCH();
-        if (kept)
-            dz = own_dz;
         if (db)
             hipLaunchKernelGGL(join_columns_kernel<T>, dim3((unsigned) ((out + 63) / 64)), dim3(kBlock), 0, s, partial, slices, out, db);
         MIQ_CHECK_LAUNCH();
     }
     int rc = MIQ_OK;
     if (dx)
-        rc = product<T, MIQ_ACT_NONE>({dz, rows, out, false, kept || at16}, {w, in, out, true, at16}, nullptr, nullptr, dx,
-                                      nullptr, at, s);
+        rc = product<T, MIQ_ACT_NONE>(o.dz_rows(dz), o.w_columns(w), nullptr, nullptr, dx, nullptr, at, s);
     if (rc == MIQ_OK && dw)
-        rc = product<T, MIQ_ACT_NONE>({dz, out, rows, true, kept || at16}, {x, in, rows, true, at16}, nullptr, nullptr, dw,
-                                      nullptr, at, s);
+        rc = product<T, MIQ_ACT_NONE>(o.dz_columns(dz), o.x_columns(x), nullptr, nullptr, dw, nullptr, at, s);
     return rc;
 }
 }   // namespace
@@ -768,8 +828,13 @@ int64_t miq_linear_workspace_bytes(int64_t rows, int64_t in_features, int64_t ou
 {
     if (rows < 0 || in_features < 0 || out_features < 0)
         return 0;
-    return bf16 ? workspace_bytes<uint16_t>(rows, in_features, out_features, activation, backward != 0, aligned != 0)
-                : workspace_bytes<float>(rows, in_features, out_features, activation, backward != 0, aligned != 0);
+    if (bf16)
+    {
+        const Operands<uint16_t> o = {rows, in_features, out_features, activation, aligned != 0};
+        return backward ? o.backward_bytes() : o.forward_bytes();
+    }
+    const Operands<float> o = {rows, in_features, out_features, activation, aligned != 0};
+    return backward ? o.backward_bytes() : o.forward_bytes();
 }
 
 int miq_linear_fwd_f32(const float* x, const float* weight, const float* bias, const float* residual, int64_t rows,
