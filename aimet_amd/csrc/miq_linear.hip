@@ -325,7 +325,9 @@ int64_t up256(int64_t n)
 int check_shape(int64_t rows, int64_t in, int64_t out, int activation)
 {
     MIQ_CHECK_ARG(rows >= 0 && in >= 0 && out >= 0, "rows, in_features and out_features must not be negative");
-    MIQ_CHECK_ARG(rows <= INT32_MAX && in <= INT32_MAX && out <= INT32_MAX, "a size is 2^31 or more");
+    MIQ_CHECK_ARG(rows <= INT32_MAX, "rows must be below 2^31");
+    // (a lane's offset within the rows that a load spans has 32 bits)
+    MIQ_CHECK_ARG(in <= 1 << 27 && out <= 1 << 27, "in_features and out_features must be at most 2^27");
     MIQ_CHECK_ARG(activation >= MIQ_ACT_NONE && activation <= MIQ_ACT_GELU_TANH, "unknown activation %d", activation);
     return MIQ_OK;
 }
@@ -374,14 +376,17 @@ int64_t max_slices(int64_t k)
 }
 
 // Whether a float32 product is formed from its operands as they lie (miq_direct.h) or from halves made beforehand.
-// Measured: the first runs at about 170 TFLOP/s, the second at up to 380 once the halves are there; making them takes
-// about 22 us of launches and 3 ps a value of an operand in rows, 5 ps in columns (one more pass).  E.g. [512, 4096] x
-// [4096, 4096]^T: 115 us and 107 us, [256, 4096] x [11008, 4096]^T: 177 us and 192 us, [1024, 4096] x [4096, 4096]^T:
-// 204 us and 171 us.
+// Measured: the first runs at about 160 TFLOP/s, the second at up to 380 once the halves are there; making them takes
+// 3 ps a value of an operand in rows and 5 ps in columns (one more pass), and 22 us of launches, 20 more for each operand in
+// columns.  In us, as they lie and by halves: [512, 4096] x [4096, 4096]^T 106 and 122, [1024, 4096] x [4096, 4096]^T 189 and
+// 162; the input's gradient of [512, 4096] x [11008, 4096]^T 246 and 349, of [1024, ...] 476 and 460; the weight's
+// gradient of [256, 4096] x [11008, 4096]^T 150 and 194, of [512, ...] 266 and 256.
 template <typename T>
 bool direct_pays(const Matrix<T>& a, const Matrix<T>& b)
 {
-    const auto halves = [](const Matrix<T>& x) { return (double) x.count * x.k * (x.columns ? 5e-12 : 3e-12); };
+    const auto halves = [](const Matrix<T>& x) {
+        return (double) x.count * x.k * (x.columns ? 5e-12 : 3e-12) + (x.columns ? 20e-6 : 0);
+    };
     return 3.5e-15 * 2.0 * a.count * b.count * a.k <= 22e-6 + halves(a) + halves(b);
 }
 

@@ -41,6 +41,8 @@ def test_linear_refusals(lib, suffix):
     big = 1 << 40
     _refused(lib, fwd(P, P, None, None, -1, 8, 8, 0, P, None, P, big, None), "negative")
     _refused(lib, fwd(P, P, None, None, 1 << 31, 8, 8, 0, P, None, P, big, None), "2^31")
+    _refused(lib, fwd(P, P, None, None, 4, (1 << 27) + 1, 8, 0, P, None, P, big, None), "2^27")
+    _refused(lib, fwd(P, P, None, None, 4, 8, (1 << 27) + 1, 0, P, None, P, big, None), "2^27")
     _refused(lib, fwd(P, P, None, None, 4, 8, 8, 5, P, None, P, big, None), "activation")
     _refused(lib, fwd(None, P, None, None, 4, 8, 8, 0, P, None, P, big, None), "null")
     _refused(lib, fwd(P, P, None, None, 4, 8, 8, 0, None, None, P, big, None), "null")

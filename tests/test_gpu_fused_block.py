@@ -328,9 +328,13 @@ def test_linear_without_rows_or_features(fused):
             dx, dw, db = torch.autograd.grad(y, [x, w, b], torch.empty_like(y))
             assert dx.shape == (0, 24) and not dw.any() and not db.any()
             # no input features: the bias is all there is
-            x0, w0 = torch.empty(5, 0, dtype=dtype, device="cuda"), torch.empty(40, 0, dtype=dtype, device="cuda")
-            y = fused.linear(x0, w0, b.detach(), "none")
-            assert torch.equal(y, b.detach().expand(5, 40))
+            for rows in (5, 300):
+                x0 = torch.empty(rows, 0, dtype=dtype, device="cuda", requires_grad=True)
+                w0 = torch.empty(40, 0, dtype=dtype, device="cuda", requires_grad=True)
+                y = fused.linear(x0, w0, b, "none")
+                assert torch.equal(y, b.detach().expand(rows, 40))
+                dx, dw, db = torch.autograd.grad(y, [x0, w0, b], torch.ones_like(y))
+                assert dx.shape == (rows, 0) and dw.shape == (40, 0) and (db == rows).all()
 
 
 def test_linear_keeps_bad_rows_to_themselves(fused):
@@ -554,6 +558,11 @@ def test_refusals(fused):
     d, = torch.autograd.grad(fused.layer_norm(leaf, 32).square().sum(), leaf, create_graph=True)
     with pytest.raises(RuntimeError):
         d.sum().backward()
+    leaf, lw = x.clone().requires_grad_(), w.clone().requires_grad_()
+    d, dw = torch.autograd.grad(fused.linear(leaf, lw, b, "silu", res).square().sum(), [leaf, lw], create_graph=True)
+    for g in (d, dw):
+        with pytest.raises(RuntimeError):
+            g.sum().backward(retain_graph=True)
 
 
 # ------------------------------------------------------------------------------------------- modules and simulation
