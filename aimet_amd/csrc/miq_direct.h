@@ -123,7 +123,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void direct_kernel(const DirectProd
         lb.p += (int64_t) first * lb.step;
         int64_t left     = p.k - (int64_t) first * kDeep;
         const auto issue = [&](int buffer) {
-            char* to = lds + buffer * (LA::kBytes + LB::kBytes);
+            const uint32_t to = lds_address(lds) + (uint32_t) buffer * (LA::kBytes + LB::kBytes);
             la.load(p.a, m0, to, wave, lane, left);
             lb.load(p.b, n0, to + LA::kBytes, wave, lane, left);
             left -= kDeep;

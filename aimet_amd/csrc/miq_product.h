@@ -126,13 +126,13 @@ struct Loader
         edge   = first + COUNT > o.count;
     }
 
-    // Starts load i of a slice with `left` values of k remaining (from its first) into `lds`.  INSIDE: all of the slice is
+    // Starts load i of a slice with `left` values of k remaining (from its first) into `lds` (an address in LDS).  INSIDE: all of the slice is
     // inside of the operand; otherwise what is not is read as zeros.
     template <bool INSIDE>
-    __device__ __forceinline__ void load_one(int i, const Operand<E>& o, int64_t first, char* lds, int wave, int lane,
+    __device__ __forceinline__ void load_one(int i, const Operand<E>& o, int64_t first, uint32_t lds, int wave, int lane,
                                              int64_t left)
     {
-        const uint32_t to = __builtin_amdgcn_readfirstlane(lds_address(lds + (i * WAVES + wave) * 1024));
+        const uint32_t to = __builtin_amdgcn_readfirstlane(lds + (i * WAVES + wave) * 1024);
         if (INSIDE)
             asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to),
                          "v"(offset_of(i, wave, lane)), "s"(p + i * apart)
@@ -148,7 +148,8 @@ struct Loader
                          : "memory");
         }
     }
-    __device__ __forceinline__ void load(const Operand<E>& o, int64_t first, char* lds, int wave, int lane, int64_t left)
+    __device__ __forceinline__ void load(const Operand<E>& o, int64_t first, uint32_t lds, int wave, int lane,
+                                         int64_t left)
     {
         const bool inside = !edge && left >= kDeep;
 #pragma unroll
@@ -480,9 +481,10 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(const Product<T> p
     // is fixed step by step: left to itself the compiler starts all loads first and waits for all reads at once.
     constexpr int kReads = (FM + FN + FM - FM / 4 - 1) / (FM - FM / 4), kAll = LA::kLoads + LB::kLoads,
                   kStarts = (kAll + FM - 1) / FM;
+    const uint32_t lds0 = lds_address(lds);
     Fragments f0, f1;
     const auto half_slice = [&](auto multiplies, const Fragments& f, auto reads, Fragments& next, const char* from, int half,
-                                auto starts, auto inside, char* to) {
+                                auto starts, auto inside, uint32_t to) {
 #pragma unroll
         for (int i = 0; i < FM; ++i)
         {
@@ -518,26 +520,27 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(const Product<T> p
         constexpr auto yes = std::true_type();
         constexpr auto no  = std::false_type();
         const auto buffer  = [&](int s) { return lds + (s & 1) * (LA::kBytes + LB::kBytes); };
-        half_slice(no, f0, no, f0, nullptr, 0, yes, inside, buffer(0));
+        const auto place   = [&](int s) { return lds0 + (uint32_t) (s & 1) * (LA::kBytes + LB::kBytes); };
+        half_slice(no, f0, no, f0, nullptr, 0, yes, inside, place(0));
         arrived();
         if (count > 1)
-            half_slice(no, f0, yes, f0, buffer(0), 0, yes, inside, buffer(1));
+            half_slice(no, f0, yes, f0, buffer(0), 0, yes, inside, place(1));
         else
-            half_slice(no, f0, yes, f0, buffer(0), 0, no, inside, nullptr);
-        half_slice(yes, f0, yes, f1, buffer(0), 1, no, inside, nullptr);
+            half_slice(no, f0, yes, f0, buffer(0), 0, no, inside, 0u);
+        half_slice(yes, f0, yes, f1, buffer(0), 1, no, inside, 0u);
         for (int s = 1; s + 1 < count; ++s)
         {
             arrived();   // slice s has arrived, and everybody has read slice s - 1
-            half_slice(yes, f1, yes, f0, buffer(s), 0, yes, inside, buffer(s + 1));
-            half_slice(yes, f0, yes, f1, buffer(s), 1, no, inside, nullptr);
+            half_slice(yes, f1, yes, f0, buffer(s), 0, yes, inside, place(s + 1));
+            half_slice(yes, f0, yes, f1, buffer(s), 1, no, inside, 0u);
         }
         if (count > 1)
         {
             arrived();
-            half_slice(yes, f1, yes, f0, buffer(count - 1), 0, no, inside, nullptr);
-            half_slice(yes, f0, yes, f1, buffer(count - 1), 1, no, inside, nullptr);
+            half_slice(yes, f1, yes, f0, buffer(count - 1), 0, no, inside, 0u);
+            half_slice(yes, f0, yes, f1, buffer(count - 1), 1, no, inside, 0u);
         }
-        half_slice(yes, f1, no, f1, nullptr, 0, no, inside, nullptr);
+        half_slice(yes, f1, no, f1, nullptr, 0, no, inside, 0u);
     };
     const bool inside = !la.edge && !lb.edge && p.k % kSlice == 0;
     for (int pass = 0; pass < (kF32 ? 2 : 1) && first < last; ++pass)
