@@ -4,6 +4,7 @@
 //   dz = g act'(z), dx = dz w, dw = dz^T x, db = sum over rows of dz, dresidual = g
 #include "miq_direct.h"
 #include "miq_few_rows.h"
+#include "miq_halves.h"
 
 #include <algorithm>
 
@@ -56,7 +57,8 @@ __device__ __forceinline__ void put_parts(const float* v, int shift, uint16_t* c
     *(uint4*) coarse = make_uint4(c[0] | c[1] << 16, c[2] | c[3] << 16, c[4] | c[5] << 16, c[6] | c[7] << 16);
     *(uint4*) fine   = make_uint4(f[0] | f[1] << 16, f[2] | f[3] << 16, f[4] | f[5] << 16, f[6] | f[7] << 16);
 }
-// out[r][0 .. kp) = src[r][0 .. k), zeros behind; float32: out[r][0 .. kp) coarse, out[r][kp .. 2 kp) fine, scale[r] = -s.
+// out[r] = the halves of src[r][0 .. k), of zeros up to kp (a multiple of kHalves): for every kHalves values their coarse
+// halves and then their fine ones; scale[r] = -s.
 // LANES threads hold a row of up to 32 LANES values in registers between its largest value and its halves; of a longer
 // one what is past them is read again.
 template <int LANES>
@@ -107,12 +109,12 @@ __global__ __launch_bounds__(kBlock) void pack_rows_kernel(const float* __restri
     {
         const int64_t c = (i * LANES + lane) * 8;
         if (c < kp)
-            put_parts(v[i], shift, to + c, to + kp + c);
+            put_parts(v[i], shift, to + place_of_half(c), to + place_of_half(c) + kHalves);
     }
     for (int64_t c = (kHeld * LANES + lane) * 8; c < kp; c += LANES * 8)
     {
         load8(from + c, k - c, t);
-        put_parts(t, shift, to + c, to + kp + c);
+        put_parts(t, shift, to + place_of_half(c), to + place_of_half(c) + kHalves);
     }
     if (lane == 0)
         scale[r] = -shift;
@@ -221,8 +223,8 @@ __global__ __launch_bounds__(kBlock) void pack_columns_kernel(const float* __res
 #pragma unroll
         for (int u = 0; u < 8; ++u)
             v[u] = tile[c + u][r];
-        uint16_t* to = out + (r0 + r) * 2 * kp + k0 + c;
-        put_parts(v, shifts[r], to, to + kp);
+        uint16_t* to = out + (r0 + r) * 2 * kp + place_of_half(k0 + c);
+        put_parts(v, shifts[r], to, to + kHalves);
     }
 }
 
@@ -485,7 +487,7 @@ Plan plan_product(const Matrix<T>& a, const Matrix<T>& b)
     p.a_bytes = copied(a), p.b_bytes = copied(b);
     if (kF32)
     {
-        p.kp      = (k + kSlice - 1) / kSlice * kSlice;
+        p.kp      = (k + kHalves - 1) / kHalves * kHalves;
         p.a_bytes = up256(m * 2 * p.kp * 2), p.b_bytes = up256(n * 2 * p.kp * 2);
         p.scale_a = up256(m * 4 * (1 + (a.columns ? max_slices(k) : 0)));
         p.scale_b = up256(n * 4 * (1 + (b.columns ? max_slices(k) : 0)));
@@ -566,10 +568,21 @@ int launch_product(Product<T>& p, bool big, hipStream_t s)
     p.tiles_m = (int) ((p.e.m + tile - 1) / tile), p.tiles_n = (int) ((p.e.n + tile - 1) / tile);
     const int64_t blocks = (int64_t) p.tiles_m * p.tiles_n * p.splits;
     MIQ_CHECK_ARG(blocks <= INT32_MAX, "the product has too many tiles");
-    if (big)
-        hipLaunchKernelGGL((product_kernel<T, ACT, 2, 4, 8, 4, AC, BC>), dim3((unsigned) blocks), dim3(512), 0, s, p);
+    const dim3 grid((unsigned) blocks), threads(big ? 512 : 256);
+    if constexpr (std::is_same<T, float>::value)
+    {
+        if (big)
+            hipLaunchKernelGGL((halves_kernel<ACT, 2, 4, 8, 4>), grid, threads, 0, s, p);
+        else
+            hipLaunchKernelGGL((halves_kernel<ACT, 2, 2, 4, 4>), grid, threads, 0, s, p);
+    }
     else
-        hipLaunchKernelGGL((product_kernel<T, ACT, 2, 2, 4, 4, AC, BC>), dim3((unsigned) blocks), dim3(256), 0, s, p);
+    {
+        if (big)
+            hipLaunchKernelGGL((product_kernel<ACT, 2, 4, 8, 4, AC, BC>), grid, threads, 0, s, p);
+        else
+            hipLaunchKernelGGL((product_kernel<ACT, 2, 2, 4, 4, AC, BC>), grid, threads, 0, s, p);
+    }
     MIQ_CHECK_LAUNCH();
     return launch_join<T, ACT>(p.partial, p.splits, p.e, s);
 }

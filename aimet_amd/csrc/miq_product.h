@@ -390,7 +390,7 @@ template <typename T>
 struct Product
 {
     Operand<uint16_t> a, b;
-    int64_t k;             // length of the sum (float32: padded to whole slices)
+    int64_t k;             // length of the sum (float32: padded to whole slices of kHalves)
     int tiles_m, tiles_n;
     int splits;            // the sum over k is cut into this many pieces, whose results go to `partial`
     float* partial;        // [splits][m][n]
@@ -413,15 +413,32 @@ __device__ __forceinline__ void tile_of_block(int block, int blocks, int tiles_m
     *tn = t / height;
 }
 
-template <typename T, int ACT, int WM, int WN, int FM, int FN, bool AC, bool BC>
-__global__ __launch_bounds__(WM* WN * 64) void product_kernel(const Product<T> p)
+// Whether a tile reaches past the end of a matrix
+template <typename T>
+__device__ __forceinline__ bool la_edge(const Product<T>& p, int64_t m0, int64_t n0, int tm, int tn)
 {
-    constexpr bool kF32  = std::is_same<T, float>::value;
+    return m0 + tm > p.a.count || n0 + tn > p.b.count;
+}
+
+// 8 values of row r from column q on: finished, or kept as a piece of a sum
+template <typename T, int ACT>
+__device__ __forceinline__ void finish_or_keep(const Product<T>& p, int split, int64_t r, int64_t q, float* z)
+{
+    if (p.splits == 1)
+        finish8<T, ACT>(p.e, r, q, z);
+    else
+        store8(p.partial + ((int64_t) split * p.e.m + r) * p.e.n + q, p.e.n - q, z);
+}
+
+// bfloat16
+template <int ACT, int WM, int WN, int FM, int FN, bool AC, bool BC>
+__global__ __launch_bounds__(WM* WN * 64) void product_kernel(const Product<uint16_t> p)
+{
+    using T              = uint16_t;
     constexpr int kWaves = WM * WN, kTM = WM * FM * 16, kTN = WN * FN * 16;
     constexpr int kKeyA = AC ? 2 : 0, kKeyB = BC ? 3 : 1;
     using LA             = Loader<uint16_t, kTM, kWaves, AC, kKeyA>;
     using LB             = Loader<uint16_t, kTN, kWaves, BC, kKeyB>;
-    using Kind           = std::integral_constant<bool, !kF32>;
     __shared__ __attribute__((aligned(1024))) char lds[2 * (LA::kBytes + LB::kBytes)];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -440,23 +457,12 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(const Product<T> p
     la.start(p.a, m0, wave, lane);
     lb.start(p.b, n0, wave, lane);
     la.p += (int64_t) first * la.step;
-    lb.p += (int64_t) first * lb.step + (kF32 ? p.k : 0);
-    int64_t left = p.k - (int64_t) first * kSlice;
-    int issued   = 0;
-    // After a slice's loads: on to the next one.  float32: three times over k, A's coarse halves with B's fine ones, fine
-    // with coarse, coarse with coarse.
-    const auto advance = [&] {
+    lb.p += (int64_t) first * lb.step;
+    int64_t left       = p.k - (int64_t) first * kSlice;
+    const auto advance = [&] {   // after a slice's loads: on to the next one
         la.p += la.step;
         lb.p += lb.step;
         left -= kSlice;
-        ++issued;
-        if (kF32 && (issued == last - first || issued == 2 * (last - first)))
-        {
-            const int64_t back = (int64_t) (last - first) * kSlice;
-            left += back;
-            la.p += (issued == last - first ? p.k : -p.k) - back;
-            lb.p += (issued == last - first ? -p.k : 0) - back;
-        }
     };
 
     f4 acc[FM][FN];
@@ -501,7 +507,7 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(const Product<T> p
             if constexpr (decltype(multiplies)::value)
 #pragma unroll
                 for (int j = 0; j < FN; ++j)
-                    acc[i][j] = mfma_16x16x32(f.b[j], f.a[i], acc[i][j], Kind());
+                    acc[i][j] = mfma_16x16x32(f.b[j], f.a[i], acc[i][j], std::true_type());
             if constexpr (decltype(reads)::value)
 #pragma unroll
                 for (int u = i * kReads; u < (i + 1) * kReads && u < FM + FN; ++u)
@@ -516,7 +522,8 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(const Product<T> p
         if constexpr (decltype(starts)::value)
             advance();
     };
-    const auto sum = [&](int count, auto inside) {
+    const int count = last - first;
+    const auto sum  = [&](auto inside) {
         constexpr auto yes = std::true_type();
         constexpr auto no  = std::false_type();
         const auto buffer  = [&](int s) { return lds + (s & 1) * (LA::kBytes + LB::kBytes); };
@@ -542,28 +549,12 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(const Product<T> p
         }
         half_slice(yes, f1, no, f1, nullptr, 0, no, inside, 0u);
     };
-    const bool inside = !la.edge && !lb.edge && p.k % kSlice == 0;
-    for (int pass = 0; pass < (kF32 ? 2 : 1) && first < last; ++pass)
+    if (count > 0)
     {
-        // float32: the corrections, then the coarse halves
-        const int count = (last - first) * (kF32 && pass == 0 ? 2 : 1);
-        if (inside)
-            sum(count, std::true_type());
+        if (!la_edge(p, m0, n0, kTM, kTN) && p.k % kSlice == 0)
+            sum(std::true_type());
         else
-            sum(count, std::false_type());
-        if (kF32 && pass == 0)
-        {
-            // Corrections are finite for finite operands: where an infinity or a NaN made them anything else, the coarse
-            // halves alone say what comes out.
-#pragma unroll
-            for (int i = 0; i < FM; ++i)
-#pragma unroll
-                for (int j = 0; j < FN; ++j)
-#pragma unroll
-                    for (int u = 0; u < 4; ++u)
-                        acc[i][j][u] = __builtin_isfinite(acc[i][j][u]) ? acc[i][j][u] : 0.f;
-            arrived();   // everybody has read the last slice
-        }
+            sum(std::false_type());
     }
 
 #pragma unroll
@@ -572,7 +563,6 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(const Product<T> p
         const int64_t r = m0 + wm * FM * 16 + i * 16 + lane % 16;
         if (r >= p.e.m)
             continue;
-        const int sr = kF32 ? p.scale_a[r] : 0;
 #pragma unroll
         for (int j = 0; j < FN; j += 2)
         {
@@ -582,15 +572,8 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(const Product<T> p
             float z[8];
 #pragma unroll
             for (int u = 0; u < 8; ++u)
-            {
                 z[u] = acc[i][j + u / 4][u % 4];
-                if (kF32)
-                    z[u] = ldexpf(z[u], sr + (q + u < p.e.n ? p.scale_b[q + u] : 0));
-            }
-            if (p.splits == 1)
-                finish8<T, ACT>(p.e, r, q, z);
-            else
-                store8(p.partial + ((int64_t) split * p.e.m + r) * p.e.n + q, p.e.n - q, z);
+            finish_or_keep<T, ACT>(p, split, r, q, z);
         }
     }
 }
