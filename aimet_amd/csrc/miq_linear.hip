@@ -377,19 +377,20 @@ int64_t max_slices(int64_t k)
     return std::max<int64_t>(1, std::min<int64_t>(32, k / 16));
 }
 
-// Whether a float32 product is formed from its operands as they lie (miq_direct.h) or from halves made beforehand.
-// Measured: the first runs at about 160 TFLOP/s, the second at up to 380 once the halves are there; making them takes
-// 3 ps a value of an operand in rows and 5 ps in columns (one more pass), and 22 us of launches, 20 more for each operand in
-// columns.  In us, as they lie and by halves: [512, 4096] x [4096, 4096]^T 106 and 122, [1024, 4096] x [4096, 4096]^T 189 and
-// 162; the input's gradient of [512, 4096] x [11008, 4096]^T 246 and 349, of [1024, ...] 476 and 460; the weight's
-// gradient of [256, 4096] x [11008, 4096]^T 150 and 194, of [512, ...] 266 and 256.
+// Whether a float32 product is formed from its operands as they lie (miq_direct.h) or from halves made beforehand
+// (miq_halves.h).  The first runs at about 160 TFLOP/s, the second at up to 490 once the halves are there; making them takes
+// 2 ps a value of an operand in rows and 3 ps in columns (one more pass), and 10 us of launches, 15 more for each operand
+// in columns.  The rule is within 5 % of the better way on 48 measured products.  In us, as they lie and by halves:
+// [256, 4096] x [4096, 4096]^T 62 and 71, [512, 4096] x [4096, 4096]^T 106 and 93, the input's gradient of
+// [512, 4096] x [11008, 4096]^T 246 and 263, of [768, 4096] x [4096, 4096]^T 172 and 141, the weight's gradient of
+// [512, 4096] x [4096, 4096]^T 102 and 91.
 template <typename T>
 bool direct_pays(const Matrix<T>& a, const Matrix<T>& b)
 {
     const auto halves = [](const Matrix<T>& x) {
-        return (double) x.count * x.k * (x.columns ? 5e-12 : 3e-12) + (x.columns ? 20e-6 : 0);
+        return (double) x.count * x.k * (x.columns ? 3e-12 : 2e-12) + (x.columns ? 15e-6 : 0);
     };
-    return 3.5e-15 * 2.0 * a.count * b.count * a.k <= 22e-6 + halves(a) + halves(b);
+    return 3.5e-15 * 2.0 * a.count * b.count * a.k <= 10e-6 + halves(a) + halves(b);
 }
 
 enum class Way
