@@ -7,21 +7,6 @@
 
 namespace miq
 {
-// One value of the result: bias, activation, residual, and z for the backward pass
-template <typename T, int ACT>
-__device__ __forceinline__ void finish1(const Epilogue<T>& e, int64_t r, int64_t q, float z)
-{
-    const int64_t at = r * e.n + q;
-    if (e.bias)
-        z += value_at(e.bias + q);
-    if (e.saved)
-        put_at(e.saved + at, z);
-    z = act_value<ACT>(z);
-    if (e.residual)
-        z += value_at(e.residual + at);
-    put_at(e.c + at, z);
-}
-
 __device__ __forceinline__ void load4(const float* p, float* v)
 {
     load_any(p, v);

@@ -165,15 +165,55 @@ __global__ __launch_bounds__(WM* WN * 64) void halves_kernel(const Product<float
     }
 
     // Corrections are finite for finite operands.  Where an infinity or a NaN made a sum anything else, the coarse halves
-    // alone say what comes out: the corrections are formed apart, cleared where they are not finite, and the rest added.
-    bool finite = true;
+    // alone say what comes out: those sums are formed once more, corrections first, cleared where they are not finite, and
+    // the rest added.  The others are stored as they are.
+    uint32_t bad[FM * FN / 8] = {};
+    bool finite               = true;
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
         for (int j = 0; j < FN; ++j)
 #pragma unroll
             for (int u = 0; u < 4; ++u)
-                finite = finite && __builtin_isfinite(acc[i][j][u]);
+                if (!__builtin_isfinite(acc[i][j][u]))
+                {
+                    bad[(i * FN + j) / 8] |= 1u << ((i * FN + j) % 8 * 4 + u);
+                    finite = false;
+                }
+    const auto store = [&](auto again) {
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+        {
+            const int64_t r = m0 + wm * FM * 16 + i * 16 + lane % 16;
+            if (r >= p.e.m)
+                continue;
+            const int sr = p.scale_a[r];
+#pragma unroll
+            for (int j = 0; j < FN; j += 2)
+            {
+                const int64_t q = n0 + wn * FN * 16 + 16 * j + 8 * (lane / 16);
+                if (q >= p.e.n)
+                    continue;
+                float z[8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u)
+                    z[u] = ldexpf(acc[i][j + u / 4][u % 4], sr + (q + u < p.e.n ? p.scale_b[q + u] : 0));
+                if constexpr (!decltype(again)::value)
+                    finish_or_keep<float, ACT>(p, split, r, q, z);
+                else
+#pragma unroll
+                    for (int u = 0; u < 8; ++u)
+                        if ((bad[(i * FN + j) / 8] >> ((i * FN + j) % 8 * 4 + u) & 1) && q + u < p.e.n)
+                        {
+                            if (p.splits == 1)
+                                finish1<float, ACT>(p.e, r, q + u, z[u]);
+                            else
+                                p.partial[((int64_t) split * p.e.m + r) * p.e.n + q + u] = z[u];
+                        }
+            }
+        }
+    };
+    store(std::false_type());
     if (__syncthreads_or(!finite))
     {
 #pragma unroll
@@ -217,27 +257,7 @@ __global__ __launch_bounds__(WM* WN * 64) void halves_kernel(const Product<float
                         for (int u = 0; u < 4; ++u)
                             acc[i][j][u] = __builtin_isfinite(acc[i][j][u]) ? acc[i][j][u] : 0.f;
         }
-    }
-
-#pragma unroll
-    for (int i = 0; i < FM; ++i)
-    {
-        const int64_t r = m0 + wm * FM * 16 + i * 16 + lane % 16;
-        if (r >= p.e.m)
-            continue;
-        const int sr = p.scale_a[r];
-#pragma unroll
-        for (int j = 0; j < FN; j += 2)
-        {
-            const int64_t q = n0 + wn * FN * 16 + 16 * j + 8 * (lane / 16);
-            if (q >= p.e.n)
-                continue;
-            float z[8];
-#pragma unroll
-            for (int u = 0; u < 8; ++u)
-                z[u] = ldexpf(acc[i][j + u / 4][u % 4], sr + (q + u < p.e.n ? p.scale_b[q + u] : 0));
-            finish_or_keep<float, ACT>(p, split, r, q, z);
-        }
+        store(std::true_type());
     }
 }
 }   // namespace miq

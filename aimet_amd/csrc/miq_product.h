@@ -344,6 +344,21 @@ __device__ __forceinline__ void finish8(const Epilogue<T>& e, int64_t r, int64_t
     store8(e.c + at, left, z);
 }
 
+// One value of the result: bias, activation, residual, and z for the backward pass
+template <typename T, int ACT>
+__device__ __forceinline__ void finish1(const Epilogue<T>& e, int64_t r, int64_t q, float z)
+{
+    const int64_t at = r * e.n + q;
+    if (e.bias)
+        z += value_at(e.bias + q);
+    if (e.saved)
+        put_at(e.saved + at, z);
+    z = act_value<ACT>(z);
+    if (e.residual)
+        z += value_at(e.residual + at);
+    put_at(e.c + at, z);
+}
+
 // the same for 4 values of a float32 matrix
 __device__ __forceinline__ void load4(const float* p, int64_t left, float* v)
 {
