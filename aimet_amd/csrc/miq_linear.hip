@@ -378,19 +378,21 @@ int64_t max_slices(int64_t k)
 }
 
 // Whether a float32 product is formed from its operands as they lie (miq_direct.h) or from halves made beforehand
-// (miq_halves.h).  The first runs at about 160 TFLOP/s, the second at up to 490 once the halves are there; making them takes
-// 2 ps a value of an operand in rows and 3 ps in columns (one more pass), and 10 us of launches, 15 more for each operand
-// in columns.  The rule is within 5 % of the better way on 48 measured products.  In us, as they lie and by halves:
+// (miq_halves.h).  The first runs at about 160 TFLOP/s (130 on columns, whole tiles counted), the second at up to 490 once the halves are there; making them takes
+// 2 ps a value of an operand in rows and 3 ps in columns (one more pass), and 18 us of launches, 15 more for each operand
+// in columns.  The rule is within 5 % of the better way on most of 90 measured products.  In us, as they lie and by halves:
 // [256, 4096] x [4096, 4096]^T 62 and 71, [512, 4096] x [4096, 4096]^T 106 and 93, the input's gradient of
 // [512, 4096] x [11008, 4096]^T 246 and 263, of [768, 4096] x [4096, 4096]^T 172 and 141, the weight's gradient of
 // [512, 4096] x [4096, 4096]^T 102 and 91.
 template <typename T>
 bool direct_pays(const Matrix<T>& a, const Matrix<T>& b)
 {
-    const auto halves = [](const Matrix<T>& x) {
-        return (double) x.count * x.k * (x.columns ? 3e-12 : 2e-12) + (x.columns ? 15e-6 : 0);
+    const auto halves = [](const Matrix<T>& x, double columns) {
+        return (double) x.count * x.k * (x.columns ? columns : 2e-12) + (x.columns ? 15e-6 : 0);
     };
-    return 3.5e-15 * 2.0 * a.count * b.count * a.k <= 10e-6 + halves(a) + halves(b);
+    const auto tiles = [](int64_t n) { return (double) ((n + 127) / 128 * 128); };
+    return (a.columns ? 4.2e-15 : 3.5e-15) * 2.0 * tiles(a.count) * tiles(b.count) * a.k <=
+           18e-6 + halves(a, 2.5e-12) + halves(b, 3e-12);
 }
 
 enum class Way
@@ -411,13 +413,14 @@ struct Plan
     int64_t a_bytes, b_bytes, scale_a, scale_b, partial, total;   // of the workspace
 };
 
-// Tiles and pieces of the sum for a product of `slices` slices a pass.  What a launch costs, in us, as measured on many
-// shapes (within 10 % for most): 5, and for each round of tiles that the device holds at a time and each slice of theirs
-//   256 x 256, one a CU: 1.5, 1.25 when half of the CUs have none    128 x 128, two a CU: 1.05, 0.6 when there is one
-// and to join the pieces 4 and 1 for each million of partial values.  E.g. [4096, 1024] x [1024, 1024]^T: 15 whole, 26 in two
-// pieces; [512, 4096] x [4096, 4096]^T: 42, 32 and 32 in two and four; [2048, 11008] x [4096, 11008]^T: 191 in 128 x 128
-// tiles, 165 in 256 x 256 in two pieces.
-void choose_tiles(int64_t m, int64_t n, int64_t slices, int passes, Plan* p)
+// Tiles and pieces of the sum for a product of `slices` slices a pass whose values take `bytes`.  What a launch costs, in
+// us, as measured on many shapes (within 10 % for most): 5, and for each round of tiles that the device holds at a time
+//   256 x 256, one a CU: 1.5 a slice, 1.25 when half of the CUs have none, and the result at 20 bytes a ns and CU
+//   128 x 128, two a CU: 1.05 a slice, 0.6 when there is one, and half of that, for one writes while the other sums
+// and to join the pieces 4 and 1 for each million of partial values.  E.g. bfloat16 [4096, 1024] x [1024, 1024]^T: 15 whole,
+// 26 in two pieces; [512, 4096] x [4096, 4096]^T: 42, 32 and 32 in two and four; [2048, 11008] x [4096, 11008]^T: 191 in
+// 128 x 128 tiles, 165 in 256 x 256 in two pieces.
+void choose_tiles(int64_t m, int64_t n, int64_t slices, int passes, int bytes, Plan* p)
 {
     double best = 1e30;
     for (const bool big : {false, true})
@@ -428,7 +431,8 @@ void choose_tiles(int64_t m, int64_t n, int64_t slices, int passes, Plan* p)
             const int64_t blocks = tiles * splits, at_once = big ? 256 : 512, rounds = (blocks + at_once - 1) / at_once;
             const bool sparse    = rounds == 1 && blocks <= at_once / 2;
             const double slice   = big ? (sparse ? 1.25 : 1.5) : (sparse ? 0.6 : 1.05);
-            const double cost    = 5 + (double) rounds * ((slices + splits - 1) / splits) * passes * slice +
+            const double write   = (big ? 1.0 : 0.25) * 256 * 256 * bytes / 20e3;
+            const double cost    = 5 + (double) rounds * (((slices + splits - 1) / splits) * passes * slice + write) +
                                 (splits > 1 ? 4 + 1e-6 * splits * m * n : 0);
             if (cost < best)
             {
@@ -484,7 +488,7 @@ Plan plan_product(const Matrix<T>& a, const Matrix<T>& b)
         return done();
     }
     p.way = Way::kTiles;
-    choose_tiles(m, n, (k + kSlice - 1) / kSlice, kF32 ? 3 : 1, &p);
+    choose_tiles(m, n, (k + kSlice - 1) / kSlice, kF32 ? 3 : 1, (int) sizeof(T), &p);
     p.a_bytes = copied(a), p.b_bytes = copied(b);
     if (kF32)
     {
