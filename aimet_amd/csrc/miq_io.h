@@ -131,7 +131,8 @@ __device__ __forceinline__ void store_any(float* p, const float* f)
 }
 __device__ __forceinline__ void store_any(uint16_t* p, const float* f)
 {
-    const uint4 w  = IOTraits<uint16_t>::pack(f);
+    // (the hardware's conversion: a NaN stays one, with what payload does not matter here)
+    const uint4 w  = IOTraits<uint16_t>::pack_no_nan(f);
     const any_u4 v = {w.x, w.y, w.z, w.w};
     *(any_u4*) p   = v;
 }

@@ -144,7 +144,8 @@ __global__ __launch_bounds__(LANES < kBlock ? kBlock : LANES) void ln_fwd_kernel
     const int64_t row = (int64_t) blockIdx.x * kRows + threadIdx.x / LANES;
     if (row >= rows)
         return;   // (a whole wave: with one row a block there are as many blocks as rows)
-    const T* px = x + row * width;
+    const T* px      = x + row * width;
+    const bool whole = width % VEC == 0;   // the same for all: no piece starts earlier
     float v[PER][VEC], s = 0.f;
 #pragma unroll
     for (int i = 0; i < PER; ++i)
@@ -160,9 +161,14 @@ __global__ __launch_bounds__(LANES < kBlock ? kBlock : LANES) void ln_fwd_kernel
     for (int i = 0; i < PER; ++i)
     {
         const Piece<VEC> piece((i * LANES + lane) * VEC, width);
+        if (whole)
 #pragma unroll
-        for (int u = 0; u < VEC; ++u)
-            s += u < piece.twice ? 0.f : v[i][u];
+            for (int u = 0; u < VEC; ++u)
+                s += v[i][u];
+        else
+#pragma unroll
+            for (int u = 0; u < VEC; ++u)
+                s += u < piece.twice ? 0.f : v[i][u];
     }
     const float m = lanes_sum<LANES>(s, lds) / (float) width;
     float q       = 0.f;
@@ -170,13 +176,22 @@ __global__ __launch_bounds__(LANES < kBlock ? kBlock : LANES) void ln_fwd_kernel
     for (int i = 0; i < PER; ++i)
     {
         const Piece<VEC> piece((i * LANES + lane) * VEC, width);
+        if (!piece.has)
+            continue;
+        if (whole)
 #pragma unroll
-        for (int u = 0; u < VEC; ++u)
-        {
-            v[i][u] -= m;
-            const bool counts = piece.has && u >= piece.twice && (width >= VEC || u < width);
-            q                 = counts ? fmaf(v[i][u], v[i][u], q) : q;
-        }
+            for (int u = 0; u < VEC; ++u)
+            {
+                v[i][u] -= m;
+                q = fmaf(v[i][u], v[i][u], q);
+            }
+        else
+#pragma unroll
+            for (int u = 0; u < VEC; ++u)
+            {
+                v[i][u] -= m;
+                q = u >= piece.twice && (width >= VEC || u < width) ? fmaf(v[i][u], v[i][u], q) : q;
+            }
     }
     const float r = 1.0f / sqrtf(lanes_sum<LANES>(q, lds) / (float) width + eps);
 #pragma unroll
