@@ -1,5 +1,7 @@
 // Products with few rows on the left (single tokens, small batches): the weight is read once, from memory to registers,
-// and nothing else takes time.
+// and nothing else takes time.  [1, 4096] x [11008, 4096]^T bfloat16: 18.3 us (4.9 TB/s); [16, 4096] x [4096, 4096]^T
+// float32: 18 us (3.8 TB/s), its input's gradient 20.  The 128 x 128 tiles take 21.6 us for the first and, with the halves
+// they need, 82 for the second.  From 17 rows on the tiles (bfloat16) and the direct products (float32) are faster.
 #ifndef MIQ_FEW_ROWS_H
 #define MIQ_FEW_ROWS_H
 
@@ -71,160 +73,106 @@ struct Chunk<float>
     }
 };
 
-// C[m, n] = act(sum over k of a[m][k] b[n][k] + bias) + residual for m <= 16 MT rows.
-// A block makes 16 NT columns; its waves share the sum over k and add their parts through LDS, in order.  A wave takes
+// C[m, n] = act(sum over k of a[m][k] b[n][k] + bias) + residual for up to 16 rows of a.
+// A block makes 16 columns; its waves share the sum over k and add their parts through LDS, in order.  A wave takes
 // 16 rows of b at a time, 64 bytes of each: lane l row l % 16, bytes from 16 (l / 16).  Rows of a and b past the end
 // are the last one again: what they make is not stored.
-template <typename T, int ACT, int MT, int NT>
-__global__ __launch_bounds__(MT == 1 ? 1024 : 512) void few_rows_kernel(const T* __restrict__ a, const T* __restrict__ b, int64_t k,
+template <typename T, int ACT>
+__global__ __launch_bounds__(1024) void few_rows_kernel(const T* __restrict__ a, const T* __restrict__ b, int64_t k,
                                                         const Epilogue<T> e)
 {
-    using C              = Chunk<T>;
-    constexpr int kStep  = 4 * C::VEC, kUnroll = MT * NT >= 4 ? 4 : 8;
-    extern __shared__ f4 parts[];   // [waves][MT NT][64]
+    using C             = Chunk<T>;
+    constexpr int kStep = 4 * C::VEC, kUnroll = 8;
+    extern __shared__ f4 parts[];   // [waves][64]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6),
               waves = blockDim.x >> 6;
-    const int64_t n0 = (int64_t) blockIdx.x * (16 * NT);
+    const int64_t n0    = (int64_t) blockIdx.x * 16;
     const int64_t whole = k / kStep, first = whole * wave / waves, last = whole * (wave + 1) / waves;
-    const int in = lane / 16 * C::VEC;
-    const T* pb[NT];
-    const T* pa[MT];
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-    {
-        const int64_t n = n0 + j * 16 + lane % 16;
-        pb[j]           = b + (n < e.n ? n : e.n - 1) * k + first * kStep + in;   // past the end: the last row, not stored
-    }
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-    {
-        const int64_t m = i * 16 + lane % 16;
-        pa[i]           = a + (m < e.m ? m : e.m - 1) * k + first * kStep + in;
-    }
-    f4 acc[MT][NT];
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-            acc[i][j] = f4{0.f, 0.f, 0.f, 0.f};
-    C fa[MT], fb[NT];
-    int64_t s = first;
+    const int in    = lane / 16 * C::VEC;
+    const int64_t n = n0 + lane % 16, m = lane % 16;
+    const T* pb     = b + (n < e.n ? n : e.n - 1) * k + first * kStep + in;
+    const T* pa     = a + (m < e.m ? m : e.m - 1) * k + first * kStep + in;
+    f4 acc          = f4{0.f, 0.f, 0.f, 0.f};
+    int64_t s       = first;
     for (; s + kUnroll <= last; s += kUnroll)
     {
-        C wide[kUnroll][NT], rows[kUnroll][MT];
+        C wide[kUnroll], rows[kUnroll];
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u)
-#pragma unroll
-            for (int j = 0; j < NT; ++j)
-                wide[u][j].load(pb[j] + u * kStep);
+            wide[u].load(pb + u * kStep);
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u)
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-                rows[u][i].load(pa[i] + u * kStep);
+            rows[u].load(pa + u * kStep);
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u)
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int j = 0; j < NT; ++j)
-                    acc[i][j] = C::mad(wide[u][j], rows[u][i], acc[i][j]);
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-            pb[j] += kUnroll * kStep;
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-            pa[i] += kUnroll * kStep;
+            acc = C::mad(wide[u], rows[u], acc);
+        pb += kUnroll * kStep;
+        pa += kUnroll * kStep;
     }
     const int64_t end = last + (wave == waves - 1 && whole * kStep < k ? 1 : 0);
     for (; s < end; ++s)
     {
         const int64_t left = k - s * kStep - in;
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
+        C fa, fb;
+        if (left >= C::VEC)
         {
-            if (left >= C::VEC)
-                fb[j].load(pb[j]);
-            else
-                fb[j].load_some(pb[j], left);
-            pb[j] += kStep;
+            fb.load(pb);
+            fa.load(pa);
         }
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
+        else
         {
-            if (left >= C::VEC)
-                fa[i].load(pa[i]);
-            else
-                fa[i].load_some(pa[i], left);
-            pa[i] += kStep;
+            fb.load_some(pb, left);
+            fa.load_some(pa, left);
         }
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int j = 0; j < NT; ++j)
-                acc[i][j] = C::mad(fb[j], fa[i], acc[i][j]);
+        pb += kStep;
+        pa += kStep;
+        acc = C::mad(fb, fa, acc);
     }
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-            parts[(wave * MT * NT + i * NT + j) * 64 + lane] = acc[i][j];
+    parts[threadIdx.x] = acc;
     __syncthreads();
-    for (int at = threadIdx.x; at < MT * NT * 64; at += blockDim.x)
-    {
-        f4 z = parts[at];
-        for (int w = 1; w < waves; ++w)
-            z += parts[w * MT * NT * 64 + at];
-        const int f = at / 64, l = at % 64;
-        const int64_t r = f / NT * 16 + l % 16, q = n0 + f % NT * 16 + l / 16 * 4;
-        if (r < e.m)
+    if (threadIdx.x >= 64)
+        return;
+    for (int w = 1; w < waves; ++w)
+        acc += parts[w * 64 + lane];
+    if (m < e.m)
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-                if (q + u < e.n)
-                    finish1<T, ACT>(e, r, q + u, z[u]);
-    }
+        for (int u = 0; u < 4; ++u)
+            if (n0 + lane / 16 * 4 + u < e.n)
+                finish1<T, ACT>(e, m, n0 + lane / 16 * 4 + u, acc[u]);
 }
 
-// C[m, n] or, for one of several pieces of k, partial[split][m][n] = sum over k of a[m][k] b[k][n], m <= 16 MT rows.
+// C[m, n] or, for one of several pieces of k, partial[split][m][n] = sum over k of a[m][k] b[k][n], up to 16 rows of a.
 // b is read as it lies: lane l takes 16 bytes, VEC columns from VEC (l % 16), of row 4 (l / 16) + t of 16 rows, t = 0 .. 3.
 // As float32 they are the first factor of v_mfma_f32_16x16x4: value u of all lanes makes columns VEC r + u, r = 0 .. 15,
 // so that a lane ends up with 4 VEC consecutive columns of one m.  A block makes 16 VEC columns; its waves share the sum.
-template <typename T, int MT>
+template <typename T>
 __global__ __launch_bounds__(512) void few_rows_columns_kernel(const T* __restrict__ a, int64_t lda,
-                                                               const T* __restrict__ b, int64_t k, int64_t per_split, float* __restrict__ partial,
-                                                               const Epilogue<T> e)
+                                                               const T* __restrict__ b, int64_t k, int64_t per_split,
+                                                               float* __restrict__ partial, const Epilogue<T> e)
 {
-    constexpr int VEC = IOTraits<T>::VEC, kUnroll = MT * VEC >= 16 ? 1 : 2;
-    extern __shared__ f4 parts[];   // [waves][MT VEC][64]
+    constexpr int VEC = IOTraits<T>::VEC, kUnroll = 2;
+    extern __shared__ f4 parts[];   // [waves][VEC][64]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6),
               waves = blockDim.x >> 6;
     const int64_t c    = ((int64_t) blockIdx.x * 16 + lane % 16) * VEC;
     const int64_t from = blockIdx.y * per_split, to = from + per_split < k ? from + per_split : k;
     const int64_t steps = to > from ? (to - from + 15) / 16 : 0;
     const int64_t first = steps * wave / waves, last = steps * (wave + 1) / waves;
-    const T* pa[MT];
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-    {
-        const int64_t m = i * 16 + lane % 16;
-        pa[i]           = a + (m < e.m ? m : e.m - 1) * lda;
-    }
+    const T* pa       = a + (lane % 16 < e.m ? lane % 16 : e.m - 1) * lda;
     const bool inside = c + VEC <= e.n;
-    f4 acc[MT][VEC];
+    f4 acc[VEC];
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int u = 0; u < VEC; ++u)
-            acc[i][u] = f4{0.f, 0.f, 0.f, 0.f};
+    for (int u = 0; u < VEC; ++u)
+        acc[u] = f4{0.f, 0.f, 0.f, 0.f};
     for (int64_t s = first; s < last; s += kUnroll)
     {
-        float w[kUnroll][4][VEC], x[kUnroll][MT][4];
+        float w[kUnroll][4][VEC], x[kUnroll][4];
 #pragma unroll
         for (int v = 0; v < kUnroll; ++v)
         {
-            const int64_t k0 = from + (s + v) * 16 + lane / 16 * 4;
+            const int64_t k0   = from + (s + v) * 16 + lane / 16 * 4;
             const int64_t left = s + v < last ? to - k0 : 0;
-            const bool whole = left >= 4;
+            const bool whole   = left >= 4;
 #pragma unroll
             for (int t = 0; t < 4; ++t)
                 if (whole && inside)
@@ -233,36 +181,30 @@ __global__ __launch_bounds__(512) void few_rows_columns_kernel(const T* __restri
 #pragma unroll
                     for (int u = 0; u < VEC; ++u)
                         w[v][t][u] = t < left && c + u < e.n ? value_at(b + (k0 + t) * e.n + c + u) : 0.f;
+            if (whole)
+                load4(pa + k0, x[v]);
+            else
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
-                if (whole)
-                    load4(pa[i] + k0, x[v][i]);
-                else
-#pragma unroll
-                    for (int t = 0; t < 4; ++t)
-                        x[v][i][t] = t < left ? value_at(pa[i] + k0 + t) : 0.f;
+                for (int t = 0; t < 4; ++t)
+                    x[v][t] = t < left ? value_at(pa + k0 + t) : 0.f;
         }
 #pragma unroll
         for (int v = 0; v < kUnroll; ++v)
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
-                for (int i = 0; i < MT; ++i)
-#pragma unroll
-                    for (int u = 0; u < VEC; ++u)
-                        acc[i][u] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[v][t][u], x[v][i][t], acc[i][u], 0, 0, 0);
+                for (int u = 0; u < VEC; ++u)
+                    acc[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[v][t][u], x[v][t], acc[u], 0, 0, 0);
     }
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int u = 0; u < VEC; ++u)
-            parts[((wave * MT + i) * VEC + u) * 64 + lane] = acc[i][u];
+    for (int u = 0; u < VEC; ++u)
+        parts[(wave * VEC + u) * 64 + lane] = acc[u];
     __syncthreads();
-    // a thread finishes 4 VEC values, VEC at a time: row r = 4 (l / 16) + v, values u of it
-    for (int at = threadIdx.x; at < MT * 64 * 4; at += blockDim.x)
+    // a thread finishes 4 VEC values, VEC at a time: row l % 16, value v of lane l
+    for (int at = threadIdx.x; at < 64 * 4; at += blockDim.x)
     {
-        const int v = at % 4, l = at / 4 % 64, i = at / 256;
-        const int64_t row = i * 16 + l % 16, q = ((int64_t) blockIdx.x * 16 + l / 16 * 4 + v) * VEC;
+        const int v = at % 4, l = at / 4;
+        const int64_t row = l % 16, q = ((int64_t) blockIdx.x * 16 + l / 16 * 4 + v) * VEC;
         if (row >= e.m)
             continue;
 #pragma unroll
@@ -270,7 +212,7 @@ __global__ __launch_bounds__(512) void few_rows_columns_kernel(const T* __restri
         {
             float z = 0.f;
             for (int w = 0; w < waves; ++w)
-                z += parts[((w * MT + i) * VEC + u) * 64 + l][v];
+                z += parts[(w * VEC + u) * 64 + l][v];
             if (q + u >= e.n)
                 continue;
             if (partial)
