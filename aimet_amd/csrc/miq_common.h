@@ -43,6 +43,14 @@ inline bool aligned16(const void* p)
     return (reinterpret_cast<uintptr_t>(p) & 15u) == 0;
 }
 
+// `blocks` blocks of `threads` as a grid: an axis holds fewer than 2^32 threads, so that more of them go into rows (the
+// last row may reach past the last block)
+inline dim3 grid_of(int64_t blocks, int threads)
+{
+    const int64_t most = UINT32_MAX / threads, rows = blocks > most ? (blocks + most - 1) / most : 1;
+    return dim3((unsigned) ((blocks + rows - 1) / rows), (unsigned) rows);
+}
+
 constexpr int kBlock  = 256;   // 4 wavefronts of 64 lanes
 constexpr int kUnroll = 2;     // 16-byte vectors in flight per lane (measured: 2 beats 4 and 8 for streaming)
 

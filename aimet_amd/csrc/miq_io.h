@@ -6,6 +6,12 @@
 
 namespace miq
 {
+// this block's index in a grid made by grid_of()
+__device__ __forceinline__ int64_t block_index()
+{
+    return (int64_t) blockIdx.y * gridDim.x + blockIdx.x;
+}
+
 // ------------------------------------------------------------------------------------------------ IO vector types
 // Streaming accesses are marked non-temporal: every byte is touched exactly once, and on this part that alone is
 // worth about 10 % of bandwidth for both the read-once inputs and the write-once outputs.

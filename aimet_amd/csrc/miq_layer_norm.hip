@@ -145,9 +145,9 @@ __global__ __launch_bounds__(LANES < kBlock ? kBlock : LANES) void ln_fwd_kernel
     constexpr int VEC = IOTraits<T>::VEC, kRows = LANES < kBlock ? kBlock / LANES : 1;
     __shared__ float lds[LANES / 64];
     const int lane    = threadIdx.x % LANES;
-    const int64_t row = (int64_t) blockIdx.x * kRows + threadIdx.x / LANES;
+    const int64_t row = block_index() * kRows + threadIdx.x / LANES;
     if (row >= rows)
-        return;   // (a whole wave: with one row a block there are as many blocks as rows)
+        return;   // a whole wave, or, with one row a block, the whole block
     const T* px      = x + row * width;
     const bool whole = width % VEC == 0;   // the same for all: no piece starts earlier
     float v[PER][VEC], s = 0.f;
@@ -229,13 +229,15 @@ __global__ __launch_bounds__(LANES < kBlock ? kBlock : LANES) void ln_fwd_kernel
 // Rows too long for registers: read three times, the second and third from the caches
 template <typename T>
 __global__ __launch_bounds__(1024) void ln_fwd_long_kernel(const T* __restrict__ x, const T* __restrict__ w,
-                                                           const T* __restrict__ b, int64_t width, float eps,
-                                                           T* __restrict__ y, float* __restrict__ mean,
+                                                           const T* __restrict__ b, int64_t rows, int64_t width,
+                                                           float eps, T* __restrict__ y, float* __restrict__ mean,
                                                            float* __restrict__ rstd)
 {
     using IO = IOTraits<T>;
     __shared__ float lds[1024 / 64];
-    const int64_t row = blockIdx.x;
+    const int64_t row = block_index();
+    if (row >= rows)
+        return;
     const T* px       = x + row * width;
     float s           = 0.f;
     for (int64_t c = threadIdx.x; c < width; c += 1024)
@@ -409,12 +411,14 @@ __global__ __launch_bounds__(LANES < kBlock ? kBlock : LANES) void ln_bwd_kernel
 template <typename T>
 __global__ __launch_bounds__(1024) void ln_dx_long_kernel(const T* __restrict__ x, const T* __restrict__ g,
                                                           const T* __restrict__ w, const float* __restrict__ mean,
-                                                          const float* __restrict__ rstd, int64_t width,
-                                                          T* __restrict__ dx)
+                                                          const float* __restrict__ rstd, int64_t rows,
+                                                          int64_t width, T* __restrict__ dx)
 {
     using IO = IOTraits<T>;
     __shared__ float2 lds[1024 / 64];
-    const int64_t row = blockIdx.x;
+    const int64_t row = block_index();
+    if (row >= rows)
+        return;
     const T* px       = x + row * width;
     const T* pg       = g + row * width;
     const float m = mean[row], r = rstd[row];
@@ -467,7 +471,7 @@ __global__ __launch_bounds__(1024) void ln_join_kernel(const float* __restrict__
                                                        int64_t width, T* __restrict__ dw, T* __restrict__ db)
 {
     __shared__ float lds[32][33];
-    const int64_t c = (int64_t) blockIdx.x * 32 + threadIdx.x % 32;
+    const int64_t first = ((int64_t) blockIdx.z * gridDim.x + blockIdx.x) * 32, c = first + threadIdx.x % 32;
     const int part  = threadIdx.x / 32;
     T* out          = blockIdx.y == 0 ? dw : db;
     if (!out)
@@ -483,7 +487,7 @@ __global__ __launch_bounds__(1024) void ln_join_kernel(const float* __restrict__
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1)
         v += __shfl_xor(v, o, 64);
-    const int64_t to = (int64_t) blockIdx.x * 32 + part;
+    const int64_t to = first + part;
     if (threadIdx.x % 32 == 0 && to < width)
         IOTraits<T>::store1(out + to, v);
 }
@@ -559,13 +563,13 @@ int layer_norm_fwd(const T* x, const T* w, const T* b, int64_t rows, int64_t wid
     MIQ_CHECK_ARG((mean != nullptr) == (rstd != nullptr), "mean and rstd go together");
     hipStream_t s  = (hipStream_t) stream;
     if (rows_of(width) == Rows::kLong)
-        hipLaunchKernelGGL(ln_fwd_long_kernel<T>, dim3((unsigned) rows), dim3(1024), 0, s, x, w, b, width, eps, y, mean,
+        hipLaunchKernelGGL(ln_fwd_long_kernel<T>, grid_of(rows, 1024), dim3(1024), 0, s, x, w, b, rows, width, eps, y, mean,
                            rstd);
     else
         with_rows<T>(width, [&](auto per, auto lanes) {
             constexpr int P = decltype(per)::value, L = decltype(lanes)::value;
             constexpr int kRows = L < kBlock ? kBlock / L : 1, kThreads = L < kBlock ? kBlock : L;
-            hipLaunchKernelGGL((ln_fwd_kernel<T, P, L>), dim3((unsigned) ((rows + kRows - 1) / kRows)),
+            hipLaunchKernelGGL((ln_fwd_kernel<T, P, L>), grid_of((rows + kRows - 1) / kRows, kThreads),
                                dim3(kThreads), 0, s, x, w, b, rows, (int) width, eps, y, mean, rstd);
         });
     MIQ_CHECK_LAUNCH();
@@ -588,8 +592,8 @@ int layer_norm_bwd(const T* x, const T* g, const T* w, const float* mean, const 
     if (rows_of(width) == Rows::kLong)
     {
         if (dx && rows)
-            hipLaunchKernelGGL(ln_dx_long_kernel<T>, dim3((unsigned) rows), dim3(1024), 0, s, x, g, w, mean, rstd, width,
-                               dx);
+            hipLaunchKernelGGL(ln_dx_long_kernel<T>, grid_of(rows, 1024), dim3(1024), 0, s, x, g, w, mean, rstd, rows,
+                               width, dx);
         MIQ_CHECK_LAUNCH();
         if (partial)
             hipLaunchKernelGGL(ln_dparams_long_kernel<T>, dim3((unsigned) ((width + kBlock - 1) / kBlock), (unsigned) slices),
@@ -608,8 +612,8 @@ int layer_norm_bwd(const T* x, const T* g, const T* w, const float* mean, const 
     }
     if (partial)
     {
-        hipLaunchKernelGGL(ln_join_kernel<T>, dim3((unsigned) ((width + 31) / 32), 2), dim3(1024), 0, s, partial, slices,
-                           width, dw, db);
+        const dim3 over = grid_of((width + 31) / 32, 1024);   // (y: weight and bias)
+        hipLaunchKernelGGL(ln_join_kernel<T>, dim3(over.x, 2, over.y), dim3(1024), 0, s, partial, slices, width, dw, db);
         MIQ_CHECK_LAUNCH();
     }
     return MIQ_OK;

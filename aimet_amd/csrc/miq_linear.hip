@@ -69,7 +69,7 @@ __global__ __launch_bounds__(kBlock) void pack_rows_kernel(const float* __restri
 {
     constexpr int kHeld = 4;
     const int lane  = threadIdx.x % LANES;
-    const int64_t r = (int64_t) blockIdx.x * (kBlock / LANES) + threadIdx.x / LANES;
+    const int64_t r = block_index() * (kBlock / LANES) + threadIdx.x / LANES;
     if (r >= rows)
         return;
     const float* from = src + r * ld;
@@ -127,7 +127,7 @@ __global__ __launch_bounds__(kBlock) void copy_rows_kernel(const T* __restrict__
                                                            int64_t kp, T* __restrict__ out)
 {
     constexpr int VEC = IOTraits<T>::VEC;
-    const int64_t per = kp / VEC, at = (int64_t) blockIdx.x * kBlock + threadIdx.x;
+    const int64_t per = kp / VEC, at = block_index() * kBlock + threadIdx.x;
     if (at >= rows * per)
         return;
     const int64_t r = at / per, c = at % per * VEC;
@@ -508,8 +508,7 @@ int copy_rows(const T* src, int64_t rows, int64_t k, int64_t kp, T* to, hipStrea
     const int64_t blocks = (rows * (kp / IOTraits<T>::VEC) + kBlock - 1) / kBlock;
     if (blocks == 0)
         return MIQ_OK;
-    MIQ_CHECK_ARG(blocks <= INT32_MAX, "an operand is too large");
-    hipLaunchKernelGGL(copy_rows_kernel<T>, dim3((unsigned) blocks), dim3(kBlock), 0, s, src, rows, k, kp, to);
+    hipLaunchKernelGGL(copy_rows_kernel<T>, grid_of(blocks, kBlock), dim3(kBlock), 0, s, src, rows, k, kp, to);
     MIQ_CHECK_LAUNCH();
     return MIQ_OK;
 }
@@ -523,10 +522,10 @@ int pack(const Matrix<float>& x, int64_t kp, char* to, char* scale, hipStream_t 
     if (!x.columns)
     {
         if (x.k <= 2048)
-            hipLaunchKernelGGL(pack_rows_kernel<64>, dim3((unsigned) ((x.count + 3) / 4)), dim3(kBlock), 0, s, x.p, x.ld,
+            hipLaunchKernelGGL(pack_rows_kernel<64>, grid_of((x.count + 3) / 4, kBlock), dim3(kBlock), 0, s, x.p, x.ld,
                                x.count, x.k, kp, (uint16_t*) to, exponents);
         else
-            hipLaunchKernelGGL(pack_rows_kernel<256>, dim3((unsigned) x.count), dim3(kBlock), 0, s, x.p, x.ld, x.count,
+            hipLaunchKernelGGL(pack_rows_kernel<256>, grid_of(x.count, kBlock), dim3(kBlock), 0, s, x.p, x.ld, x.count,
                                x.k, kp, (uint16_t*) to, exponents);
         MIQ_CHECK_LAUNCH();
         return MIQ_OK;
@@ -536,7 +535,7 @@ int pack(const Matrix<float>& x, int64_t kp, char* to, char* scale, hipStream_t 
                        x.p, x.ld, x.k, x.count, (x.k + slices - 1) / slices, largest);
     MIQ_CHECK_LAUNCH();
     const int64_t tiles = ((x.count + 63) / 64) * ((kp + 63) / 64);
-    MIQ_CHECK_ARG(tiles <= INT32_MAX, "an operand has too many tiles");
+    MIQ_CHECK_ARG(tiles * kBlock <= UINT32_MAX, "an operand has too many tiles");
     hipLaunchKernelGGL(pack_columns_kernel, dim3((unsigned) tiles), dim3(kBlock), 0, s, x.p, x.ld, x.k, x.count, kp,
                        largest, (int) slices, (uint16_t*) to, exponents);
     MIQ_CHECK_LAUNCH();
@@ -574,8 +573,8 @@ int launch_product(Product<T>& p, bool big, hipStream_t s)
     const int tile = big ? 256 : 128;
     p.tiles_m = (int) ((p.e.m + tile - 1) / tile), p.tiles_n = (int) ((p.e.n + tile - 1) / tile);
     const int64_t blocks = (int64_t) p.tiles_m * p.tiles_n * p.splits;
-    MIQ_CHECK_ARG(blocks <= INT32_MAX, "the product has too many tiles");
     const dim3 grid((unsigned) blocks), threads(big ? 512 : 256);
+    MIQ_CHECK_ARG(blocks * threads.x <= UINT32_MAX, "the product has too many tiles");
     if constexpr (std::is_same<T, float>::value)
     {
         if (big)
@@ -599,7 +598,7 @@ int launch_direct(DirectProduct& p, bool big, hipStream_t s)
 {
     p.tiles_m = (int) ((p.e.m + (big ? 127 : 63)) / (big ? 128 : 64)), p.tiles_n = (int) ((p.e.n + 127) / 128);
     const int64_t blocks = (int64_t) p.tiles_m * p.tiles_n * p.splits;
-    MIQ_CHECK_ARG(blocks <= INT32_MAX, "the product has too many tiles");
+    MIQ_CHECK_ARG(blocks * 256 <= UINT32_MAX, "the product has too many tiles");
     if (big)
         hipLaunchKernelGGL((direct_kernel<ACT, 2, 2, 4, 4, AC, BC>), dim3((unsigned) blocks), dim3(256), 0, s, p);
     else
@@ -653,7 +652,7 @@ int product(const Matrix<T>& a, const Matrix<T>& b, const T* bias, const T* resi
         if (plan.way == Way::kShortSum)
         {
             const int64_t tiles = ((e.m + 127) / 128) * ((e.n + 127) / 128);
-            MIQ_CHECK_ARG(tiles <= INT32_MAX, "the product has too many tiles");
+            MIQ_CHECK_ARG(tiles * kBlock <= UINT32_MAX, "the product has too many tiles");
             hipLaunchKernelGGL(short_sum_kernel, dim3((unsigned) tiles), dim3(kBlock), 0, s, a.p, a.ld, b.p, (int) a.k, e);
             MIQ_CHECK_LAUNCH();
             return MIQ_OK;

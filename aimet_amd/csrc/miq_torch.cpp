@@ -60,9 +60,17 @@ P* data(const Tensor& t)
     return t.defined() ? static_cast<P*>(t.data_ptr()) : nullptr;
 }
 
+// t's values, row after row in memory (a lazily negated tensor, as the imaginary part of a conjugate is, holds others)
 Tensor contiguous(const Tensor& t)
 {
-    return t.defined() ? t.contiguous() : t;
+    return !t.defined() ? t : t.is_neg() ? t.resolve_neg().contiguous() : t.contiguous();
+}
+
+void no_forward_mode(std::initializer_list<const Tensor*> tensors)
+{
+    for (const Tensor* t : tensors)
+        TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(),
+                    "aimet_amd kernels are not differentiated in forward mode: got a dual tensor");
 }
 
 bool is_bf16(const Tensor& x)
@@ -86,7 +94,7 @@ Tensor layer_norm_fwd(const Tensor& x, int64_t width, const Tensor& weight, cons
     TORCH_CHECK(!weight.defined() || weight.numel() == width, "weight has ", weight.numel(), " elements, a row has ", width);
     TORCH_CHECK(!bias.defined() || bias.numel() == width, "bias has ", bias.numel(), " elements, a row has ", width);
     const c10::DeviceGuard guard(x.device());
-    const Tensor xc = x.contiguous(), w = contiguous(weight), b = contiguous(bias);
+    const Tensor xc = contiguous(x), w = contiguous(weight), b = contiguous(bias);
     Tensor y        = at::empty(x.sizes(), xc.options());
     float* mean     = nullptr;
     if (stats)
@@ -120,7 +128,7 @@ NormGrads layer_norm_bwd(const Tensor& x, const Tensor& grad, int64_t width, con
                 "stats is not what layer_norm_fwd returned for these rows");
     TORCH_CHECK(!weight.defined() || weight.numel() == width, "weight has ", weight.numel(), " elements, a row has ", width);
     const c10::DeviceGuard guard(x.device());
-    const Tensor xc = x.contiguous(), g = grad.contiguous(), w = contiguous(weight);
+    const Tensor xc = contiguous(x), g = contiguous(grad), w = contiguous(weight);
     NormGrads out;
     Tensor workspace;
     if (want_x)
@@ -176,7 +184,7 @@ Tensor linear_fwd(const Tensor& x, const Tensor& weight, const Tensor& bias, int
                 residual.sizes(), ", ", at::IntArrayRef(shape), " is expected");
     const c10::DeviceGuard guard(x.device());
     const bool bf16 = is_bf16(x);
-    const Tensor xc = x.contiguous(), w = weight.contiguous(), b = contiguous(bias), r = contiguous(residual);
+    const Tensor xc = contiguous(x), w = contiguous(weight), b = contiguous(bias), r = contiguous(residual);
     Tensor y = at::empty(shape, xc.options()), workspace;
     if (saved && activation)
         *saved = at::empty(shape, xc.options().dtype(bf16 ? at::kHalf : at::kFloat));
@@ -210,7 +218,7 @@ LinearGrads linear_bwd(const Tensor& grad, const Tensor& saved, const Tensor& x,
                                 saved.scalar_type() == (bf16 ? at::kHalf : at::kFloat) && saved.numel() == rows * out),
                 "saved is not what linear_fwd returned for these shapes");
     const c10::DeviceGuard guard(x.device());
-    const Tensor g = grad.contiguous(), xc = x.contiguous(), w = weight.contiguous();
+    const Tensor g = contiguous(grad), xc = contiguous(x), w = contiguous(weight);
     LinearGrads to;
     Tensor workspace;
     if (want_x)
@@ -271,7 +279,7 @@ struct LayerNormNode : torch::autograd::Function<LayerNormNode>
     {
         const Tensor weight = weight_.value_or(Tensor()), bias = bias_.value_or(Tensor());
         Tensor stats;
-        const Tensor xc = x.contiguous();
+        const Tensor xc = contiguous(x);
         Tensor y        = layer_norm_fwd(xc, width, weight, bias, eps, &stats);
         ctx->save_for_backward({xc, weight, stats});
         ctx->saved_data["width"] = width;
@@ -313,7 +321,7 @@ struct LinearNode : torch::autograd::Function<LinearNode>
         const Tensor bias = bias_.value_or(Tensor()), residual = residual_.value_or(Tensor());
         // `products`: x, weight or bias want a gradient, not the residual alone
         Tensor saved;
-        const Tensor xc = x.contiguous(), w = weight.contiguous();
+        const Tensor xc = contiguous(x), w = contiguous(weight);
         Tensor y        = linear_fwd(xc, w, bias, (int) activation, residual, products ? &saved : nullptr);
         if (products)
             ctx->save_for_backward({xc, w, saved});
@@ -359,7 +367,7 @@ bool differentiates(std::initializer_list<const Tensor*> tensors)
 
 Tensor cast(const Tensor& t, at::ScalarType type)
 {
-    return t.defined() && t.is_floating_point() && t.scalar_type() != type ? t.to(type) : t;
+    return t.defined() && t.is_floating_point() && t.scalar_type() != at::kDouble && t.scalar_type() != type ? t.to(type) : t;
 }
 
 Tensor layer_norm(Tensor x, at::IntArrayRef shape, Tensor weight, Tensor bias, double eps)
@@ -372,6 +380,7 @@ Tensor layer_norm(Tensor x, at::IntArrayRef shape, Tensor weight, Tensor bias, d
     TORCH_CHECK(!bias.defined() || bias.sizes() == shape, "bias has shape ", bias.sizes(), ", ", shape, " is expected");
     if (at::autocast::is_autocast_enabled(at::kCUDA))
         x = cast(x, at::kFloat), weight = cast(weight, at::kFloat), bias = cast(bias, at::kFloat);
+    no_forward_mode({&x, &weight, &bias});
     int64_t width = 1;
     for (const int64_t d : shape)
         width *= d;
@@ -387,6 +396,7 @@ Tensor linear(Tensor x, Tensor weight, Tensor bias, int activation, Tensor resid
         const at::ScalarType type = at::autocast::get_autocast_dtype(at::kCUDA);
         x = cast(x, type), weight = cast(weight, type), bias = cast(bias, type), residual = cast(residual, type);
     }
+    no_forward_mode({&x, &weight, &bias, &residual});
     if (differentiates({&x, &weight, &bias, &residual}))
         return LinearNode::apply(x, weight, given(bias), given(residual), (int64_t) activation,
                                  differentiates({&x, &weight, &bias}));

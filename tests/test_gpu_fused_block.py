@@ -190,6 +190,31 @@ def test_layer_norm_gradient_against_differences(fused):
         assert abs((grads[k].double() * v).sum() - want) <= bound
 
 
+def test_layer_norm_of_more_rows_than_a_grid_axis_holds(fused):
+    rows, width = (1 << 26) + 5, 8                             # 64 threads a row: 2^32 threads and a few
+    x = torch.zeros(rows, width, dtype=torch.bfloat16, device="cuda")
+    tail = randn(9, width, dtype=torch.bfloat16, seed=1)
+    x[-9:] = tail
+    x[:9] = tail
+    y = fused.layer_norm(x, width)
+    want = fused.layer_norm(tail, width)
+    assert torch.equal(y[-9:], want) and torch.equal(y[:9], want) and not y[9:-9].any()
+
+
+def test_layer_norm_of_the_widest_rows(fused):
+    from aimet_amd import ops
+    width = (1 << 27) + 3                                      # the columns' sums: 32 threads a column
+    x = randn(1, width, dtype=torch.bfloat16, seed=1)
+    g = randn(1, width, dtype=torch.bfloat16, seed=2)
+    _, stats = ops.layer_norm_fwd(x, width, want_stats=True)
+    _, dw, db = ops.layer_norm_bwd(x, g, width, None, stats, False, True, True)
+    assert torch.equal(db, g[0])                               # one row: its own gradient, unrounded
+    # two roundings of 32 bits in (x - mean) rstd, one for the product with g, one to bfloat16
+    for at in (slice(0, 1000), slice(width - 1000, width)):
+        want = g[0, at].double() * (x[0, at].double() - stats[0].double()) * stats[1].double()
+        assert_within(dw[at], want, want.abs() * (2 ** -8 * 1.001) + 2 ** -130, "dweight")
+
+
 def test_layer_norm_offsets_past_32_bits(fused):
     rows, width = 270000, 8200                                # 2.2e9 elements
     x = torch.zeros(rows, width, dtype=torch.bfloat16, device="cuda")
@@ -526,7 +551,43 @@ def test_two_streams_at_once(fused):
             assert all(torch.equal(p, q) for p, q in zip(out, want[k]))
 
 
+def test_lazily_negated_tensors(fused):
+    """A tensor may stand for the negative of what lies in memory (the imaginary part of a conjugate does)."""
+    x, w, b, res, g = linear_case(20, 64, 48, torch.float32, True)
+    lazy = [torch._neg_view(-t) for t in (x, w, b, res)]       # pylint: disable=protected-access
+    assert all(t.is_neg() for t in lazy)
+    assert torch.equal(fused.linear(lazy[0], lazy[1], lazy[2], "gelu", lazy[3]), fused.linear(x, w, b, "gelu", res))
+    assert torch.equal(fused.layer_norm(lazy[0], 64, lazy[1][0], lazy[1][1]), fused.layer_norm(x, 64, w[0], w[1]))
+    for f in (lambda t: fused.linear(t, w, b, "gelu", res), lambda t: fused.layer_norm(t, 64).repeat(1, 2)[:, :48]):
+        leaf = x.clone().requires_grad_()
+        want, = torch.autograd.grad(f(leaf), leaf, g)
+        got, = torch.autograd.grad(f(leaf), leaf, torch._neg_view(-g))    # pylint: disable=protected-access
+        assert torch.equal(got, want)
+
+
 # ------------------------------------------------------------------------------------------------------- refusals
+def test_forward_mode_is_refused(fused):
+    import torch.autograd.forward_ad as fwad
+    x, w, b, res, _ = linear_case(4, 32, 24, torch.float32, True)
+    with fwad.dual_level():
+        for i in range(4):
+            args = [x, w, b, res]
+            args[i] = fwad.make_dual(args[i], torch.ones_like(args[i]))
+            with pytest.raises(RuntimeError, match="forward mode"):
+                fused.linear(args[0], args[1], args[2], "none", args[3])
+        with pytest.raises(RuntimeError, match="forward mode"):
+            fused.layer_norm(fwad.make_dual(x, x), 32)
+
+
+def test_autocast_leaves_float64_to_be_refused(fused):
+    x, w, _, _, _ = linear_case(4, 32, 24, torch.float32, True)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        for call in (lambda: fused.linear(x.double(), w), lambda: fused.linear(x, w.double()),
+                     lambda: fused.layer_norm(x.double(), 32)):
+            with pytest.raises(RuntimeError):
+                call()
+
+
 def test_refusals(fused):
     x, w, b, res, _ = linear_case(4, 32, 24, torch.float32, True)
     bad = [
