@@ -11,6 +11,7 @@
 #include <ATen/autocast_mode.h>
 #include <ATen/core/grad_mode.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -266,6 +267,26 @@ variable_list not_twice(variable_list grads)
     return grads;
 }
 
+// A leaf's gradient is accumulated on the stream of the first graph that is still alive.  Where that is an eager one of the
+// default stream, a backward pass under capture would have the default stream wait for a captured one, which ends the
+// process: refused beforehand.
+void refuse_eager_leaves_under_capture()
+{
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None)
+        return;
+    const auto node = torch::autograd::get_current_node();
+    if (!node)
+        return;
+    for (const torch::autograd::Edge& edge : node->next_edges())
+    {
+        if (!edge.function || edge.function->name() != "torch::autograd::AccumulateGrad")
+            continue;
+        const std::optional<c10::Stream> stream = edge.function->stream();
+        TORCH_CHECK(!stream || stream->id() != 0, "a backward pass cannot be captured into a graph while an eager autograd graph "
+                    "of the same leaves, made on the default stream, is alive: delete its outputs first");
+    }
+}
+
 // A node has an edge for every tensor it was given, and none for those it was not
 std::optional<Tensor> given(const Tensor& t)
 {
@@ -292,6 +313,7 @@ struct LayerNormNode : torch::autograd::Function<LayerNormNode>
 
     static variable_list backward(AutogradContext* ctx, variable_list grads)
     {
+        refuse_eager_leaves_under_capture();
         const bool twice = at::GradMode::is_enabled();
         variable_list out(5);
         {
@@ -333,6 +355,7 @@ struct LinearNode : torch::autograd::Function<LinearNode>
 
     static variable_list backward(AutogradContext* ctx, variable_list grads)
     {
+        refuse_eager_leaves_under_capture();
         const bool twice = at::GradMode::is_enabled();
         variable_list out(6);
         size_t edge         = 0;

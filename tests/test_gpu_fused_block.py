@@ -529,6 +529,34 @@ def test_captured_training_step(fused, dtype, rows):
             assert all(torch.equal(p, q) for p, q in zip(out, want)), k
 
 
+@pytest.mark.parametrize("norm", [True, False])
+def test_capture_beside_a_living_eager_graph_is_refused(fused, norm):
+    x, w, b, _, g = linear_case(8, 64, 64, torch.float32, False)
+    leaves = [t.clone().requires_grad_() for t in ((x, w[0].contiguous(), b) if norm else (x, w, b))]
+
+    def forward():
+        return fused.layer_norm(leaves[0], 64, leaves[1], leaves[2]) if norm else fused.linear(*leaves)
+
+    want = torch.autograd.grad(forward(), leaves, g)
+    torch.cuda.synchronize()
+    alive = forward()                                          # on the default stream
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = forward()
+        with pytest.raises(RuntimeError, match="eager autograd graph"):
+            torch.autograd.grad(y, leaves, g)
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(alive, leaves, g), want))
+    del y, alive                                               # now it can be
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(forward(), leaves, g)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
 def test_two_streams_at_once(fused):
     """Calls that overlap share no scratch memory."""
     cases = [linear_case(900, 512, 520, torch.float32, False, seed=s) for s in (1, 2)]
