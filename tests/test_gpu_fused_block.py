@@ -529,6 +529,22 @@ def test_captured_training_step(fused, dtype, rows):
             assert all(torch.equal(p, q) for p, q in zip(out, want)), k
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_one_tensor_in_several_places(fused, dtype):
+    """Its gradient is the sum of those of separate tensors (two summands: in either order the same)."""
+    x, w, b, _, g = linear_case(64, 64, 64, dtype, True)
+    for f, places in ((lambda p, q: fused.linear(p, q, b, "silu"), (x, x)),
+                      (lambda p, q: fused.linear(p, w, b, "gelu", q), (x, x)),
+                      (lambda p, q: fused.linear(x, w, p, "none", q.expand(64, 64)), (b, b)),
+                      (lambda p, q: fused.layer_norm(x, 64, p, q), (b, b))):
+        apart = [t.clone().requires_grad_() for t in places]
+        one = places[0].clone().requires_grad_()
+        first, second = torch.autograd.grad(f(*apart), apart, g)
+        y = f(one, one)
+        assert torch.equal(y, f(*apart))
+        assert torch.equal(torch.autograd.grad(y, one, g)[0], first + second)
+
+
 @pytest.mark.parametrize("norm", [True, False])
 def test_capture_beside_a_living_eager_graph_is_refused(fused, norm):
     x, w, b, _, g = linear_case(8, 64, 64, torch.float32, False)
