@@ -317,7 +317,7 @@ void with_activation(int activation, F&& f)
 
 int64_t slope_slices(int64_t rows, int64_t cols)
 {
-    const int64_t columns = (cols + kBlock - 1) / kBlock;
+    const int64_t columns = std::max<int64_t>(1, (cols + kBlock - 1) / kBlock);   // (a layer may have no outputs)
     return std::max<int64_t>(1, std::min<int64_t>((1024 + columns - 1) / columns, rows / 16));
 }
 

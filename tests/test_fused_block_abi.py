@@ -1,8 +1,13 @@
 """Arguments that the layer norm and linear entry points refuse, and their workspace sizes, on the host: every check
 comes before the first use of the GPU."""
 import ctypes
+import os
+import subprocess
+import sys
 
 import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 P = ctypes.c_void_p(256)         # stands for a device pointer; never read
 
@@ -56,6 +61,24 @@ def test_linear_refusals(lib, suffix):
             _refused(lib, fwd(P, P, None, None, rows, n_in, n_out, 3, P, None, P, need - 1, None), "workspace")
     assert fwd(None, None, None, None, 0, 8, 8, 0, None, None, None, 0, None) == 0
     assert lib.miq_linear_workspace_bytes(-1, 8, 8, 0, 0, 1, 1) == 0
+
+
+def test_linear_workspace_of_layers_without_outputs():
+    """In a process of its own: a division by zero on the host would end the test run, not fail a test."""
+    code = ("import sys; sys.path.insert(0, %r)\n"
+            "from aimet_amd._lib import lib\n"
+            "for bf16 in (0, 1):\n"
+            "    for activation in (0, 3):\n"
+            "        for shape in ((5, 24, 0), (300, 4096, 0), (0, 24, 0), (5, 0, 0), (5, 0, 7), (0, 0, 0)):\n"
+            "            for backward in (0, 1):\n"
+            "                for aligned in (0, 1):\n"
+            "                    print(bf16, activation, shape, backward, aligned, end=' ', flush=True)\n"
+            "                    print(lib.miq_linear_workspace_bytes(*shape, activation, bf16, backward, aligned))"
+            % ROOT)
+    run = subprocess.run([sys.executable, "-c", code], stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True, check=False)
+    lines = run.stdout.splitlines()
+    assert run.returncode == 0, (run.returncode, lines[-1:], run.stderr)
+    assert len(lines) == 96 and all(int(line.split()[-1]) >= 0 for line in lines)
 
 
 def test_functions_refuse_before_any_launch():

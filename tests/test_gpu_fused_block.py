@@ -362,6 +362,19 @@ def test_linear_without_rows_or_features(fused):
                 assert dx.shape == (rows, 0) and dw.shape == (40, 0) and (db == rows).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ["none", "gelu"])
+@pytest.mark.parametrize("rows,k", [(5, 24), (300, 520), (0, 24), (5, 0)])
+def test_linear_without_outputs(fused, dtype, act, rows, k):
+    x = randn(rows, k, dtype=dtype, seed=1).requires_grad_()
+    w = torch.empty(0, k, dtype=dtype, device="cuda", requires_grad=True)
+    b = torch.empty(0, dtype=dtype, device="cuda", requires_grad=True)
+    y = fused.linear(x, w, b, act)
+    assert y.shape == (rows, 0)
+    dx, dw, db = torch.autograd.grad(y, [x, w, b], torch.empty_like(y))
+    assert dx.shape == (rows, k) and not dx.any() and dw.shape == (0, k) and db.shape == (0,)
+
+
 def test_linear_keeps_bad_rows_to_themselves(fused):
     """An infinity or a NaN in a row of x reaches that row of the output alone, as what float32 arithmetic makes of it."""
     for dtype in DTYPES:
