@@ -326,12 +326,15 @@ int64_t up256(int64_t n)
     return (n + 255) / 256 * 256;
 }
 
+// Longest row of an operand, in values of up to 4 bytes (a value's two halves take 4): a load spans 8 rows, and a lane's
+// offset within them has 32 bits
+constexpr int64_t kLongest = 1 << 27;
+
 int check_shape(int64_t rows, int64_t in, int64_t out, int activation)
 {
     MIQ_CHECK_ARG(rows >= 0 && in >= 0 && out >= 0, "rows, in_features and out_features must not be negative");
     MIQ_CHECK_ARG(rows <= INT32_MAX, "rows must be below 2^31");
-    // (a lane's offset within the rows that a load spans has 32 bits)
-    MIQ_CHECK_ARG(in <= 1 << 27 && out <= 1 << 27, "in_features and out_features must be at most 2^27");
+    MIQ_CHECK_ARG(in <= kLongest && out <= kLongest, "in_features and out_features must be at most 2^27");
     MIQ_CHECK_ARG(activation >= MIQ_ACT_NONE && activation <= MIQ_ACT_GELU_TANH, "unknown activation %d", activation);
     return MIQ_OK;
 }
@@ -386,9 +389,12 @@ int64_t max_slices(int64_t k)
 // [256, 4096] x [4096, 4096]^T 62 and 71, [512, 4096] x [4096, 4096]^T 106 and 93, the input's gradient of
 // [512, 4096] x [11008, 4096]^T 246 and 263, of [768, 4096] x [4096, 4096]^T 172 and 141, the weight's gradient of
 // [512, 4096] x [4096, 4096]^T 102 and 91.
+// Sums too long for rows of halves (a weight's gradient over more rows than that: both operands in columns) take the first.
 template <typename T>
 bool direct_pays(const Matrix<T>& a, const Matrix<T>& b)
 {
+    if (a.k > kLongest)
+        return true;
     const auto halves = [](const Matrix<T>& x, double columns) {
         return (double) x.count * x.k * (x.columns ? columns : 2e-12) + (x.columns ? 15e-6 : 0);
     };

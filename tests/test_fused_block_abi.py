@@ -81,6 +81,14 @@ def test_linear_workspace_of_layers_without_outputs():
     assert len(lines) == 96 and all(int(line.split()[-1]) >= 0 for line in lines)
 
 
+@pytest.mark.parametrize("rows", [(1 << 27) + 1, 160_000_000, (1 << 31) - 1])
+@pytest.mark.parametrize("features", [8, 16, 64])
+def test_sums_over_more_rows_than_a_row_of_halves_holds(lib, rows, features):
+    """The weight's gradient sums over the rows.  Rows of halves that long are past what a lane's 32-bit offset spans; the
+    way without halves needs no copy of x, which shows in the workspace: halves of x take 4 bytes for each value."""
+    assert 0 < lib.miq_linear_workspace_bytes(rows, features, features, 0, 0, 1, 1) < rows * features * 4
+
+
 def test_functions_refuse_before_any_launch():
     import torch
     from aimet_amd.v2.nn import fused

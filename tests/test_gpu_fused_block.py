@@ -491,6 +491,21 @@ def test_linear_offsets_past_32_bits(fused):
     assert not dx[:-2].any()
 
 
+def test_linear_weight_gradient_over_more_rows_than_a_row_of_halves_holds(fused):
+    """Whole numbers in a few of 160 million rows, zeros in the others: the sums are exact."""
+    from aimet_amd import ops
+    rows, n = 160_000_000, 8
+    x, g = torch.zeros(rows, n, device="cuda"), torch.zeros(rows, n, device="cuda")
+    at = torch.tensor([0, 1, 31, 32, 4095, rows // 7, (1 << 27) - 1, 1 << 27, (1 << 27) + 1, rows - 33, rows - 2, rows - 1],
+                      device="cuda")
+    small = torch.Generator(device="cuda").manual_seed(3)
+    x[at] = torch.randint(-9, 10, (len(at), n), generator=small, device="cuda").float()
+    g[at] = torch.randint(-9, 10, (len(at), n), generator=small, device="cuda").float()
+    _, dw, db = ops.linear_bwd(g, None, x, torch.zeros(n, n, device="cuda"), "none", False, True, True)
+    assert torch.equal(dw.double(), (g[at].double()[:, :, None] * x[at].double()[:, None, :]).sum(0))
+    assert torch.equal(db.double(), g[at].double().sum(0))
+
+
 def _backward_of_itself(y, x, w):
     from aimet_amd import ops
     return ops.linear_bwd(y, None, x, w, "none")
