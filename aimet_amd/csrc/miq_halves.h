@@ -22,6 +22,78 @@ __device__ __forceinline__ int64_t place_of_half(int64_t k)
     return k / kHalves * (2 * kHalves) + k % kHalves;
 }
 
+constexpr int kZeroRow = -(1 << 30);   // what a row of zeros is said to have lost; more than a row has values
+
+// Sums of a strip that are formed one by one; more take the matrix unit and 100 us.  The weight's gradient of
+// [4096, 4096] x [4096, 4096]^T with a few such sums in one column of x: 409 us, 820 by strips alone, 397 without any.
+constexpr int kFewSums = 16;
+
+// 4 values of row r from k on, zeros from `to` on
+__device__ __forceinline__ void load_plain(const Plain& x, int64_t r, int64_t k, int64_t to, float* v)
+{
+    if (!x.columns && k + 4 <= to)
+        load_any(x.p + r * x.ld + k, v);
+    else
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+            v[t] = k + t < to ? x.p[x.columns ? (k + t) * x.ld + r : r * x.ld + k + t] : 0.f;
+}
+
+// Sums over k in [from, to) of 16 rows of a (lane l: row r, of l % 16) and 16 FN rows of b from q0 on (those past the end are the
+// last one again: what they make is not stored), straight from memory, as float32.  Four values of k of a row a lane, as
+// the first and second factor of four v_mfma_f32_16x16x4: which value of k meets which step is the same for both.
+// It runs for few strips or for none: of [4096, 4096] x [4096, 4096]^T all of them take 2.6 ms, and 4.0 for the weight's gradient.
+template <int FN>
+__device__ __forceinline__ void float32_strip(const Plain a, int64_t r, const Plain b, int64_t q0, int64_t n, int64_t from,
+                                                        int64_t to, int lane, f4* sums)
+{
+    constexpr int kUnroll = 4;
+    int64_t rb[FN];
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+    {
+        const int64_t q = q0 + row_of_b(j, lane % 16);
+        rb[j]           = q < n ? q : n - 1;
+        sums[j]         = f4{0.f, 0.f, 0.f, 0.f};
+    }
+    for (int64_t k0 = from; k0 < to; k0 += 16 * kUnroll)
+    {
+        float va[kUnroll][4], vb[kUnroll][FN][4];
+#pragma unroll
+        for (int s = 0; s < kUnroll; ++s)
+        {
+            const int64_t k = k0 + 16 * s + lane / 16 * 4;
+            load_plain(a, r, k, to, va[s]);
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+                load_plain(b, rb[j], k, to, vb[s][j]);
+        }
+#pragma unroll
+        for (int s = 0; s < kUnroll; ++s)
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int j = 0; j < FN; ++j)
+                    sums[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(vb[s][j][t], va[s][t], sums[j], 0, 0, 0);
+    }
+}
+
+// The sum of one row of a and one of b, the same in all lanes
+__device__ __forceinline__ float float32_sum(const Plain a, int64_t r, const Plain b, int64_t q, int64_t from, int64_t to, int lane)
+{
+    const float* pa       = a.p + (a.columns ? r : r * a.ld);
+    const float* pb       = b.p + (b.columns ? q : q * b.ld);
+    const int64_t step_a = a.columns ? a.ld : 1, step_b = b.columns ? b.ld : 1;
+    float s              = 0.f;
+#pragma unroll 8
+    for (int64_t k = from + lane; k < to; k += 64)
+        s = fmaf(pa[k * step_a], pb[k * step_b], s);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1)
+        s += __shfl_xor(s, o, 64);
+    return s;
+}
+
 template <int ACT, int WM, int WN, int FM, int FN>
 __global__ __launch_bounds__(WM* WN * 64) void halves_kernel(const Product<float> p)
 {
@@ -56,6 +128,23 @@ __global__ __launch_bounds__(WM* WN * 64) void halves_kernel(const Product<float
         la.p += (int64_t) first * la.step;
         lb.p += (int64_t) first * lb.step;
     };
+
+    // what the lane's rows lost, and the most that one of its columns did: read here, where nobody waits for it
+    int lost_a[FM], lost_b = kZeroRow;
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+    {
+        const int64_t r = m0 + wm * FM * 16 + i * 16 + lane % 16;
+        lost_a[i]       = r < p.e.m ? p.scale_a[p.e.m + r] : kZeroRow;
+    }
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+        {
+            const int64_t q = n0 + wn * FN * 16 + row_of_b(j, lane / 16 * 4 + u);
+            lost_b          = max(lost_b, q < p.e.n ? p.scale_b[p.e.n + q] : kZeroRow);
+        }
 
     f4 acc[FM][FN];
 #pragma unroll
@@ -167,100 +256,102 @@ __global__ __launch_bounds__(WM* WN * 64) void halves_kernel(const Product<float
             sum(std::false_type());
     }
 
-    // Corrections are finite for finite operands.  Where an infinity or a NaN made a sum anything else, the coarse halves
-    // alone say what comes out: those sums are formed once more, corrections first, cleared where they are not finite, and
-    // the rest added.  The others are stored as they are.
-    uint32_t bad[FM * FN / 8] = {};
-    bool finite               = true;
+    // Sums that are formed again, from float32 operands by float32 matrix instructions:
+    // - what is not finite.  Corrections are finite for finite operands, but an infinity or a NaN makes them anything.
+    // - what lost bits may have changed.  Scaled values are below 2^15, and one that lost bits is off by at most 2^-25: the
+    //   sum by at most 2^-10 for each such value of its two rows.  That is allowed to be k / 4 times 2^-24 of the sum itself,
+    //   and so of the sum of its terms' magnitudes, of which float32 arithmetic may lose k times 2^-24.  Of normally
+    //   distributed rows of 4096 one in 15 has such a value, and one sum in 10^8 is then small enough to be formed again.
+    // The others are stored as they are.
+    static_assert(FN == 4 && FM <= 8, "16 bits a row of fragments, in two words");
+    uint64_t again[2] = {};
+    const float most  = 65536.0f / (float) p.length;
 #pragma unroll
     for (int i = 0; i < FM; ++i)
+    {
+        const int64_t r  = m0 + wm * FM * 16 + i * 16 + lane % 16;
+        const float weak = (float) (lost_a[i] + lost_b) * most;
+        bool any         = false;
 #pragma unroll
         for (int j = 0; j < FN; ++j)
 #pragma unroll
             for (int u = 0; u < 4; ++u)
-                if (!__builtin_isfinite(acc[i][j][u]))
-                {
-                    bad[(i * FN + j) / 8] |= 1u << ((i * FN + j) % 8 * 4 + u);
-                    finite = false;
-                }
-    const auto store = [&](auto again) {
-#pragma unroll
-        for (int i = 0; i < FM; ++i)
-        {
-            const int64_t r = m0 + wm * FM * 16 + i * 16 + lane % 16;
-            if (r >= p.e.m)
-                continue;
-            const int sr = p.scale_a[r];
-#pragma unroll
-            for (int j = 0; j < FN; j += 2)
-            {
-                const int64_t q = n0 + wn * FN * 16 + 16 * j + 8 * (lane / 16);
-                if (q >= p.e.n)
-                    continue;
-                float z[8];
-#pragma unroll
-                for (int u = 0; u < 8; ++u)
-                    z[u] = ldexpf(acc[i][j + u / 4][u % 4], sr + (q + u < p.e.n ? p.scale_b[q + u] : 0));
-                if constexpr (!decltype(again)::value)
-                    finish_or_keep<float, ACT>(p, split, r, q, z);
-                else
-#pragma unroll
-                    for (int u = 0; u < 8; ++u)
-                        if ((bad[(i * FN + j) / 8] >> ((i * FN + j) % 8 * 4 + u) & 1) && q + u < p.e.n)
-                        {
-                            if (p.splits == 1)
-                                finish1<float, ACT>(p.e, r, q + u, z[u]);
-                            else
-                                p.partial[((int64_t) split * p.e.m + r) * p.e.n + q + u] = z[u];
-                        }
-            }
-        }
-    };
-    store(std::false_type());
-    if (__syncthreads_or(!finite))
-    {
-#pragma unroll
-        for (int i = 0; i < FM; ++i)
+                any |= !(fabsf(acc[i][j][u]) >= weak) || !__builtin_isfinite(acc[i][j][u]);
+        if (any && r < p.e.m)
 #pragma unroll
             for (int j = 0; j < FN; ++j)
-                acc[i][j] = f4{0.f, 0.f, 0.f, 0.f};
-        for (int pass = 0; pass < 2; ++pass)
-        {
-            rewind();
-            for (int s = 0; s < count; ++s)
-            {
-                arrived();
-                la.load(p.a, m0, lds0, wave, lane, LA::kDeep);
-                lb.load(p.b, n0, lds0 + LA::kBytes, wave, lane, LB::kDeep);
-                arrived();
-                Columns c;
-                read_columns(c, lds);
 #pragma unroll
-                for (int i = 0; i < FM; ++i)
+                for (int u = 0; u < 4; ++u)
                 {
-                    Row r;
-                    read_row(r, lds, i);
+                    const int64_t q  = n0 + wn * FN * 16 + row_of_b(j, lane / 16 * 4 + u);
+                    const float here = q < p.e.n ? (float) (lost_a[i] + p.scale_b[p.e.n + q]) * most : 0.f;
+                    if (q < p.e.n && (!(fabsf(acc[i][j][u]) >= here) || !__builtin_isfinite(acc[i][j][u])))
+                        again[i / 4] |= 1ull << (i % 4 * 16 + j * 4 + u);
+                }
+    }
 #pragma unroll
-                    for (int j = 0; j < FN; ++j)
-                        if (pass == 0)
-                        {
-                            acc[i][j] = mfma_16x16x32(c.coarse[j], r.fine, acc[i][j], half);
-                            acc[i][j] = mfma_16x16x32(c.fine[j], r.coarse, acc[i][j], half);
-                        }
-                        else
-                            acc[i][j] = mfma_16x16x32(c.coarse[j], r.coarse, acc[i][j], half);
+    for (int i = 0; i < FM; ++i)
+    {
+        const int64_t r = m0 + wm * FM * 16 + i * 16 + lane % 16;
+        if (r >= p.e.m)
+            continue;
+        const int sr = p.scale_a[r];
+#pragma unroll
+        for (int j = 0; j < FN; j += 2)
+        {
+            const int64_t q = n0 + wn * FN * 16 + 16 * j + 8 * (lane / 16);
+            if (q >= p.e.n)
+                continue;
+            float z[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+                z[u] = ldexpf(acc[i][j + u / 4][u % 4], sr + (q + u < p.e.n ? p.scale_b[q + u] : 0));
+            finish_or_keep<float, ACT>(p, split, r, q, z);
+        }
+    }
+    const int64_t from = (int64_t) first * kHalves, to = (int64_t) last * kHalves < p.length ? (int64_t) last * kHalves : p.length;
+    if (__builtin_amdgcn_ballot_w64((again[0] | again[1]) != 0) == 0)
+        return;
+    const auto put = [&](int64_t r, int64_t q, float z) {
+        if (p.splits == 1)
+            finish1<float, ACT>(p.e, r, q, z);
+        else
+            p.partial[((int64_t) split * p.e.m + r) * p.e.n + q] = z;
+    };
+    for (int i = 0; i < FM; ++i)
+    {
+        uint32_t marks = (uint32_t) ((i < 4 ? again[0] : again[1]) >> (i % 4 * 16)) & 0xffffu;   // 4 bits for each j
+        if (__builtin_amdgcn_ballot_w64(marks != 0) == 0)
+            continue;
+        int count = __popc(marks);
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1)
+            count += __shfl_xor(count, o, 64);
+        const int64_t r0 = m0 + wm * FM * 16 + i * 16, q0 = n0 + wn * FN * 16, r = r0 + lane % 16;
+        if (count <= kFewSums)
+        {
+            // the first lane's first mark, until there is none
+            while (const uint64_t lanes = __builtin_amdgcn_ballot_w64(marks != 0))
+            {
+                const int l = __builtin_ctzll(lanes), bit = __builtin_ctz(__builtin_amdgcn_readlane(marks, l));
+                const int64_t q = q0 + row_of_b(bit / 4, l / 16 * 4 + bit % 4);
+                const float z   = float32_sum(p.plain_a, r0 + l % 16, p.plain_b, q, from, to, lane);
+                if (lane == l)
+                {
+                    put(r, q, z);
+                    marks &= marks - 1;
                 }
             }
-            if (pass == 0)
-#pragma unroll
-                for (int i = 0; i < FM; ++i)
-#pragma unroll
-                    for (int j = 0; j < FN; ++j)
-#pragma unroll
-                        for (int u = 0; u < 4; ++u)
-                            acc[i][j][u] = __builtin_isfinite(acc[i][j][u]) ? acc[i][j][u] : 0.f;
+            continue;
         }
-        store(std::true_type());
+        f4 sums[FN];
+        float32_strip<FN>(p.plain_a, r < p.e.m ? r : p.e.m - 1, p.plain_b, q0, p.e.n, from, to, lane, sums);
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (marks >> (4 * j + u) & 1)
+                    put(r, q0 + row_of_b(j, lane / 16 * 4 + u), sums[j][u]);
     }
 }
 }   // namespace miq

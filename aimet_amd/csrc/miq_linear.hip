@@ -24,6 +24,11 @@ namespace
 // left out, is at most 2^-22 of it and has no sign of its own: about the error of float32 arithmetic itself.  Three
 // products in the half-precision matrix unit take a fifth of the time of one in the float32 one.
 // coarse of an infinity or NaN is itself, its fine is 0.
+//
+// A value below 2^-17 of its row's largest loses bits, and one below 2^-39 is lost.  Where the row's large values meet zeros,
+// that is all there is of the sum.  So each row carries how many of its values lost bits ("lost"; of a row of zeros -2^30,
+// since its sums are zeros whatever the other operand lost), and halves_kernel forms again, from float32 operands, the
+// sums that this may have changed by more than float32 arithmetic would.
 __device__ __forceinline__ int row_shift(uint32_t largest /* bits of a finite float32 */)
 {
     if (largest == 0)
@@ -32,7 +37,8 @@ __device__ __forceinline__ int row_shift(uint32_t largest /* bits of a finite fl
     return 14 - (e ? e - 127 : (31 - __clz(largest)) - 149);
 }
 
-__device__ __forceinline__ void split_value(float x, int shift, uint16_t* coarse, uint16_t* fine)
+// whether bits of x were lost
+__device__ __forceinline__ bool split_value(float x, int shift, uint16_t* coarse, uint16_t* fine)
 {
     const float t    = ldexpf(x, shift);
     const _Float16 c = (_Float16) t;
@@ -40,6 +46,7 @@ __device__ __forceinline__ void split_value(float x, int shift, uint16_t* coarse
     const _Float16 d = __builtin_isfinite(t) ? (_Float16) f : (_Float16) 0.f;
     *coarse          = __builtin_bit_cast(uint16_t, c);
     *fine            = __builtin_bit_cast(uint16_t, d);
+    return fabsf(f - (float) d) > 0x1p-22f * fabsf(t) || (t == 0.f && x != 0.f);
 }
 
 __device__ __forceinline__ uint32_t finite_magnitude(float x)
@@ -48,24 +55,26 @@ __device__ __forceinline__ uint32_t finite_magnitude(float x)
     return b < 0x7f800000u ? b : 0u;
 }
 
-// 8 values as 16-bit operands
-__device__ __forceinline__ void put_parts(const float* v, int shift, uint16_t* coarse, uint16_t* fine)
+// 8 values as 16-bit operands; how many of them lost bits
+__device__ __forceinline__ int put_parts(const float* v, int shift, uint16_t* coarse, uint16_t* fine)
 {
     uint16_t c[8], f[8];
+    int lost = 0;
 #pragma unroll
     for (int u = 0; u < 8; ++u)
-        split_value(v[u], shift, c + u, f + u);
+        lost += split_value(v[u], shift, c + u, f + u);
     *(uint4*) coarse = make_uint4(c[0] | c[1] << 16, c[2] | c[3] << 16, c[4] | c[5] << 16, c[6] | c[7] << 16);
     *(uint4*) fine   = make_uint4(f[0] | f[1] << 16, f[2] | f[3] << 16, f[4] | f[5] << 16, f[6] | f[7] << 16);
+    return lost;
 }
 // out[r] = the halves of src[r][0 .. k), of zeros up to kp (a multiple of kHalves): for every kHalves values their coarse
-// halves and then their fine ones; scale[r] = -s.
+// halves and then their fine ones; scale[r] = -s, lost[r] as above.
 // LANES threads hold a row of up to 32 LANES values in registers between its largest value and its halves; of a longer
 // one what is past them is read again.
 template <int LANES>
 __global__ __launch_bounds__(kBlock) void pack_rows_kernel(const float* __restrict__ src, int64_t ld, int64_t rows,
                                                            int64_t k, int64_t kp, uint16_t* __restrict__ out,
-                                                           int* __restrict__ scale)
+                                                           int* __restrict__ scale, int* __restrict__ lost)
 {
     constexpr int kHeld = 4;
     const int lane  = threadIdx.x % LANES;
@@ -105,20 +114,38 @@ __global__ __launch_bounds__(kBlock) void pack_rows_kernel(const float* __restri
     }
     const int shift = row_shift(largest);
     uint16_t* to    = out + r * 2 * kp;
+    int without     = 0;
 #pragma unroll
     for (int i = 0; i < kHeld; ++i)
     {
         const int64_t c = (i * LANES + lane) * 8;
         if (c < kp)
-            put_parts(v[i], shift, to + place_of_half(c), to + place_of_half(c) + kHalves);
+            without += put_parts(v[i], shift, to + place_of_half(c), to + place_of_half(c) + kHalves);
     }
     for (int64_t c = (kHeld * LANES + lane) * 8; c < kp; c += LANES * 8)
     {
         load8(from + c, k - c, t);
-        put_parts(t, shift, to + place_of_half(c), to + place_of_half(c) + kHalves);
+        without += put_parts(t, shift, to + place_of_half(c), to + place_of_half(c) + kHalves);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1)
+        without += __shfl_xor(without, o, 64);
+    if constexpr (LANES > 64)
+    {
+        __shared__ int lds[LANES / 64];
+        if ((threadIdx.x & 63) == 0)
+            lds[threadIdx.x >> 6] = without;
+        __syncthreads();
+        without = 0;
+#pragma unroll
+        for (int i = 0; i < LANES / 64; ++i)
+            without += lds[i];
     }
     if (lane == 0)
+    {
         scale[r] = -shift;
+        lost[r]  = largest ? without : kZeroRow;
+    }
 }
 
 // out[r][0 .. kp) = src[r][0 .. k), zeros behind
@@ -148,9 +175,10 @@ __global__ __launch_bounds__(kBlock) void copy_rows_kernel(const T* __restrict__
 }
 
 // largest[slice][c] = largest finite magnitude (its bits) in a slice of the rows of column c of src [k][count]: 64 threads
-// of 4 columns across, 4 rows at a time
+// of 4 columns across, 4 rows at a time.  lost[c] = 0, for pack_columns_kernel to add to.
 __global__ __launch_bounds__(kBlock) void column_max_kernel(const float* __restrict__ src, int64_t ld, int64_t k, int64_t count,
-                                                            int64_t rows_per_slice, uint32_t* __restrict__ largest)
+                                                            int64_t rows_per_slice, uint32_t* __restrict__ largest,
+                                                            int* __restrict__ lost)
 {
     __shared__ uint32_t lds[4][256];
     const int across    = threadIdx.x % 64, down = threadIdx.x / 64;
@@ -181,8 +209,11 @@ __global__ __launch_bounds__(kBlock) void column_max_kernel(const float* __restr
     __syncthreads();
     const int at = threadIdx.x % 4 * 64 + threadIdx.x / 4;   // column threadIdx.x of the block's 256
     const int64_t q = (int64_t) blockIdx.x * 256 + threadIdx.x;
-    if (q < count)
-        largest[blockIdx.y * count + q] = max(max(lds[0][at], lds[1][at]), max(lds[2][at], lds[3][at]));
+    if (q >= count)
+        return;
+    largest[blockIdx.y * count + q] = max(max(lds[0][at], lds[1][at]), max(lds[2][at], lds[3][at]));
+    if (blockIdx.y == 0)
+        lost[q] = 0;
 }
 
 // As pack_rows_kernel, of the transpose: src [k][count], row r of the result is column r of src.  64 x 64 values a block,
@@ -190,10 +221,11 @@ __global__ __launch_bounds__(kBlock) void column_max_kernel(const float* __restr
 __global__ __launch_bounds__(kBlock) void pack_columns_kernel(const float* __restrict__ src, int64_t ld, int64_t k,
                                                               int64_t count, int64_t kp,
                                                               const uint32_t* __restrict__ largest, int slices,
-                                                              uint16_t* __restrict__ out, int* __restrict__ scale)
+                                                              uint16_t* __restrict__ out, int* __restrict__ scale,
+                                                              int* __restrict__ lost)
 {
     __shared__ float tile[64][65];
-    __shared__ int shifts[64];
+    __shared__ int shifts[64], without[64];
     const int64_t across = (count + 63) / 64;
     const int64_t r0 = blockIdx.x % across * 64, k0 = blockIdx.x / across * 64;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -209,7 +241,8 @@ __global__ __launch_bounds__(kBlock) void pack_columns_kernel(const float* __res
         if (r0 + lane < count)
             for (int i = 0; i < slices; ++i)
                 m = max(m, largest[i * count + r0 + lane]);
-        shifts[lane] = row_shift(m);
+        shifts[lane]  = row_shift(m);
+        without[lane] = k0 == 0 && m == 0 ? kZeroRow : 0;
         if (k0 == 0 && r0 + lane < count)
             scale[r0 + lane] = -row_shift(m);
     }
@@ -225,8 +258,13 @@ __global__ __launch_bounds__(kBlock) void pack_columns_kernel(const float* __res
         for (int u = 0; u < 8; ++u)
             v[u] = tile[c + u][r];
         uint16_t* to = out + (r0 + r) * 2 * kp + place_of_half(k0 + c);
-        put_parts(v, shifts[r], to, to + kHalves);
+        if (const int n = put_parts(v, shifts[r], to, to + kHalves))
+            atomicAdd(&without[r], n);
     }
+    __syncthreads();
+    // (few columns lose anything; whole numbers have one sum in any order)
+    if (threadIdx.x < 64 && r0 + lane < count && without[lane])
+        atomicAdd(lost + r0 + lane, without[lane]);
 }
 
 // dz = g act'(z) and its column sums over a slice of the rows, at memory's rate (4096 x 11008 bfloat16: 65 us, 4.2 TB/s;
@@ -418,7 +456,7 @@ struct Plan
     int64_t kp;   // kTiles, float32: length of the rows of halves
     bool big;     // kTiles: 256 x 256, else 128 x 128; kDirect: 128 x 128, else 64 x 128
     int splits;
-    int64_t a_bytes, b_bytes, scale_a, scale_b, partial, total;   // of the workspace
+    int64_t a_bytes, b_bytes, scale_a, scale_b, partial, total;   // of the workspace (scale: scale, lost, columns' maxima)
 };
 
 // Tiles and pieces of the sum for a product of `slices` slices a pass whose values take `bytes`.  What a launch costs, in
@@ -502,8 +540,8 @@ Plan plan_product(const Matrix<T>& a, const Matrix<T>& b)
     {
         p.kp      = (k + kHalves - 1) / kHalves * kHalves;
         p.a_bytes = up256(m * 2 * p.kp * 2), p.b_bytes = up256(n * 2 * p.kp * 2);
-        p.scale_a = up256(m * 4 * (1 + (a.columns ? max_slices(k) : 0)));
-        p.scale_b = up256(n * 4 * (1 + (b.columns ? max_slices(k) : 0)));
+        p.scale_a = up256(m * 4 * (2 + (a.columns ? max_slices(k) : 0)));
+        p.scale_b = up256(n * 4 * (2 + (b.columns ? max_slices(k) : 0)));
     }
     return done();
 }
@@ -524,26 +562,27 @@ int pack(const Matrix<float>& x, int64_t kp, char* to, char* scale, hipStream_t 
     if (x.count == 0 || kp == 0)
         return MIQ_OK;
     int* exponents    = (int*) scale;
-    uint32_t* largest = (uint32_t*) scale + x.count;
+    int* lost         = exponents + x.count;
+    uint32_t* largest = (uint32_t*) lost + x.count;
     if (!x.columns)
     {
         if (x.k <= 2048)
             hipLaunchKernelGGL(pack_rows_kernel<64>, grid_of((x.count + 3) / 4, kBlock), dim3(kBlock), 0, s, x.p, x.ld,
-                               x.count, x.k, kp, (uint16_t*) to, exponents);
+                               x.count, x.k, kp, (uint16_t*) to, exponents, lost);
         else
             hipLaunchKernelGGL(pack_rows_kernel<256>, grid_of(x.count, kBlock), dim3(kBlock), 0, s, x.p, x.ld, x.count,
-                               x.k, kp, (uint16_t*) to, exponents);
+                               x.k, kp, (uint16_t*) to, exponents, lost);
         MIQ_CHECK_LAUNCH();
         return MIQ_OK;
     }
     const int64_t slices = max_slices(x.k);
     hipLaunchKernelGGL(column_max_kernel, dim3((unsigned) ((x.count + 255) / 256), (unsigned) slices), dim3(kBlock), 0, s,
-                       x.p, x.ld, x.k, x.count, (x.k + slices - 1) / slices, largest);
+                       x.p, x.ld, x.k, x.count, (x.k + slices - 1) / slices, largest, lost);
     MIQ_CHECK_LAUNCH();
     const int64_t tiles = ((x.count + 63) / 64) * ((kp + 63) / 64);
     MIQ_CHECK_ARG(tiles * kBlock <= UINT32_MAX, "an operand has too many tiles");
     hipLaunchKernelGGL(pack_columns_kernel, dim3((unsigned) tiles), dim3(kBlock), 0, s, x.p, x.ld, x.k, x.count, kp,
-                       largest, (int) slices, (uint16_t*) to, exponents);
+                       largest, (int) slices, (uint16_t*) to, exponents, lost);
     MIQ_CHECK_LAUNCH();
     return MIQ_OK;
 }
@@ -699,6 +738,8 @@ int product(const Matrix<T>& a, const Matrix<T>& b, const T* bias, const T* resi
         p.b       = {(const uint16_t*) pb, 2 * plan.kp, b.count};
         p.k       = plan.kp;
         p.scale_a = (const int*) sa, p.scale_b = (const int*) sb;
+        p.plain_a = {a.p, a.ld, a.columns}, p.plain_b = {b.p, b.ld, b.columns};
+        p.length  = a.k;
         p.partial = (float*) (sb + plan.scale_b);
         return launch_product<T, ACT, false, false>(p, plan.big, s);
     }

@@ -407,6 +407,14 @@ __device__ __forceinline__ void finish4(const Epilogue<float>& e, int64_t r, int
     store4(e.c + at, left, z);
 }
 
+// A float32 operand as it lies
+struct Plain
+{
+    const float* p;
+    int64_t ld;
+    bool columns;
+};
+
 template <typename T>
 struct Product
 {
@@ -415,8 +423,10 @@ struct Product
     int tiles_m, tiles_n;
     int splits;            // the sum over k is cut into this many pieces, whose results go to `partial`
     float* partial;        // [splits][m][n]
-    const int* scale_a;    // float32: exponents of the rows' scales (see split_rows_kernel)
+    const int* scale_a;    // float32: exponents of the rows' scales and, behind them, what the rows lost (pack_rows_kernel)
     const int* scale_b;
+    Plain plain_a, plain_b;   // float32: what the halves were made from
+    int64_t length;           // float32: of the sum, not padded
     Epilogue<T> e;
 };
 

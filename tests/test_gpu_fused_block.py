@@ -411,6 +411,57 @@ def test_linear_of_float32_far_from_one(fused, rows):
         assert not fused.linear(torch.zeros(rows, 64, device="cuda"), tiny).any()
 
 
+# float32 products of these sizes are formed from halves, forward and backward: rows of halves from registers and from longer
+# rows, from columns, odd sizes, 128 x 128 and 256 x 256 tiles, sums in pieces
+HALVES = [(2048, 2100, 2048), (1500, 4100, 2049), (1024, 16384, 1024), (3000, 3001, 2900)]
+
+
+@pytest.mark.parametrize("rows,k,n", HALVES)
+def test_linear_of_large_float32_products(fused, rows, k, n):
+    check_linear(fused, *linear_case(rows, k, n, torch.float32, True), "gelu")
+
+
+@pytest.mark.parametrize("rows,k,n", HALVES)
+@pytest.mark.parametrize("outlier", [1e4, 1e6, 1e8, 1e10, 1e13, 1e16])
+def test_linear_of_large_float32_products_with_outliers(fused, rows, k, n, outlier):
+    """Values of very different magnitudes in a row, the largest of which meet zeros: what is left of the sum is of the small
+    ones, which have to be there."""
+    x, w, b, res, g = linear_case(rows, k, n, torch.float32, False)
+    x[::2, 0], x[1::3, k - 1] = outlier, -outlier              # features that many outputs do not look at
+    w[::2, 0], w[1::2, k - 1], w[::3, k - 1] = 0, 0, 0
+    g[3] *= outlier                                            # a row with a huge gradient, where x is zeros
+    x[3] = 0
+    g[:, n // 2] *= outlier                                    # an output with one, whose weights are zeros
+    w[n // 2] = 0
+    check_linear(fused, x, w, b, None, g, "none")
+    lone = torch.zeros(k, k, device="cuda")                    # every output looks at one feature
+    lone[torch.arange(k), torch.randperm(k, generator=torch.Generator().manual_seed(1))] = 1
+    if k >= 2048:
+        want = x.double() @ lone.double().t()
+        with torch.no_grad():
+            assert_within(fused.linear(x, lone), want, (k + 6) * U * want.abs(), "one feature each")
+
+
+@pytest.mark.parametrize("rows,k,n", HALVES)
+def test_linear_of_large_float32_products_with_infinities(fused, rows, k, n):
+    """Infinities meet weights that are nothing beside the others of their row."""
+    x, w, _, _, _ = linear_case(rows, k, n, torch.float32, False)
+    good = fused.linear(x, w)
+    small = torch.logspace(-37, 0, n, device="cuda") * torch.where(torch.arange(n, device="cuda") % 3 == 0, -1.0, 1.0)
+    w[:, 3] = small
+    w[5, 3] = 0
+    x[:, 3] = 0
+    x[1, 3], x[2, 3], x[4, 7] = float("inf"), -float("inf"), float("nan")
+    y = fused.linear(x, w)
+    want = small.sign() * float("inf")
+    want[5] = float("nan")                                     # an infinity times nothing
+    for got, e in ((y[1], want), (y[2], -want)):
+        assert torch.equal(torch.isnan(got), torch.isnan(e)) and torch.equal(got.nan_to_num(0), e.nan_to_num(0))
+    assert torch.isnan(y[4]).all()
+    rest = [0, 3, *range(5, rows)]
+    assert torch.isfinite(y[rest]).all() and torch.isfinite(good).all()
+
+
 def test_linear_shapes_strides_and_alignment(fused):
     for dtype in DTYPES:
         for k, n in ((64, 72), (65, 71), (256, 264)):
