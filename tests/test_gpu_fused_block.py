@@ -411,6 +411,43 @@ def test_linear_of_float32_far_from_one(fused, rows):
         assert not fused.linear(torch.zeros(rows, 64, device="cuda"), tiny).any()
 
 
+# bfloat16 products of these sizes take 256 x 256 tiles, forward and backward: whole tiles, sums in two pieces, and sizes that
+# leave 1, 8 and 63 values in the last slice of 64 and in the last tile
+@pytest.mark.parametrize("rows,k,n,act", [(4096, 4096, 4096, "gelu"), (4096, 1025, 4096, "none"), (4033, 4040, 4095, "silu"),
+                                          (2055, 5000, 5001, "gelu_tanh")])
+def test_linear_of_large_bfloat16_products(fused, rows, k, n, act):
+    check_linear(fused, *linear_case(rows, k, n, torch.bfloat16, True), act)
+
+
+def test_linear_of_large_bfloat16_products_with_bad_rows(fused):
+    x, w, b, _, _ = linear_case(4033, 4040, 4095, torch.bfloat16, False)
+    good = fused.linear(x, w, b)
+    bad = [0, 255, 1000, 4032]
+    x[0, 0], x[255, 4039], x[1000, 64], x[4032, 2000] = float("nan"), float("inf"), -float("inf"), float("nan")
+    y = fused.linear(x, w, b)
+    keep = torch.ones(4033, dtype=torch.bool, device="cuda")
+    keep[bad] = False
+    assert torch.equal(y[keep], good[keep])
+    assert torch.isnan(y[0]).all() and torch.isnan(y[4032]).all()
+    for r, c, sign in ((255, 4039, 1), (1000, 64, -1)):
+        want = torch.sign(w[:, c].float()) * sign * float("inf")   # (a weight of 0 makes it NaN, here as there)
+        assert torch.equal(torch.isnan(y[r]), torch.isnan(want))
+        assert torch.equal(y[r].float().nan_to_num(0), want.nan_to_num(0))
+
+
+def test_linear_offsets_past_32_bits_in_large_tiles(fused):
+    rows, k, n = 70000, 1024, 65536                            # 4.6e9 outputs
+    x = torch.zeros(rows, k, dtype=torch.bfloat16, device="cuda")
+    at = [0, 1, 65535, rows - 300, rows - 2, rows - 1]
+    x[at] = randn(len(at), k, dtype=torch.bfloat16, seed=1)
+    w = randn(n, k, dtype=torch.bfloat16, seed=2, scale=1 / 32)
+    y = fused.linear(x, w)
+    want, tol = x[at].double() @ w.double().t(), (k + 6) * U * (x[at].double().abs() @ w.double().abs().t())
+    assert_within(y[at], want, tol + 2 ** -8 * (want.abs() + tol), "y")
+    y[at] = 0
+    assert not y.any()
+
+
 # float32 products of these sizes are formed from halves, forward and backward: rows of halves from registers and from longer
 # rows, from columns, odd sizes, 128 x 128 and 256 x 256 tiles, sums in pieces
 HALVES = [(2048, 2100, 2048), (1500, 4100, 2049), (1024, 16384, 1024), (3000, 3001, 2900)]
