@@ -512,7 +512,8 @@ Plan plan_product(const Matrix<T>& a, const Matrix<T>& b)
         p.way = Way::kFewRows;
         return done();
     }
-    if (!a.columns && b.columns && m <= 16 && (kF32 || !b.whole()))
+    // (by the row's length, not by where b starts: a sum's order is the same wherever its operands lie)
+    if (!a.columns && b.columns && m <= 16 && (kF32 || padded<T>(b.ld) != b.ld))
     {
         // about 2048 waves in blocks of 8; pieces of k of 128 at least
         const int64_t wide = (n + 16 * IOTraits<T>::VEC - 1) / (16 * IOTraits<T>::VEC);

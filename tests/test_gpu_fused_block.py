@@ -527,6 +527,29 @@ def test_linear_shapes_strides_and_alignment(fused):
             assert all(torch.equal(i, j) for i, j in zip(p, q))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [1, 5, 16, 17])
+@pytest.mark.parametrize("k,n", [(64, 72), (4096, 1000), (520, 4096), (65, 71)])
+def test_linear_of_few_rows_does_not_depend_on_where_tensors_start(fused, dtype, rows, k, n):
+    """Every operand in turn starts one element into its storage: the same values, to the bit."""
+    x, w, b, res, g = linear_case(rows, k, n, dtype, True)
+
+    def shifted(t):
+        flat = torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")[1:]
+        return flat.copy_(t.reshape(-1)).view(t.shape)
+
+    def step(x, w, b, res, g):
+        leaves = [t.detach().requires_grad_() for t in (x, w, b, res)]
+        y = fused.linear(leaves[0], leaves[1], leaves[2], "silu", leaves[3])
+        return [y.detach(), *torch.autograd.grad(y, leaves, g)]
+
+    want = step(x, w, b, res, g)
+    for one in range(5):
+        args = [shifted(t) if i == one else t for i, t in enumerate((x, w, b, res, g))]
+        for name, p, q in zip(("y", "dx", "dweight", "dbias", "dresidual"), step(*args), want):
+            assert torch.equal(p, q), (one, name)
+
+
 def test_linear_results_do_not_change_from_run_to_run(fused):
     for dtype in DTYPES:
         x, w, b, res, g = linear_case(700, 520, 392, dtype, True)
