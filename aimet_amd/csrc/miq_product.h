@@ -132,6 +132,10 @@ struct Loader
         edge   = first + COUNT > o.count;
     }
 
+    // (m0 is listed as written, though the compiler says that it keeps no value there across statements: what it puts into m0
+    // for an instruction of its own then stays behind the asm or before it)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
     // Starts load i of a slice with `left` values of k remaining (from its first) into `lds` (an address in LDS).  INSIDE: all of the slice is
     // inside of the operand; otherwise what is not is read as zeros.
     template <bool INSIDE>
@@ -142,7 +146,7 @@ struct Loader
         if (INSIDE)
             asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to),
                          "v"(offset_of(i, wave, lane)), "s"(p + i * apart)
-                         : "memory");
+                         : "m0", "memory");
         else
         {
             const int r   = (i * WAVES + wave) * kAtOnce + lane / kChunks;
@@ -151,9 +155,11 @@ struct Loader
             const char* from =
                 in ? (const char*) (p + i * apart) + offset_of(i, wave, lane) : (const char*) &g_zero16;
             asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from)
-                         : "memory");
+                         : "m0", "memory");
         }
     }
+#pragma clang diagnostic pop
+
     __device__ __forceinline__ void load(const Operand<E>& o, int64_t first, uint32_t lds, int wave, int lane,
                                          int64_t left)
     {
