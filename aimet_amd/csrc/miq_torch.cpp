@@ -269,7 +269,7 @@ variable_list not_twice(variable_list grads)
 
 // A leaf's gradient is accumulated on the stream of the first graph that is still alive.  Where that is an eager one of the
 // default stream, a backward pass under capture would have the default stream wait for a captured one, which ends the
-// process: refused beforehand.
+// process: refused beforehand.  Only leaves that this pass wants a gradient of are looked at.
 void refuse_eager_leaves_under_capture()
 {
     if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None)
@@ -277,11 +277,14 @@ void refuse_eager_leaves_under_capture()
     const auto node = torch::autograd::get_current_node();
     if (!node)
         return;
-    for (const torch::autograd::Edge& edge : node->next_edges())
+    for (size_t i = 0; i < node->num_outputs(); ++i)
     {
-        if (!edge.function || edge.function->name() != "torch::autograd::AccumulateGrad")
+        if (!node->task_should_compute_output(i))
             continue;
-        const std::optional<c10::Stream> stream = edge.function->stream();
+        torch::autograd::Node* next = node->next_edge(i).function.get();
+        if (next->name() != "torch::autograd::AccumulateGrad")
+            continue;
+        const std::optional<c10::Stream> stream = next->stream();
         TORCH_CHECK(!stream || stream->id() != 0, "a backward pass cannot be captured into a graph while an eager autograd graph "
                     "of the same leaves, made on the default stream, is alive: delete its outputs first");
     }

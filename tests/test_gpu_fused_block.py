@@ -712,6 +712,30 @@ def test_capture_beside_a_living_eager_graph_is_refused(fused, norm):
         assert all(torch.equal(p, q) for p, q in zip(got, want))
 
 
+@pytest.mark.parametrize("norm", [True, False])
+def test_capture_beside_a_living_eager_graph_of_leaves_without_a_gradient(fused, norm):
+    """What lives on the default stream is a graph of the weight and the bias, and this pass wants neither's gradient."""
+    x, w, b, _, g = linear_case(8, 64, 64, torch.float32, False)
+    w, b = (w[0].contiguous() if norm else w).requires_grad_(), b.requires_grad_()
+    leaf = x.clone().requires_grad_()
+
+    def forward(t):
+        return fused.layer_norm(t, 64, w, b) if norm else fused.linear(t, w, b)
+
+    want, = torch.autograd.grad(forward(leaf), leaf, g)
+    want_w, = torch.autograd.grad(forward(leaf), w, g)
+    torch.cuda.synchronize()
+    alive = forward(x)                                         # of w and b alone
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got, = torch.autograd.grad(forward(leaf), leaf, g)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+    assert torch.equal(torch.autograd.grad(alive, w, g)[0], want_w)
+
+
 def test_two_streams_at_once(fused):
     """Calls that overlap share no scratch memory."""
     cases = [linear_case(900, 512, 520, torch.float32, False, seed=s) for s in (1, 2)]
