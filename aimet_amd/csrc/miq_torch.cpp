@@ -269,7 +269,8 @@ variable_list not_twice(variable_list grads)
 
 // A leaf's gradient is accumulated on the stream of the first graph that is still alive.  Where that is an eager one of the
 // default stream, a backward pass under capture would have the default stream wait for a captured one, which ends the
-// process: refused beforehand.  Only leaves that this pass wants a gradient of are looked at.
+// process: refused beforehand.  Only leaves that this pass wants a gradient of are looked at, also those behind the casts that
+// autocast makes here.
 void refuse_eager_leaves_under_capture()
 {
     if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None)
@@ -282,6 +283,8 @@ void refuse_eager_leaves_under_capture()
         if (!node->task_should_compute_output(i))
             continue;
         torch::autograd::Node* next = node->next_edge(i).function.get();
+        while (next->name() == "ToCopyBackward0" && next->num_outputs() == 1 && next->task_should_compute_output(0))
+            next = next->next_edge(0).function.get();
         if (next->name() != "torch::autograd::AccumulateGrad")
             continue;
         const std::optional<c10::Stream> stream = next->stream();

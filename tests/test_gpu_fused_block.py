@@ -736,6 +736,37 @@ def test_capture_beside_a_living_eager_graph_of_leaves_without_a_gradient(fused,
     assert torch.equal(torch.autograd.grad(alive, w, g)[0], want_w)
 
 
+@pytest.mark.parametrize("norm", [True, False])
+def test_capture_under_autocast_beside_a_living_eager_graph_is_refused(fused, norm):
+    """Autocast puts a cast between the function and the leaf."""
+    x, w, b, _, g = linear_case(8, 64, 64, torch.bfloat16 if norm else torch.float32, False)
+    leaf, w = x.clone().requires_grad_(), (w[0].contiguous() if norm else w).requires_grad_()
+
+    def forward():
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            return fused.layer_norm(leaf, 64, w) if norm else fused.linear(leaf, w)
+
+    g = torch.ones_like(forward())
+    want = torch.autograd.grad(forward(), [leaf, w], g)
+    torch.cuda.synchronize()
+    alive = forward()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = forward()
+        with pytest.raises(RuntimeError, match="eager autograd graph"):
+            torch.autograd.grad(y, [leaf, w], g)
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(alive, [leaf, w], g), want))
+    del y, alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(forward(), [leaf, w], g)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
 def test_two_streams_at_once(fused):
     """Calls that overlap share no scratch memory."""
     cases = [linear_case(900, 512, 520, torch.float32, False, seed=s) for s in (1, 2)]
