@@ -182,19 +182,25 @@ def _load():
 lib = _load()
 
 
-def _load_native():
-    """The torch binding of some of the entry points (csrc/miq_torch.cpp).  torch comes first: it loads the libraries
-    the binding is linked against."""
-    import torch  # noqa: F401  pylint: disable=import-outside-toplevel,unused-import
-    try:
-        from . import _native  # pylint: disable=import-outside-toplevel
-    except ImportError as exc:
-        raise ImportError(f"aimet_amd/_native.so cannot be loaded ({exc}). Build it with `make -C aimet_amd/csrc`.") \
-            from exc
-    return _native
+class _Native:
+    """The torch binding of some of the entry points (csrc/miq_torch.cpp), loaded when a function of it is first wanted:
+    everything else needs libmiq.so alone.  torch comes first: it loads the libraries the binding is linked against."""
+
+    def __getattr__(self, name):
+        if name.startswith("__"):
+            raise AttributeError(name)
+        import torch  # noqa: F401  pylint: disable=import-outside-toplevel,unused-import
+        try:
+            from . import _native  # pylint: disable=import-outside-toplevel
+        except ImportError as exc:
+            raise ImportError(f"aimet_amd/_native.so cannot be loaded ({exc}). Build it with `make -C aimet_amd/csrc`.") \
+                from exc
+        function = getattr(_native, name)
+        setattr(self, name, function)          # from here on an ordinary attribute
+        return function
 
 
-native = _load_native()
+native = _Native()
 
 
 def check(status):

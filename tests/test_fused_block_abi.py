@@ -2,6 +2,7 @@
 comes before the first use of the GPU."""
 import ctypes
 import os
+import shutil
 import subprocess
 import sys
 
@@ -103,3 +104,30 @@ def test_functions_refuse_before_any_launch():
         fused.FusedLinear(8, 6, activation="swish")
     with pytest.raises(ValueError):
         fused.FusedLinear.from_linear(torch.nn.Linear(8, 6), "swish")
+
+
+def test_only_the_functions_of_the_torch_binding_need_it(tmp_path):
+    """A tree without _native.so: the package imports and quantizes, layer_norm() and linear() say what is missing."""
+    package = tmp_path / "aimet_amd"
+    shutil.copytree(os.path.join(ROOT, "aimet_amd"), package,
+                    ignore=shutil.ignore_patterns("*.so", "*.o", "__pycache__", "csrc"))
+    os.symlink(os.path.join(ROOT, "aimet_amd", "libmiq.so"), package / "libmiq.so")
+    code = ("import sys; sys.path.insert(0, %r)\n"
+            "from aimet_amd import _lib\n"
+            "assert _lib.__file__.startswith(%r) and _lib.lib.miq_version() >= 1\n"
+            "import aimet_amd.common.libpymo as pymo\n"
+            "assert 'torch' not in sys.modules\n"
+            "import torch, aimet_amd.v1.quantsim, aimet_amd.v2.quantsim\n"
+            "from aimet_amd.v2.nn import fused\n"
+            "fused.FusedLinear(8, 6)\n"
+            "for call in (lambda: fused.linear(torch.zeros(4, 8), torch.zeros(6, 8)),\n"
+            "             lambda: fused.layer_norm(torch.zeros(4, 8), 8)):\n"
+            "    try:\n"
+            "        call()\n"
+            "    except ImportError as e:\n"
+            "        assert '_native.so' in str(e)\n"
+            "    else:\n"
+            "        raise AssertionError('not refused')\n" % (str(tmp_path), str(tmp_path)))
+    run = subprocess.run([sys.executable, "-c", code], stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True, check=False,
+                         cwd=str(tmp_path))
+    assert run.returncode == 0, run.stderr
