@@ -8,7 +8,9 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/TracerMode.h>
 #include <ATen/autocast_mode.h>
+#include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/core/grad_mode.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
@@ -18,6 +20,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/object_ptr.h>
+#include <torch/library.h>
 
 #include "../../include/miq.h"
 
@@ -399,8 +402,9 @@ Tensor cast(const Tensor& t, at::ScalarType type)
     return t.defined() && t.is_floating_point() && t.scalar_type() != at::kDouble && t.scalar_type() != type ? t.to(type) : t;
 }
 
-Tensor layer_norm(Tensor x, at::IntArrayRef shape, Tensor weight, Tensor bias, double eps)
+Tensor layer_norm(const Tensor& x_, at::IntArrayRef shape, const Tensor& weight_, const Tensor& bias_, double eps)
 {
+    Tensor x = x_, weight = weight_, bias = bias_;
     const int64_t dims = (int64_t) shape.size();
     TORCH_CHECK(dims >= 1 && x.dim() >= dims && x.sizes().slice(x.dim() - dims) == shape, "normalized_shape ", shape,
                 " is not the end of the input's shape ", x.sizes());
@@ -418,8 +422,9 @@ Tensor layer_norm(Tensor x, at::IntArrayRef shape, Tensor weight, Tensor bias, d
     return layer_norm_fwd(x, width, weight, bias, eps, nullptr);
 }
 
-Tensor linear(Tensor x, Tensor weight, Tensor bias, int activation, Tensor residual)
+Tensor linear(const Tensor& x_, const Tensor& weight_, const Tensor& bias_, int64_t activation, const Tensor& residual_)
 {
+    Tensor x = x_, weight = weight_, bias = bias_, residual = residual_;
     if (at::autocast::is_autocast_enabled(at::kCUDA))
     {
         const at::ScalarType type = at::autocast::get_autocast_dtype(at::kCUDA);
@@ -427,9 +432,49 @@ Tensor linear(Tensor x, Tensor weight, Tensor bias, int activation, Tensor resid
     }
     no_forward_mode({&x, &weight, &bias, &residual});
     if (differentiates({&x, &weight, &bias, &residual}))
-        return LinearNode::apply(x, weight, given(bias), given(residual), (int64_t) activation,
+        return LinearNode::apply(x, weight, given(bias), given(residual), activation,
                                  differentiates({&x, &weight, &bias}));
-    return linear_fwd(x, weight, bias, activation, residual, nullptr);
+    return linear_fwd(x, weight, bias, (int) activation, residual, nullptr);
+}
+
+// ------------------------------------------------------------------------------------------------------- tracing
+// torch.jit.trace records what goes through the dispatcher.  Of the calls above that is only the allocation of the result, so
+// a traced model would return memory that nobody wrote.  While a trace is on, layer_norm() and linear() therefore go through
+// the dispatcher as well, as operators of their own; at other times they do not pay for it.
+Tensor layer_norm_operator(const Tensor& input, at::IntArrayRef shape, const std::optional<Tensor>& weight,
+                           const std::optional<Tensor>& bias, double eps)
+{
+    return layer_norm(input, shape, weight.value_or(Tensor()), bias.value_or(Tensor()), eps);
+}
+
+Tensor linear_operator(const Tensor& input, const Tensor& weight, const std::optional<Tensor>& bias, int64_t activation,
+                       const std::optional<Tensor>& residual)
+{
+    return linear(input, weight, bias.value_or(Tensor()), activation, residual.value_or(Tensor()));
+}
+
+bool traced()
+{
+    return at::tracer::impl::is_dispatch_enabled();
+}
+
+Tensor recorded_layer_norm(const Tensor& x, at::IntArrayRef shape, const Tensor& weight, const Tensor& bias, double eps)
+{
+    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("aimet_amd::layer_norm", "")
+                               .typed<decltype(layer_norm_operator)>();
+    return op.call(x, shape, given(weight), given(bias), eps);
+}
+
+Tensor recorded_linear(const Tensor& x, const Tensor& weight, const Tensor& bias, int64_t activation, const Tensor& residual)
+{
+    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("aimet_amd::linear", "")
+                               .typed<decltype(linear_operator)>();
+    return op.call(x, weight, given(bias), activation, given(residual));
+}
+
+void not_recorded()
+{
+    TORCH_CHECK(!traced(), "this function of aimet_amd is not recorded by a trace: call layer_norm() or linear()");
 }
 
 // ---------------------------------------------------------------------------------------------- Python's side of it
@@ -496,8 +541,9 @@ PyObject* py_layer_norm(PyObject*, PyObject* const* args, Py_ssize_t n)
         for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(items.get()); ++i)
             shape.push_back(integer(PySequence_Fast_GET_ITEM(items.get(), i)));
     }
-    return wrapped(layer_norm(tensor_at(args, 0, "input", false), shape, tensor_at(args, 2, "weight", true),
-                              tensor_at(args, 3, "bias", true), real(args[4])));
+    return wrapped((traced() ? recorded_layer_norm : layer_norm)(tensor_at(args, 0, "input", false), shape,
+                                                                 tensor_at(args, 2, "weight", true),
+                                                                 tensor_at(args, 3, "bias", true), real(args[4])));
     END_HANDLE_TH_ERRORS
 }
 
@@ -505,8 +551,9 @@ PyObject* py_linear(PyObject*, PyObject* const* args, Py_ssize_t n)
 {
     HANDLE_TH_ERRORS
     expect(n, 5);
-    return wrapped(linear(tensor_at(args, 0, "input", false), tensor_at(args, 1, "weight", false),
-                          tensor_at(args, 2, "bias", true), (int) integer(args[3]), tensor_at(args, 4, "residual", true)));
+    return wrapped((traced() ? recorded_linear : linear)(tensor_at(args, 0, "input", false), tensor_at(args, 1, "weight", false),
+                                                         tensor_at(args, 2, "bias", true), integer(args[3]),
+                                                         tensor_at(args, 4, "residual", true)));
     END_HANDLE_TH_ERRORS
 }
 
@@ -514,6 +561,7 @@ PyObject* py_layer_norm_fwd(PyObject*, PyObject* const* args, Py_ssize_t n)
 {
     HANDLE_TH_ERRORS
     expect(n, 6);
+    not_recorded();
     const at::NoGradGuard no_grad;
     Tensor stats;
     const Tensor y = layer_norm_fwd(tensor_at(args, 0, "x", false), integer(args[1]), tensor_at(args, 2, "weight", true),
@@ -527,6 +575,7 @@ PyObject* py_layer_norm_bwd(PyObject*, PyObject* const* args, Py_ssize_t n)
 {
     HANDLE_TH_ERRORS
     expect(n, 8);
+    not_recorded();
     const at::NoGradGuard no_grad;
     const NormGrads g = layer_norm_bwd(tensor_at(args, 0, "x", false), tensor_at(args, 1, "grad", false), integer(args[2]),
                                        tensor_at(args, 3, "weight", true), tensor_at(args, 4, "stats", false),
@@ -539,6 +588,7 @@ PyObject* py_linear_fwd(PyObject*, PyObject* const* args, Py_ssize_t n)
 {
     HANDLE_TH_ERRORS
     expect(n, 6);
+    not_recorded();
     const at::NoGradGuard no_grad;
     Tensor saved;
     const Tensor y = linear_fwd(tensor_at(args, 0, "x", false), tensor_at(args, 1, "weight", false),
@@ -552,6 +602,7 @@ PyObject* py_linear_bwd(PyObject*, PyObject* const* args, Py_ssize_t n)
 {
     HANDLE_TH_ERRORS
     expect(n, 8);
+    not_recorded();
     const at::NoGradGuard no_grad;
     const LinearGrads g = linear_bwd(tensor_at(args, 0, "grad", false), tensor_at(args, 1, "saved", true),
                                      tensor_at(args, 2, "x", false), tensor_at(args, 3, "weight", false),
@@ -566,6 +617,13 @@ PyCFunction as_method(PyObject* (*f)(PyObject*, PyObject* const*, Py_ssize_t))
     return reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(f));
 }
 }   // namespace
+
+TORCH_LIBRARY(aimet_amd, m)
+{
+    m.def("layer_norm(Tensor input, int[] normalized_shape, Tensor? weight, Tensor? bias, float eps) -> Tensor",
+          layer_norm_operator);
+    m.def("linear(Tensor input, Tensor weight, Tensor? bias, int activation, Tensor? residual) -> Tensor", linear_operator);
+}
 
 PyMODINIT_FUNC PyInit__native()
 {

@@ -911,6 +911,38 @@ def test_block_trains_like_its_float64_form(fused, activation):
         assert (a.double() - e).norm() <= 16 * 3 * (2 * math.sqrt(160 + 64) + 8) * U * e.norm()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_traced_modules_compute(fused, dtype):
+    """torch.jit.trace records the calls themselves: on other inputs, of other sizes, forward and backward, also loaded."""
+    import io
+    torch.manual_seed(0)
+    block = Block(fused, activation="silu").to("cuda", dtype)
+    traced = torch.jit.trace(block, randn(3, 64, dtype=dtype, seed=1))
+    kinds = [n.kind() for n in traced.inlined_graph.nodes()]
+    assert kinds.count("aimet_amd::layer_norm") == 1 and kinds.count("aimet_amd::linear") == 2
+    buffer = io.BytesIO()
+    torch.jit.save(traced, buffer)
+    buffer.seek(0)
+    loaded = torch.jit.load(buffer)
+    for rows in (3, 50, 700):
+        x, g = randn(rows, 64, dtype=dtype, seed=rows), randn(rows, 64, dtype=dtype, seed=rows + 1)
+        want = block(x)
+        wanted = torch.autograd.grad(want, list(block.parameters()), g)
+        for other in (traced, loaded):
+            y = other(x)
+            assert torch.equal(y, want)
+            assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(y, list(other.parameters()), g), wanted))
+
+
+def test_calls_that_a_trace_would_not_record_are_refused(fused):
+    from aimet_amd import ops
+    x, w, _, _, _ = linear_case(4, 32, 24, torch.float32, False)
+    for f in (lambda t: ops.linear_fwd(t, w)[0], lambda t: ops.layer_norm_fwd(t, 32)[0],
+              lambda t: ops.linear_bwd(t @ w.t(), None, t, w)[0]):
+        with pytest.raises(RuntimeError, match="trace"):
+            torch.jit.trace(f, x)
+
+
 def test_modules_are_made_from_torch_modules_and_pickle(fused):
     import copy
     import pickle
