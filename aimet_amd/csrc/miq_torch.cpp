@@ -13,6 +13,7 @@
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/core/grad_mode.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -75,6 +76,13 @@ void no_forward_mode(std::initializer_list<const Tensor*> tensors)
     for (const Tensor* t : tensors)
         TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(),
                     "aimet_amd kernels are not differentiated in forward mode: got a dual tensor");
+}
+
+// make_fx records torch's own operators below autograd, where nothing of a call here but its allocations goes by
+void no_proxies()
+{
+    TORCH_CHECK(!c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY),
+                "aimet_amd kernels cannot be recorded into a graph of torch's operators");
 }
 
 bool is_bf16(const Tensor& x)
@@ -414,6 +422,7 @@ Tensor layer_norm(const Tensor& x_, at::IntArrayRef shape, const Tensor& weight_
     if (at::autocast::is_autocast_enabled(at::kCUDA))
         x = cast(x, at::kFloat), weight = cast(weight, at::kFloat), bias = cast(bias, at::kFloat);
     no_forward_mode({&x, &weight, &bias});
+    no_proxies();
     int64_t width = 1;
     for (const int64_t d : shape)
         width *= d;
@@ -431,6 +440,7 @@ Tensor linear(const Tensor& x_, const Tensor& weight_, const Tensor& bias_, int6
         x = cast(x, type), weight = cast(weight, type), bias = cast(bias, type), residual = cast(residual, type);
     }
     no_forward_mode({&x, &weight, &bias, &residual});
+    no_proxies();
     if (differentiates({&x, &weight, &bias, &residual}))
         return LinearNode::apply(x, weight, given(bias), given(residual), activation,
                                  differentiates({&x, &weight, &bias}));
@@ -474,6 +484,7 @@ Tensor recorded_linear(const Tensor& x, const Tensor& weight, const Tensor& bias
 
 void not_recorded()
 {
+    no_proxies();
     TORCH_CHECK(!traced(), "this function of aimet_amd is not recorded by a trace: call layer_norm() or linear()");
 }
 

@@ -943,6 +943,28 @@ def test_calls_that_a_trace_would_not_record_are_refused(fused):
             torch.jit.trace(f, x)
 
 
+def test_graphs_of_torchs_operators_are_refused(fused):
+    """make_fx would hold the allocation of the result and nothing that writes to it; what else sees no memory raises too."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from aimet_amd import ops
+    x, w, _, _, _ = linear_case(4, 32, 24, torch.float32, False)
+    leaf = x.clone().requires_grad_()
+    for f in (lambda t: fused.linear(t, w), lambda t: fused.layer_norm(t, 32), lambda t: ops.linear_fwd(t, w)[0],
+              lambda t: ops.layer_norm_fwd(t, 32)[0]):
+        with pytest.raises(RuntimeError, match="recorded"):
+            make_fx(f)(x)
+        with pytest.raises(RuntimeError, match="recorded"):
+            make_fx(f)(leaf)
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(f)(x.view(2, 2, 32))
+        with FakeTensorMode(allow_non_fake_inputs=True) as mode, pytest.raises(RuntimeError):
+            f(mode.from_tensor(x))
+    for f in (lambda t: fused.linear(t, w), lambda t: fused.layer_norm(t, 32)):
+        with pytest.raises(RuntimeError):
+            torch.func.grad(lambda t: f(t).sum())(x)           # pylint: disable=cell-var-from-loop
+
+
 def test_modules_are_made_from_torch_modules_and_pickle(fused):
     import copy
     import pickle
