@@ -44,6 +44,20 @@ __device__ __forceinline__ Parts parts_of(const float* v)
     return {__builtin_bit_cast(s8v, p), __builtin_bit_cast(s8v, q), __builtin_bit_cast(s8v, r)};
 }
 
+// What 8 values are to a sum that is not finite: bfloat16 that are NaN, infinite, zero or neither as they are, and of their
+// sign.  (The upper half alone of a NaN may be an infinity, and that of the smallest values is zero.)
+__device__ __forceinline__ s8v kinds_of(const float* v)
+{
+    s8v p;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+    {
+        const uint32_t u = __float_as_uint(v[i]), m = u & 0x7fffffffu, sign = u >> 16 & 0x8000u;
+        p[i] = (short) (m > 0x7f800000u ? 0x7fc0u : m != 0 && m < 0x00800000u ? sign | 0x0080u : u >> 16);
+    }
+    return p;
+}
+
 // 8 values of k (from 8 (lane / 16)) of row lane % 16 of a float32 slice of 32
 template <bool COLUMNS, int CHUNKS>
 struct DirectReader
@@ -149,17 +163,23 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void direct_kernel(const DirectProd
             {
                 float v[8];
                 rb.read(sb, j, v);
-                fb[j] = parts_of(v);
+                if constexpr (decltype(whole)::value)
+                    fb[j] = parts_of(v);
+                else
+                    fb[j].p = kinds_of(v);
             }
 #pragma unroll
             for (int i = 0; i < FM; ++i)
             {
                 float v[8];
                 ra.read(sa, i, v);
-                const Parts fa = parts_of(v);
+                Parts fa;
                 constexpr auto kind = std::true_type();
-                if constexpr (decltype(whole)::value)
+                if constexpr (!decltype(whole)::value)
+                    fa.p = kinds_of(v);
+                else
                 {
+                    fa = parts_of(v);
 #pragma unroll
                     for (int j = 0; j < FN; ++j)
                         acc[i][j] = mfma_16x16x32(fb[j].p, fa.r, acc[i][j], kind);
@@ -184,8 +204,8 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void direct_kernel(const DirectProd
     };
     sum(std::true_type());
 
-    // An infinity or a NaN has no parts beyond the first: where the sum is not finite, what the first parts alone make of
-    // it is what float32 arithmetic would.  (If that is finite the sum has left float32's range, and stays what it is.)
+    // An infinity or a NaN has no parts beyond the first: where the sum is not finite, it is formed again of kinds_of(), which
+    // makes of it what float32 arithmetic would.  (If that is finite the sum has left float32's range, and stays what it is.)
     bool finite = true;
 #pragma unroll
     for (int i = 0; i < FM; ++i)

@@ -499,6 +499,27 @@ def test_linear_of_large_float32_products_with_infinities(fused, rows, k, n):
     assert torch.isfinite(y[rest]).all() and torch.isfinite(good).all()
 
 
+@pytest.mark.parametrize("rows,k,n", [(7, 200, 264), (300, 200, 264), (700, 520, 392), (2048, 2100, 2048)])
+def test_linear_of_float32_with_every_nan_and_the_smallest_values(fused, rows, k, n):
+    """Few rows, products of middling size, whole and in pieces, and large ones.  A NaN is one whatever its payload; an
+    infinity times the smallest value there is, is an infinity."""
+    x, w, _, _, _ = linear_case(rows, k, n, torch.float32, False)
+    payloads = [0x7f800001, 0x7f80ffff, 0x7f810000, 0x7fc00000, -0x7fffff, -0x400000]     # the last two are negative
+    for i, bits in enumerate(payloads[:rows - 3]):
+        x[i + 3].view(torch.int32)[5 * i] = bits
+    small = torch.tensor([1e-45, -1e-45, 1e-42, -1e-40, 1e-38, -1e-37, 0.0, 1.0], device="cuda").repeat(n // 8 + 1)[:n]
+    w[:, 1] = small
+    x[:, 1] = 0
+    x[1, 1], x[2, 1] = float("inf"), -float("inf")
+    y = fused.linear(x, w)
+    bad = min(len(payloads), rows - 3)
+    assert torch.isnan(y[3:3 + bad]).all()
+    want = torch.where(small == 0, torch.full_like(small, float("nan")), small.sign() * float("inf"))
+    for got, e in ((y[1], want), (y[2], -want)):
+        assert torch.equal(torch.isnan(got), torch.isnan(e)) and torch.equal(got.nan_to_num(0), e.nan_to_num(0))
+    assert torch.isfinite(y[0]).all() and torch.isfinite(y[3 + bad:]).all()
+
+
 def test_linear_shapes_strides_and_alignment(fused):
     for dtype in DTYPES:
         for k, n in ((64, 72), (65, 71), (256, 264)):
