@@ -71,8 +71,9 @@ __device__ __forceinline__ float act_slope(float z)
     }
     if (ACT == MIQ_ACT_GELU_TANH)
     {
-        const float s = sigmoid_fast(2.f * kGeluTanhA * (z + kGeluTanhB * z * z * z));
-        return s + z * s * (1.f - s) * 2.f * kGeluTanhA * (1.f + 3.f * kGeluTanhB * z * z);
+        const float s = sigmoid_fast(2.f * kGeluTanhA * (z + kGeluTanhB * z * z * z)), d = s * (1.f - s);
+        // (far out d is 0, and z^2 may be infinite)
+        return d == 0.f ? s : s + z * d * 2.f * kGeluTanhA * (1.f + 3.f * kGeluTanhB * z * z);
     }
     return 1.f;
 }

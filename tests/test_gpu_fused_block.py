@@ -342,6 +342,22 @@ def test_linear_activations(fused, dtype, act, rows, k, n):
     check_linear(fused, *linear_case(rows, k, n, dtype, True, seed=50, bias=False), act)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ACTIVATIONS)
+def test_linear_activations_far_out(fused, dtype, act):
+    """Up to the ends of the range every activation is 0 or z there, and its slope 0 or 1."""
+    z = torch.tensor([20.0, 1e3, 1e6, 1e13, 1e19, 6e19, 1e25, 1e38, 3e38], device="cuda")
+    x = torch.cat([z, -z]).to(dtype)[:, None].requires_grad_()
+    w = torch.ones(1, 1, dtype=dtype, device="cuda")
+    y = fused.linear(x, w, None, act)
+    slope, = torch.autograd.grad(y, x, torch.ones_like(y))
+    flat = x.detach() > 0 if act != "none" else torch.ones_like(x, dtype=torch.bool)
+    # SiLU is the slowest to get there: at 20 it is off by 20 e^-20 = 4.1e-8 and its slope by 19 e^-20 = 4e-8, which is less
+    # than half a step of 1; below, what is left of the zeros
+    assert_within(y.detach(), torch.where(flat, x.detach().double(), 0.0), torch.full_like(x, 5e-8, dtype=torch.float64), "y")
+    assert_within(slope, flat.double(), torch.full_like(x, 5e-8, dtype=torch.float64) + 2 * U, "slope")
+
+
 def test_linear_without_rows_or_features(fused):
     for dtype in DTYPES:
         for act in ("none", "silu"):
