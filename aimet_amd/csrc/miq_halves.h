@@ -4,8 +4,8 @@
 // A slice is 32 values of k, coarse halves and then fine ones: 128 bytes of a row, so that a slice is loaded and its
 // fragments are read as those of 64 values of a 16-bit operand are ("half" 0 and 1 of the slice).  Every fragment read
 // from LDS is multiplied three times for two here, where LDS reads, not the matrix unit, bound the 16-bit product.
-// [4096, 4096] x [4096, 4096]^T: 270 us (1530 TFLOP/s through the matrix unit, 510 of float32), and 50 to make the halves;
-// as three passes of the 16-bit product 328.  The relative error of the result is 2.5e-7 to 8e-7 there, where float32 matrix
+// [4096, 4096] x [4096, 4096]^T: 305 us (1350 TFLOP/s through the matrix unit, 450 of float32), and 53 to make the halves.
+// Three passes of the 16-bit product take a fifth longer.  The relative error of the result is 2.5e-7 to 8e-7 there, where float32 matrix
 // instructions have 7e-7 to 1.3e-6.
 #ifndef MIQ_HALVES_H
 #define MIQ_HALVES_H

@@ -270,6 +270,10 @@ __global__ __launch_bounds__(kBlock) void pack_columns_kernel(const float* __res
 // dz = g act'(z) and its column sums over a slice of the rows, at memory's rate (4096 x 11008 bfloat16: 65 us, 4.2 TB/s;
 // 4096 x 4096 float32: 41 us, 4.9 TB/s): a thread takes 8 columns, 32 threads across and 8 rows at
 // a time.  dz may be null for ACT none; its rows are `ld` values apart, zeros behind the last column.
+// For bfloat16 tensors dz is rounded to bfloat16 here (the column sums are of what it was before), for it is a factor of two
+// products whose matrix instructions take nothing wider beside a bfloat16: in two parts, it would double them, 590 us more on
+// 4096 x 4096 -> 11008.  The gradients behind an activation are then off by 0.0024 of their norm instead of the 0.0017 that
+// their own rounding makes.
 template <typename T, int ACT>
 __global__ __launch_bounds__(kBlock) void slope_kernel(const T* __restrict__ g, const Saved<T>* __restrict__ z,
                                                        int64_t rows, int64_t cols, int64_t ld, int64_t rows_per_slice,
@@ -421,7 +425,7 @@ int64_t max_slices(int64_t k)
 }
 
 // Whether a float32 product is formed from its operands as they lie (miq_direct.h) or from halves made beforehand
-// (miq_halves.h).  The first runs at about 160 TFLOP/s (130 on columns, whole tiles counted), the second at up to 490 once the halves are there; making them takes
+// (miq_halves.h).  The first runs at about 160 TFLOP/s (130 on columns, whole tiles counted), the second at up to 450 once the halves are there; making them takes
 // 2 ps a value of an operand in rows and 3 ps in columns (one more pass), and 18 us of launches, 15 more for each operand
 // in columns.  The rule is within 5 % of the better way on most of 90 measured products.  In us, as they lie and by halves:
 // [256, 4096] x [4096, 4096]^T 62 and 71, [512, 4096] x [4096, 4096]^T 106 and 93, the input's gradient of
@@ -460,7 +464,8 @@ struct Plan
 };
 
 // Tiles and pieces of the sum for a product of `slices` slices a pass whose values take `bytes`.  What a launch costs, in
-// us, as measured on many shapes (within 10 % for most): 5, and for each round of tiles that the device holds at a time
+// us, as measured on many shapes (within 10 % for most that are whole tiles and slices; others, whose loads are guarded, take up to
+// twice as long: 30 instead of 16 for [1021, 1003] x [1531, 1003]^T): 5, and for each round of tiles that the device holds at a time
 //   256 x 256, one a CU: 1.5 a slice, 1.25 when half of the CUs have none, and the result at 20 bytes a ns and CU
 //   128 x 128, two a CU: 1.05 a slice, 0.6 when there is one, and half of that, for one writes while the other sums
 // and to join the pieces 4 and 1 for each million of partial values.  E.g. bfloat16 [4096, 1024] x [1024, 1024]^T: 15 whole,

@@ -1,13 +1,17 @@
 """Layer norm and linear layers whose whole forward -- and whose backward -- is one call into the HIP kernels, as
 functions, as modules and as quantized modules.
 
-A quantized transformer block places one quantizer behind a supergroup ([Gemm, Relu] and the like in the reference's
-default_config.json) but runs its members as separate torch modules.  FusedLinear is such a group as one module: product,
-bias, activation and residual in one pass over the output, with one output quantizer behind it.  FusedLayerNorm is
-nn.LayerNorm on one pass over the input.  Both train: gradients of input, weight, bias and residual.
+FusedLinear is a linear layer, its activation and the addition of a residual as one module: one pass over the output, with
+one output quantizer behind it.  With ReLU that is what a configuration with the supergroup [Gemm, Relu] (the reference's
+default_config.json) has for the two modules.  With another activation or a residual it is fewer quantizers than
+separate modules get: nothing is quantized between the product, the activation and the sum.  A model whose target
+quantizes there keeps separate modules.  FusedLayerNorm is nn.LayerNorm on one pass over the input.  Both train: gradients of
+input, weight, bias and residual.
 
-float32 and bfloat16 tensors on the GPU; sums and statistics are float32; differentiable once.  Under torch.autocast the functions follow
-torch's own: linear() computes in the autocast type, layer_norm() in float32.
+float32 and bfloat16 tensors on the GPU; sums and statistics are float32; differentiable once.  In bfloat16 the gradient behind an
+activation is rounded on its way into the gradients of input and weight, as between two torch layers.  Under torch.autocast
+the functions follow torch's own: linear() computes in the autocast type, layer_norm() in float32.  torch.jit.trace records
+them as aimet_amd::linear and aimet_amd::layer_norm; make_fx, torch.export and functorch's transforms are refused.
 """
 from typing import Optional, Sequence
 

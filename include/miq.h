@@ -733,6 +733,7 @@ int miq_layer_norm_bwd_bf16(const uint16_t* x, const uint16_t* grad, const uint1
  * All tensors contiguous and of one type; in and out at most 2^27, rows below 2^31.  Sums are float32; z is rounded nowhere on its way to y, and y once.
  * A float32 sum of k terms is off by at most (k + 12) 2^-24 of the sum of its terms' magnitudes, whatever the range of the
  * values in a row (above 2^-109), and is the infinity or NaN that float32 arithmetic has.
+ * bfloat16: behind an activation dz is rounded to bfloat16 on its way into dx and dweight, not into dbias.
  * bias and residual may be NULL.  saved (NULL where no backward pass follows, or for MIQ_ACT_NONE): what the backward
  * pass needs of z, [rows, out], float for the f32 entry points and half for the bf16 ones.  dx, dweight, dbias may each
  * be NULL where that gradient is not wanted.
