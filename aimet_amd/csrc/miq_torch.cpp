@@ -85,6 +85,18 @@ void no_proxies()
                 "aimet_amd kernels cannot be recorded into a graph of torch's operators");
 }
 
+bool traced()
+{
+    return at::tracer::impl::is_dispatch_enabled();
+}
+
+// what neither make_fx nor torch.jit.trace may record: the backward passes, and the functions that give or take statistics
+void not_recorded()
+{
+    no_proxies();
+    TORCH_CHECK(!traced(), "only layer_norm() and linear() of aimet_amd are recorded by a trace, no backward pass and nothing below them");
+}
+
 bool is_bf16(const Tensor& x)
 {
     return x.scalar_type() == at::kBFloat16;
@@ -330,6 +342,7 @@ struct LayerNormNode : torch::autograd::Function<LayerNormNode>
 
     static variable_list backward(AutogradContext* ctx, variable_list grads)
     {
+        not_recorded();
         refuse_eager_leaves_under_capture();
         const bool twice = at::GradMode::is_enabled();
         variable_list out(5);
@@ -372,6 +385,7 @@ struct LinearNode : torch::autograd::Function<LinearNode>
 
     static variable_list backward(AutogradContext* ctx, variable_list grads)
     {
+        not_recorded();
         refuse_eager_leaves_under_capture();
         const bool twice = at::GradMode::is_enabled();
         variable_list out(6);
@@ -463,11 +477,6 @@ Tensor linear_operator(const Tensor& input, const Tensor& weight, const std::opt
     return linear(input, weight, bias.value_or(Tensor()), activation, residual.value_or(Tensor()));
 }
 
-bool traced()
-{
-    return at::tracer::impl::is_dispatch_enabled();
-}
-
 Tensor recorded_layer_norm(const Tensor& x, at::IntArrayRef shape, const Tensor& weight, const Tensor& bias, double eps)
 {
     static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("aimet_amd::layer_norm", "")
@@ -480,12 +489,6 @@ Tensor recorded_linear(const Tensor& x, const Tensor& weight, const Tensor& bias
     static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("aimet_amd::linear", "")
                                .typed<decltype(linear_operator)>();
     return op.call(x, weight, given(bias), activation, given(residual));
-}
-
-void not_recorded()
-{
-    no_proxies();
-    TORCH_CHECK(!traced(), "this function of aimet_amd is not recorded by a trace: call layer_norm() or linear()");
 }
 
 // ---------------------------------------------------------------------------------------------- Python's side of it

@@ -1002,6 +1002,23 @@ def test_graphs_of_torchs_operators_are_refused(fused):
             torch.func.grad(lambda t: f(t).sum())(x)           # pylint: disable=cell-var-from-loop
 
 
+def test_recording_a_backward_pass_is_refused(fused):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x, w, b, _, g = linear_case(4, 32, 32, torch.float32, False)
+    leaf = x.clone().requires_grad_()
+    for y in (fused.linear(leaf, w, b), fused.layer_norm(leaf, 32)):
+        want, = torch.autograd.grad(y, leaf, g, retain_graph=True)
+        with pytest.raises(RuntimeError, match="recorded"):
+            make_fx(lambda t: torch.autograd.grad(y, leaf, t, retain_graph=True)[0])(g)    # pylint: disable=cell-var-from-loop
+        assert torch.equal(torch.autograd.grad(y, leaf, g)[0], want)
+
+    def step(t):
+        return torch.autograd.grad(fused.linear(t, w, b).sum(), t)[0]   # (a trace takes no gradient from outside)
+
+    with pytest.raises(RuntimeError):
+        torch.jit.trace(step, leaf, check_trace=False)
+
+
 def test_modules_are_made_from_torch_modules_and_pickle(fused):
     import copy
     import pickle
